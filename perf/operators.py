@@ -379,7 +379,8 @@ def _run_own(st):
     stream = torch.cuda.current_stream().cuda_stream
     if "caches" not in st:  # the descriptors, and the attention's workspace
         if st["op"] == "accept":
-            st["caches"] = [_cache(lrs, st, k, v) for k, v in zip(st["pool_k"], st["pool_v"])]
+            caches = [_cache(lrs, st, k, v) for k, v in zip(st["pool_k"], st["pool_v"])]
+            st["caches"] = (lrs.KvCache * len(caches))(*caches)
         else:
             st["caches"] = [_cache(lrs, st, st["pool_k"], st["pool_v"])]
         if st["op"] == "tree":
