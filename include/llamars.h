@@ -178,7 +178,7 @@ typedef struct lrs_model_desc {
 } lrs_model_desc;
 
 /* KV-cache element type on the device. */
-enum { LRS_KV_F32 = 0, LRS_KV_BF16 = 1 };
+enum { LRS_KV_F32 = 0, LRS_KV_BF16 = 1, LRS_KV_Q8_0 = 2 };
 
 typedef struct lrs_model_options {
   uint32_t max_seq_len;   /* context per sequence (KVCache::new max_seq_len, src/cache.rs:12-36) */
@@ -270,6 +270,110 @@ lrs_status lrs_model_profile_step(lrs_model* model, size_t n_seqs, const uint32_
 /* Kernel launches in one decode step of the most recent decode_enqueue
  * (kernel nodes of its CUDA graph); 0 before the first graph-captured step. */
 uint32_t lrs_model_step_kernels(const lrs_model* model);
+
+/* ------------------------------------------- operators over a paged KV cache --
+ * No counterpart in the reference, whose KVCache (src/cache.rs:1-57) is one f32
+ * array per layer and sequence.  A cache here is two pools of pages and a page
+ * table, all in device memory that the caller owns; the models' caches have
+ * this form.  One page holds LRS_KV_PAGE positions of every KV head.
+ *
+ * Layout of the tile of one (page, KV head), tiles being [page][kv_head]:
+ *   LRS_KV_F32, LRS_KV_BF16: [LRS_KV_PAGE][head_dim] values.
+ *   LRS_KV_Q8_0: Q8_0 blocks (32 values of a row share an f16 scale d; a value
+ *     is d * code, code in -127..127), codes and scales in separate planes:
+ *     K: codes [head_dim/16][LRS_KV_PAGE][16], scales [LRS_KV_PAGE][head_dim/32];
+ *     V: codes [LRS_KV_PAGE/4][head_dim][4] (four positions of a column side by
+ *        side), scales [head_dim/32][LRS_KV_PAGE];
+ *     LRS_KV_PAGE * head_dim / 32 * 34 bytes, as many as the same GGML blocks.
+ *     Codes and scales are those of lrs_quantize_matrix(LRS_GGML_Q8_0) of the
+ *     row clamped to +-65024 (NaN as 0), so that every value held is a finite f16.
+ *
+ * All of these queue work on `stream` (a cudaStream_t; NULL = the backend's
+ * stream, cudaStreamLegacy names the default stream) of the backend's device
+ * and return without synchronizing; the calling thread's current device stays
+ * as it was.  They allocate nothing and can be captured into a CUDA graph.
+ * What device arrays hold (slots, positions, page numbers, node indices,
+ * lengths) is checked on the device: an entry out of range is skipped, nothing
+ * outside the pools and arrays is read or written, and the next
+ * lrs_backend_synchronize (after the work has finished) returns
+ * LRS_ERR_INVALID. */
+#define LRS_KV_PAGE 64
+#define LRS_TREE_MAX_NODES 64
+
+typedef struct lrs_kv_cache {
+  void* k_pool;         /* device, 16-byte aligned: n_pages * kv_heads tiles */
+  void* v_pool;
+  const int32_t* pages; /* device [n_seqs][max_pages]: page i of slot s holds its positions
+                           [i * LRS_KV_PAGE, (i + 1) * LRS_KV_PAGE) */
+  uint32_t n_pages, n_seqs, max_pages;
+  uint32_t kv_heads, head_dim; /* head_dim 64 or 128 */
+  uint32_t kv_dtype;           /* LRS_KV_* */
+} lrs_kv_cache;
+
+/* Checks a cache description (no CUDA call).  *tile_bytes (may be NULL) is the
+ * size of one (page, KV head) tile: a pool has n_pages * kv_heads of them. */
+lrs_status lrs_kv_check(const lrs_kv_cache* cache, size_t* tile_bytes);
+
+/* KVCache::update (src/cache.rs:38-53) for n rows, in the cache's type: row i of
+ * d_k and d_v (kv_heads * head_dim floats each, rows `ld` floats apart, 0 =
+ * packed; K already rotated) becomes position d_pos[i] of slot d_seq[i].  The
+ * positions of one call are distinct: which of two rows for one position
+ * stays is not defined. */
+lrs_status lrs_kv_store(lrs_backend* backend, const lrs_kv_cache* cache, const int32_t* d_seq,
+                        const int32_t* d_pos, size_t n, const float* d_k, const float* d_v,
+                        size_t ld, void* stream);
+
+/* The values that the cache holds, as f32: position d_pos[i] of slot d_seq[i]
+ * into row i of d_k and d_v (either may be NULL).  A row whose slot, position
+ * or page is out of range is left as it was. */
+lrs_status lrs_kv_load(lrs_backend* backend, const lrs_kv_cache* cache, const int32_t* d_seq,
+                       const int32_t* d_pos, size_t n, float* d_k, float* d_v, size_t ld,
+                       void* stream);
+
+/* Token trees, one per entry of `seq`: nodes start[t] .. start[t + 1] of the
+ * packed node arrays belong to tree t, which continues the ctx[t] committed
+ * positions of slot seq[t]; node j of a tree is held at position ctx[t] + j. */
+typedef struct lrs_tree_batch {
+  const int32_t* seq;   /* device [n_trees] */
+  const int32_t* ctx;   /* device [n_trees] committed positions (0 allowed) */
+  const int32_t* start; /* device [n_trees + 1], ascending from 0 to at most n_nodes */
+  const uint64_t* mask; /* device [n_nodes]: bit j of a node's mask = it attends to node j of
+                           its tree (its ancestors and itself); NULL = chains (bits 0..i) */
+  uint32_t n_trees;
+  uint32_t n_nodes;   /* rows of the node arrays */
+  uint32_t max_nodes; /* no tree has more nodes; at most LRS_TREE_MAX_NODES */
+  uint32_t max_len;   /* no tree has ctx + nodes above this; at most max_pages * LRS_KV_PAGE */
+} lrs_tree_batch;
+
+/* Attention of every node to its slot's committed positions and to the nodes
+ * of its mask, all of them in the cache already (lrs_kv_store):
+ *   out[i][h] = sum_p softmax_p(scale * q[i][h] . K[p][h / G]) V[p][h / G],
+ * G = n_heads / kv_heads (at most 64), q and out f32 rows of n_heads * head_dim
+ * (q_ld, out_ld floats apart, 0 = packed), q already rotated.  A node that
+ * attends to nothing gets zeros; rows from start[n_trees] on are left as they
+ * were.  What a node's mask leaves out does not reach its output, be it NaN or
+ * infinite; a non-finite value that it does attend to makes its outputs
+ * non-finite (all of the row's, if the value belongs to another node).
+ * `d_workspace` (16-byte aligned, lrs_tree_attention_workspace bytes, contents
+ * free) is in use until the work has finished: calls that may overlap, and
+ * graphs that may run at once, need one each. */
+lrs_status lrs_tree_attention_workspace(const lrs_backend* backend, const lrs_kv_cache* cache,
+                                        const lrs_tree_batch* trees, uint32_t n_heads,
+                                        size_t* bytes);
+lrs_status lrs_tree_attention(lrs_backend* backend, const lrs_kv_cache* cache,
+                              const lrs_tree_batch* trees, const float* d_q, size_t q_ld,
+                              float* d_out, size_t out_ld, uint32_t n_heads, float scale,
+                              void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* Keeps one path of each tree: node d_nodes[d_start[t] + j] of tree t, held at
+ * position d_ctx[t] + d_nodes[..], moves to position d_ctx[t] + j, in each of the
+ * n_caches caches (the layers of a model: equal but for their pools).  A path's
+ * nodes ascend, all below LRS_TREE_MAX_NODES; a tree whose path does not, or
+ * leaves the slot's pages, is left as it was.  d_start is [n_trees + 1],
+ * ascending from 0 to at most n_nodes; the slots of one call are distinct. */
+lrs_status lrs_kv_accept(lrs_backend* backend, const lrs_kv_cache* caches, size_t n_caches,
+                         const int32_t* d_seq, const int32_t* d_ctx, const int32_t* d_start,
+                         const int32_t* d_nodes, size_t n_trees, size_t n_nodes, void* stream);
 
 /* Device stream (cudaStream_t) the model and backend queue work on. */
 void* lrs_backend_stream(lrs_backend* backend);

@@ -153,6 +153,44 @@ class Sampler(C.Structure):
         super().__init__(temperature, top_p, top_k, repetition_penalty)
 
 
+class KvType(enum.IntEnum):
+    """KV-cache element types (LRS_KV_*)."""
+
+    F32 = 0
+    BF16 = 1
+    Q8_0 = 2
+
+
+#: LRS_KV_PAGE: positions a page of the KV cache holds
+KV_PAGE = 64
+#: LRS_TREE_MAX_NODES: the most nodes of one token tree
+TREE_MAX_NODES = 64
+
+
+class KvCache(C.Structure):
+    """A paged KV cache in device memory that the caller owns (lrs_kv_cache):
+    device addresses of the two pools and of the page table [n_seqs][max_pages]
+    of int32, and their sizes."""
+    _fields_ = [("k_pool", C.c_void_p), ("v_pool", C.c_void_p), ("pages", C.c_void_p),
+                ("n_pages", C.c_uint32), ("n_seqs", C.c_uint32), ("max_pages", C.c_uint32),
+                ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("kv_dtype", C.c_uint32)]
+
+    def tile_bytes(self) -> int:
+        """Bytes of one (page, KV head) tile, after the checks of lrs_kv_check."""
+        n = C.c_size_t()
+        _check(_lib.lrs_kv_check(C.byref(self), C.byref(n)))
+        return n.value
+
+
+class TreeBatch(C.Structure):
+    """Token trees over a cache (lrs_tree_batch): device addresses of the int32
+    arrays seq, ctx [n_trees] and start [n_trees + 1], and of the uint64 masks
+    [n_nodes] (None = chains)."""
+    _fields_ = [("seq", C.c_void_p), ("ctx", C.c_void_p), ("start", C.c_void_p),
+                ("mask", C.c_void_p), ("n_trees", C.c_uint32), ("n_nodes", C.c_uint32),
+                ("max_nodes", C.c_uint32), ("max_len", C.c_uint32)]
+
+
 #: LRS_SAMPLE_MAX_TOP_K: the largest top_k the device sampler takes
 SAMPLE_MAX_TOP_K = 4096
 
@@ -236,6 +274,16 @@ _sig("lrs_sample_logits", C.c_int32, _P, C.c_void_p, C.c_size_t, C.POINTER(Sampl
 _sig("lrs_model_forward_sample", C.c_int32, _P, C.c_uint32, C.c_uint32, C.c_uint32,
      C.POINTER(Sampler), _U32, C.c_size_t, C.c_float, _U32)
 
+_KV = C.POINTER(KvCache)
+_sig("lrs_kv_check", C.c_int32, _KV, C.POINTER(C.c_size_t))
+_sig("lrs_kv_store", C.c_int32, _P, _KV, _P, _P, C.c_size_t, _P, _P, C.c_size_t, _P)
+_sig("lrs_kv_load", C.c_int32, _P, _KV, _P, _P, C.c_size_t, _P, _P, C.c_size_t, _P)
+_sig("lrs_kv_accept", C.c_int32, _P, _KV, C.c_size_t, _P, _P, _P, _P, C.c_size_t, C.c_size_t, _P)
+_sig("lrs_tree_attention_workspace", C.c_int32, _P, _KV, C.POINTER(TreeBatch), C.c_uint32,
+     C.POINTER(C.c_size_t))
+_sig("lrs_tree_attention", C.c_int32, _P, _KV, C.POINTER(TreeBatch), _P, C.c_size_t, _P,
+     C.c_size_t, C.c_uint32, C.c_float, _P, C.c_size_t, _P)
+
 #: every symbol include/*.h declares (checked by the CPU tests)
 EXPORTED_SYMBOLS = (
     "lrs_last_error", "lrs_type_geometry", "lrs_backend_create", "lrs_backend_destroy",
@@ -254,12 +302,21 @@ EXPORTED_SYMBOLS = (
     "lrs_sampler_check", "lrs_sample_logits", "lrs_model_forward_sample",
     "lrs_st_open", "lrs_st_close", "lrs_st_tensor_count", "lrs_st_tensor", "lrs_st_qwen2_desc",
     "lrs_model_load", "lrs_loaded_close",
+    "lrs_kv_check", "lrs_kv_store", "lrs_kv_load", "lrs_kv_accept",
+    "lrs_tree_attention_workspace", "lrs_tree_attention",
 )
 
 
 def _check(code: int) -> None:
     if code != 0:
         raise LrsError(code, (_lib.lrs_last_error() or b"").decode(errors="replace"))
+
+
+def _cuda_stream(stream: Optional[int]) -> Optional[int]:
+    """A cudaStream_t for the C ABI, where NULL is the backend's stream: None
+    stays that, and 0, the default stream's handle elsewhere, becomes
+    cudaStreamLegacy."""
+    return 1 if stream == 0 else stream
 
 
 def _fptr(a: np.ndarray):
@@ -475,6 +532,47 @@ class CudaBackend:
         _check(_lib.lrs_quantize_matrix_device(self._h, int(quant_type), d_values, rows, cols, d_out,
                                                out_cap, _uptr(t), C.byref(n)))
         return QuantType(int(t[0])), n.value
+
+    def kv_store(self, cache: KvCache, d_seq: int, d_pos: int, n: int, d_k: int, d_v: int,
+                 ld: int = 0, stream: Optional[int] = None) -> None:
+        """Queues the write of n rows of K and V into the cache, in its type
+        (lrs_kv_store); device addresses, no synchronization."""
+        _check(_lib.lrs_kv_store(self._h, cache, d_seq, d_pos, n, d_k, d_v, ld,
+                                 _cuda_stream(stream)))
+
+    def kv_load(self, cache: KvCache, d_seq: int, d_pos: int, n: int, d_k: Optional[int],
+                d_v: Optional[int], ld: int = 0, stream: Optional[int] = None) -> None:
+        """Queues the read of n rows of the cache as f32 values (lrs_kv_load)."""
+        _check(_lib.lrs_kv_load(self._h, cache, d_seq, d_pos, n, d_k, d_v, ld,
+                                _cuda_stream(stream)))
+
+    def kv_accept(self, caches, d_seq: int, d_ctx: int, d_start: int, d_nodes: int, n_trees: int,
+                  n_nodes: int, stream: Optional[int] = None) -> None:
+        """Queues the moves that keep one path of each tree, in all `caches` (a
+        KvCache, or a list or ctypes array of them; lrs_kv_accept)."""
+        if isinstance(caches, KvCache):
+            caches = (KvCache * 1)(caches)
+        elif not isinstance(caches, C.Array):
+            caches = (KvCache * len(caches))(*caches)
+        _check(_lib.lrs_kv_accept(self._h, caches, len(caches), d_seq, d_ctx, d_start, d_nodes,
+                                  n_trees, n_nodes, _cuda_stream(stream)))
+
+    def tree_attention_workspace(self, cache: KvCache, trees: TreeBatch, n_heads: int) -> int:
+        """Bytes of workspace tree_attention needs (lrs_tree_attention_workspace)."""
+        n = C.c_size_t()
+        _check(_lib.lrs_tree_attention_workspace(self._h, cache, trees, n_heads, C.byref(n)))
+        return n.value
+
+    def tree_attention(self, cache: KvCache, trees: TreeBatch, d_q: int, d_out: int, n_heads: int,
+                       scale: Optional[float] = None, q_ld: int = 0, out_ld: int = 0,
+                       d_workspace: Optional[int] = None, workspace_bytes: int = 0,
+                       stream: Optional[int] = None) -> None:
+        """Queues the attention of the trees' nodes over the cache
+        (lrs_tree_attention); scale defaults to 1 / sqrt(head_dim)."""
+        if scale is None:
+            scale = max(1, cache.head_dim) ** -0.5
+        _check(_lib.lrs_tree_attention(self._h, cache, trees, d_q, q_ld, d_out, out_ld, n_heads,
+                                       scale, d_workspace, workspace_bytes, _cuda_stream(stream)))
 
     def dequantize_rows(self, weight: QuantTensor, row0: int, nrows: int) -> np.ndarray:
         """value_at for rows [row0, row0 + nrows) (QuantTensor::row_into)."""

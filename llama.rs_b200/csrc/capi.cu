@@ -23,6 +23,7 @@
 #include "decode.cuh"
 #include "gemv.cuh"
 #include "internal.h"
+#include "kv.cuh"
 #include "sample.cuh"
 #include "step1.cuh"
 #include "tp_p2p.cuh"
@@ -99,6 +100,9 @@ int32_t check_device_error(lrs_backend* be) {
   LRS_CUDA(cudaMemcpy(&h, be->d_err, sizeof(int), cudaMemcpyDeviceToHost));
   if (h) {
     cudaMemset(be->d_err, 0, sizeof(int));
+    if (h == kErrCacheIndex)
+      return fail(LRS_ERR_INVALID,
+                  "a KV cache operator skipped a slot, position, page, node or length out of range");
     return fail(LRS_ERR_DEVICE_TIMEOUT, "a bounded device-side wait gave up (TMA copy not completed)");
   }
   return LRS_OK;

@@ -1,0 +1,98 @@
+// kv.cuh -- the paged KV cache as the operators of kv_ops.cu and
+// tree_attention.cu see it (layout: lrs_kv_cache in include/llamars.h).
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/llamars.h"
+#include "decode.cuh"
+
+namespace lrs {
+
+static_assert(kPageSize == LRS_KV_PAGE, "one page size");
+
+// What the error word (lrs_backend::d_err) holds after a kernel skipped an
+// entry that names a slot, position, page or node out of range.
+constexpr int kErrCacheIndex = 2;
+
+// Largest magnitude of a Q8_0 cache: 512 * 127, so that d * code is a finite f16.
+constexpr float kQ8Limit = 65024.0f;
+
+__host__ __device__ constexpr size_t kv_tile_bytes(uint32_t dtype, int hd) {
+  return dtype == LRS_KV_Q8_0 ? (size_t)kPageSize * (hd / 32) * 34
+                              : (size_t)kPageSize * hd * (dtype == LRS_KV_BF16 ? 2 : 4);
+}
+// Byte offsets inside a Q8_0 tile (row r of the page, column c of the head).
+__host__ __device__ constexpr int q8_k_code(int r, int c) { return (c / 16 * kPageSize + r) * 16 + c % 16; }
+__host__ __device__ constexpr int q8_k_scale(int hd, int r, int b) {
+  return kPageSize * hd + (r * (hd / 32) + b) * 2;
+}
+__host__ __device__ constexpr int q8_v_code(int hd, int r, int c) { return (r / 4 * hd + c) * 4 + r % 4; }
+__host__ __device__ constexpr int q8_v_scale(int hd, int r, int b) {
+  return kPageSize * hd + (b * kPageSize + r) * 2;
+}
+
+struct KvView {
+  uint8_t* k;
+  uint8_t* v;
+  const int* pages;
+  int n_pages, n_seqs, max_pages, heads;
+  int* err;
+};
+
+// Physical page of position `pos` of slot `seq`, or -1 (with the error word
+// set) if any of the three is out of range.
+__device__ __forceinline__ int kv_page(const KvView& c, int seq, int pos) {
+  int page = -1;
+  if (seq >= 0 && seq < c.n_seqs && pos >= 0 && pos / kPageSize < c.max_pages)
+    page = c.pages[(size_t)seq * c.max_pages + pos / kPageSize];
+  if (page < 0 || page >= c.n_pages) {
+    atomicExch(c.err, kErrCacheIndex);
+    return -1;
+  }
+  return page;
+}
+
+// Rows (store: after RoPE of q and k when cos_t is given; rope_pos: positions
+// of the rotation, NULL = pos) and their slots and positions.
+struct KvStoreArgs {
+  KvView c;
+  const int* seq;
+  const int* pos;
+  long long n;
+  const float* k;
+  const float* v;
+  long long ld;
+};
+cudaError_t launch_kv_store(const KvStoreArgs& a, uint32_t dtype, int hd, int sms, cudaStream_t st);
+
+struct KvLoadArgs {
+  KvView c;
+  const int* seq;
+  const int* pos;
+  long long n;
+  float* k;
+  float* v;
+  long long ld;
+};
+cudaError_t launch_kv_load(const KvLoadArgs& a, uint32_t dtype, int hd, cudaStream_t st);
+
+struct TreeArgs {
+  KvView c;
+  const int* seq;
+  const int* ctx;
+  const int* start;
+  const unsigned long long* mask;
+  int n_trees, n_nodes, max_nodes, max_len;
+  const float* q;
+  float* out;
+  long long q_ld, out_ld;
+  int group;      // query heads per KV head
+  float scale;
+  void* workspace;
+};
+size_t tree_attention_workspace_bytes(const TreeArgs& a, int hd, int sms);
+cudaError_t launch_tree_attention(const TreeArgs& a, uint32_t dtype, int hd, int sms,
+                                  cudaStream_t st);
+
+}  // namespace lrs

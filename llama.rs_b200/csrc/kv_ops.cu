@@ -1,0 +1,616 @@
+// kv_ops.cu -- writing, reading back and compacting the paged KV cache in its
+// own type, and the C entry points of these operators and of the tree
+// attention (tree_attention.cu).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <string>
+
+#include "common.h"
+#include "device_common.cuh"
+#include "internal.h"
+#include "kv.cuh"
+
+namespace lrs {
+namespace {
+
+constexpr int kStoreWarps = 4;
+constexpr int kStoreRows = 32;  // most rows a CTA of the store kernel
+
+__device__ __forceinline__ float4 load4(const float* p, bool vec) {
+  if (vec) return *reinterpret_cast<const float4*>(p);
+  return make_float4(p[0], p[1], p[2], p[3]);
+}
+
+// The Q8_0 code of x under inv = 1 / d (quantize_block_q8_0, src/quant.rs:650-662:
+// f32 product, round half away from zero, clamp; NaN, which 0 * inf gives for
+// blocks of f32 subnormals, becomes 0).
+__device__ __forceinline__ uint32_t q8_code(float x, float inv) {
+  const float r = roundf(__fmul_rn(x, inv));
+  const int i = r != r ? 0 : (int)fminf(fmaxf(r, -127.0f), 127.0f);
+  return (uint32_t)i & 0xffu;
+}
+
+// Rows [blockIdx.x * rows, + rows) of K (blockIdx.z = 0) or V (1) of head
+// blockIdx.y.  A lane owns four consecutive columns.  Q8_0: eight lanes share a
+// block's maximum by shuffles; K codes go out as words.  V interleaves four
+// positions per word, so the codes of the CTA's rows meet in shared memory and
+// leave as 16-byte stores wherever four consecutive rows are four aligned
+// positions of one slot, and as single bytes elsewhere (a decode step's rows,
+// the ends of a run): byte stores never touch a neighbouring position.
+template <int HD, int DT>
+__global__ void __launch_bounds__(32 * kStoreWarps)
+    kv_store_kernel(const __grid_constant__ KvStoreArgs a, int rows, bool vec) {
+  constexpr int LPR = HD / 4, RPW = 32 / LPR;  // lanes a row, rows a warp
+  __shared__ uint32_t codes[kStoreRows][LPR];
+  __shared__ int row_page[kStoreRows], row_seq[kStoreRows], row_pos[kStoreRows];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int head = blockIdx.y;
+  const bool is_v = blockIdx.z != 0;
+  const long long i0 = (long long)blockIdx.x * rows;
+  const int cnt = (int)min((long long)rows, a.n - i0);
+  const float* src = is_v ? a.v : a.k;
+  uint8_t* pool = is_v ? a.c.v : a.c.k;
+  constexpr size_t TILE = kv_tile_bytes(DT, HD);
+  const int col = (lane % LPR) * 4;
+  for (int r0 = warp * RPW; r0 < cnt; r0 += kStoreWarps * RPW) {
+    const int r = r0 + lane / LPR;
+    const bool live = r < cnt;
+    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    int page = -1, pos = 0, seq = 0;
+    if (live) {
+      pos = a.pos[i0 + r];
+      seq = a.seq[i0 + r];
+      const float4 f = load4(src + (size_t)(i0 + r) * a.ld + (size_t)head * HD + col, vec);
+      x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+      page = kv_page(a.c, seq, pos);
+    }
+    const int pr = pos & (kPageSize - 1);
+    uint8_t* tile = pool + ((size_t)max(page, 0) * a.c.heads + head) * TILE;
+    if constexpr (DT == LRS_KV_F32) {
+      if (page >= 0)
+        *reinterpret_cast<float4*>(tile + ((size_t)pr * HD + col) * 4) =
+            make_float4(x[0], x[1], x[2], x[3]);
+    } else if constexpr (DT == LRS_KV_BF16) {
+      if (page >= 0) {
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(x[0], x[1]), hi = __floats2bfloat162_rn(x[2], x[3]);
+        *reinterpret_cast<uint2*>(tile + ((size_t)pr * HD + col) * 2) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+      }
+    } else {
+      float m = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        x[i] = x[i] != x[i] ? 0.0f : fminf(fmaxf(x[i], -kQ8Limit), kQ8Limit);
+        m = fmaxf(m, fabsf(x[i]));
+      }
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const float d = __fdiv_rn(m, 127.0f);
+      const float inv = d == 0.0f ? 0.0f : __fdiv_rn(1.0f, d);
+      uint32_t w = 0;
+#pragma unroll
+      for (int i = 0; i < 4; i++) w |= q8_code(x[i], inv) << (8 * i);
+      const int b = col / 32;
+      if (page >= 0) {
+        if ((lane & 7) == 0)
+          *reinterpret_cast<__half*>(tile + (is_v ? q8_v_scale(HD, pr, b) : q8_k_scale(HD, pr, b))) =
+              __float2half_rn(d);
+        if (!is_v) *reinterpret_cast<uint32_t*>(tile + q8_k_code(pr, col)) = w;
+      }
+      if (is_v && live) {
+        codes[r][lane % LPR] = w;
+        if (lane % LPR == 0) {
+          row_page[r] = page;
+          row_seq[r] = seq;
+          row_pos[r] = pos;
+        }
+      }
+    }
+  }
+  if constexpr (DT == LRS_KV_Q8_0) {
+    if (!is_v) return;
+    __syncthreads();
+    for (int r0 = warp * RPW; r0 < cnt; r0 += kStoreWarps * RPW) {
+      const int r = r0 + lane / LPR;
+      if (r >= cnt || row_page[r] < 0) continue;
+      const int pos = row_pos[r], g = r - (pos & 3);  // first row of the aligned group
+      bool full = g >= 0 && g + 3 < cnt;
+      for (int i = 0; i < 4 && full; i++)
+        full = row_seq[g + i] == row_seq[r] && row_pos[g + i] == (pos & ~3) + i;
+      if (full && g != r) continue;  // row g writes the group
+      const int pr = pos & (kPageSize - 1);
+      uint8_t* tile = pool + ((size_t)row_page[r] * a.c.heads + head) * TILE;
+      if (full) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[i] = codes[g + i][lane % LPR];
+        const uint32_t a0 = __byte_perm(w[0], w[1], 0x5140), a1 = __byte_perm(w[2], w[3], 0x5140);
+        const uint32_t b0 = __byte_perm(w[0], w[1], 0x7362), b1 = __byte_perm(w[2], w[3], 0x7362);
+        *reinterpret_cast<uint4*>(tile + q8_v_code(HD, pr, col)) =
+            make_uint4(__byte_perm(a0, a1, 0x5410), __byte_perm(a0, a1, 0x7632),
+                       __byte_perm(b0, b1, 0x5410), __byte_perm(b0, b1, 0x7632));
+      } else {
+        const uint32_t w = codes[r][lane % LPR];
+#pragma unroll
+        for (int i = 0; i < 4; i++) tile[q8_v_code(HD, pr, col + i)] = (uint8_t)(w >> (8 * i));
+      }
+    }
+  }
+}
+
+// The inverse: a lane owns four columns of a row; rows of a CTA are
+// consecutive, so the lines that four positions share (V codes, K's 16-byte
+// chunks) are read from L2 once.
+template <int HD, int DT>
+__global__ void __launch_bounds__(128)
+    kv_load_kernel(const __grid_constant__ KvLoadArgs a, bool vec) {
+  constexpr int LPR = HD / 4, RPC = 128 / LPR;
+  const int head = blockIdx.y;
+  const bool is_v = blockIdx.z != 0;
+  float* dst = is_v ? a.v : a.k;
+  const long long i = (long long)blockIdx.x * RPC + threadIdx.x / LPR;
+  if (!dst || i >= a.n) return;
+  const int col = (threadIdx.x % LPR) * 4;
+  const int pos = a.pos[i], page = kv_page(a.c, a.seq[i], pos);
+  if (page < 0) return;
+  const int pr = pos & (kPageSize - 1);
+  const uint8_t* tile =
+      (is_v ? a.c.v : a.c.k) + ((size_t)page * a.c.heads + head) * kv_tile_bytes(DT, HD);
+  float x[4];
+  if constexpr (DT == LRS_KV_F32) {
+    const float4 f = *reinterpret_cast<const float4*>(tile + ((size_t)pr * HD + col) * 4);
+    x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+  } else if constexpr (DT == LRS_KV_BF16) {
+    const uint2 u = *reinterpret_cast<const uint2*>(tile + ((size_t)pr * HD + col) * 2);
+    x[0] = __uint_as_float(u.x << 16), x[1] = __uint_as_float(u.x & 0xffff0000u);
+    x[2] = __uint_as_float(u.y << 16), x[3] = __uint_as_float(u.y & 0xffff0000u);
+  } else if (is_v) {
+    const uint4 u = *reinterpret_cast<const uint4*>(tile + q8_v_code(HD, pr & ~3, col));
+    const float d = __half2float(*reinterpret_cast<const __half*>(tile + q8_v_scale(HD, pr, col / 32)));
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 4; j++) x[j] = __fmul_rn(d, (float)(int8_t)(w[j] >> (8 * (pr & 3))));
+  } else {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(tile + q8_k_code(pr, col));
+    const float d = __half2float(*reinterpret_cast<const __half*>(tile + q8_k_scale(HD, pr, col / 32)));
+#pragma unroll
+    for (int j = 0; j < 4; j++) x[j] = __fmul_rn(d, (float)(int8_t)(w >> (8 * j)));
+  }
+  float* o = dst + (size_t)i * a.ld + (size_t)head * HD + col;
+  if (vec)
+    *reinterpret_cast<float4*>(o) = make_float4(x[0], x[1], x[2], x[3]);
+  else
+    for (int j = 0; j < 4; j++) o[j] = x[j];
+}
+
+// ---- accept ---------------------------------------------------------------
+constexpr int kAcceptCaches = 128;  // pools in one launch's parameters
+
+struct AcceptArgs {
+  KvView c;  // pools unused
+  uint8_t* k[kAcceptCaches];
+  uint8_t* v[kAcceptCaches];
+  int n_caches;
+  const int* seq;
+  const int* ctx;
+  const int* start;
+  const int* nodes;
+  int n_trees, n_nodes;
+};
+
+// One warp moves the path's rows of one (tree, cache, head, K or V).  The path
+// ascends, so row j's target ctx + j is at or below its source and below every
+// later source: rows move in chunks, each chunk read whole before it is
+// written, and no chunk overwrites a row that a later one reads.
+template <int HD, int DT>
+__global__ void __launch_bounds__(128) kv_accept_kernel(const __grid_constant__ AcceptArgs a) {
+  const int lane = threadIdx.x & 31;
+  long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const bool is_v = item & 1;
+  item >>= 1;
+  const int head = (int)(item % a.c.heads);
+  item /= a.c.heads;
+  const int cache = (int)(item % a.n_caches), t = (int)(item / a.n_caches);
+  if (t >= a.n_trees) return;
+  const int s = a.start[t], n = a.start[t + 1] - s, ctx = a.ctx[t], seq = a.seq[t];
+  if (n == 0) return;
+  bool ok = s >= 0 && n > 0 && n <= LRS_TREE_MAX_NODES && s + n <= a.n_nodes && seq >= 0 &&
+            seq < a.c.n_seqs && ctx >= 0 &&
+            ctx <= (int)min((long long)a.c.max_pages * kPageSize, (long long)INT_MAX) - 1;
+  int node0 = -1, node1 = -1;  // of rows `lane` and `lane + 32`
+  if (ok) {
+    if (lane < n) node0 = a.nodes[s + lane];
+    if (lane + 32 < n) node1 = a.nodes[s + lane + 32];
+  }
+  const int prev0 = __shfl_up_sync(0xffffffffu, node0, 1), top0 = __shfl_sync(0xffffffffu, node0, 31);
+  int prev1 = __shfl_up_sync(0xffffffffu, node1, 1);
+  if (lane == 0) prev1 = top0;
+  if (lane < n) ok = ok && node0 >= 0 && node0 < LRS_TREE_MAX_NODES && (lane == 0 || node0 > prev0);
+  if (lane + 32 < n) ok = ok && node1 < LRS_TREE_MAX_NODES && node1 > prev1;
+  ok = __all_sync(0xffffffffu, ok);
+  int page0 = -1, page1 = -1;  // of ctx, and of the page after it
+  if (ok) {
+    const int last = __reduce_max_sync(0xffffffffu, max(node0, node1));
+    page0 = kv_page(a.c, seq, ctx);
+    ok = page0 >= 0;
+    if (ok && ctx % kPageSize + last >= kPageSize) {
+      page1 = kv_page(a.c, seq, ctx - ctx % kPageSize + kPageSize);
+      ok = page1 >= 0;
+    }
+  }
+  if (!ok) {
+    if (lane == 0) atomicExch(a.c.err, kErrCacheIndex);
+    return;
+  }
+  uint8_t* pool = is_v ? a.v[cache] : a.k[cache];
+  constexpr size_t TILE = kv_tile_bytes(DT, HD);
+  // row at `off` positions past ctx: its tile and its row in the page
+  auto cell = [&](int off, int* r) {
+    const int p = ctx % kPageSize + off;
+    *r = p & (kPageSize - 1);
+    return pool + ((size_t)(p < kPageSize ? page0 : page1) * a.c.heads + head) * TILE;
+  };
+  auto node_of = [&](int j) {
+    const int lo = __shfl_sync(0xffffffffu, node0, j & 31), hi = __shfl_sync(0xffffffffu, node1, j & 31);
+    return j < 32 ? lo : hi;
+  };
+  if constexpr (DT != LRS_KV_Q8_0) {
+    constexpr int ROWB = HD * (DT == LRS_KV_BF16 ? 2 : 4), VPR = ROWB / 16;  // vectors a row
+    constexpr int CH = 8;                                                    // vectors a lane
+    for (int v0 = 0; v0 < n * VPR; v0 += 32 * CH) {
+      uint4 x[CH];
+#pragma unroll
+      for (int c = 0; c < CH; c++) {
+        const int e = v0 + 32 * c + lane, j = min(e / VPR, n - 1);
+        int r;
+        const uint8_t* t0 = cell(node_of(j), &r);
+        if (e < n * VPR) x[c] = *reinterpret_cast<const uint4*>(t0 + (size_t)r * ROWB + e % VPR * 16);
+      }
+      __syncwarp();
+#pragma unroll
+      for (int c = 0; c < CH; c++) {
+        const int e = v0 + 32 * c + lane;
+        int r;
+        uint8_t* t1 = cell(e / VPR, &r);
+        if (e < n * VPR) *reinterpret_cast<uint4*>(t1 + (size_t)r * ROWB + e % VPR * 16) = x[c];
+      }
+      __syncwarp();
+    }
+  } else {
+    constexpr int WPR = HD / 4, BPR = HD / 32;  // words of codes, scales of a row
+    constexpr int CH = 8;
+    for (int v0 = 0; v0 < n * WPR; v0 += 32 * CH) {
+      uint32_t x[CH];
+#pragma unroll
+      for (int c = 0; c < CH; c++) {
+        const int e = v0 + 32 * c + lane, j = min(e / WPR, n - 1), col = e % WPR * 4;
+        int r;
+        const uint8_t* t0 = cell(node_of(j), &r);
+        if (e < n * WPR) {
+          if (is_v) {
+            x[c] = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[c] |= (uint32_t)t0[q8_v_code(HD, r, col + i)] << (8 * i);
+          } else {
+            x[c] = *reinterpret_cast<const uint32_t*>(t0 + q8_k_code(r, col));
+          }
+        }
+      }
+      __syncwarp();
+#pragma unroll
+      for (int c = 0; c < CH; c++) {
+        const int e = v0 + 32 * c + lane, col = e % WPR * 4;
+        int r;
+        uint8_t* t1 = cell(e / WPR, &r);
+        if (e < n * WPR) {
+          if (is_v) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) t1[q8_v_code(HD, r, col + i)] = (uint8_t)(x[c] >> (8 * i));
+          } else {
+            *reinterpret_cast<uint32_t*>(t1 + q8_k_code(r, col)) = x[c];
+          }
+        }
+      }
+      __syncwarp();
+    }
+    for (int v0 = 0; v0 < n * BPR; v0 += 32) {  // the scales: whole rows per pass
+      const int e = v0 + lane, j = min(e / BPR, n - 1), b = e % BPR;
+      int r;
+      const uint8_t* t0 = cell(node_of(j), &r);
+      uint16_t d = 0;
+      if (e < n * BPR)
+        d = *reinterpret_cast<const uint16_t*>(t0 + (is_v ? q8_v_scale(HD, r, b) : q8_k_scale(HD, r, b)));
+      __syncwarp();
+      uint8_t* t1 = cell(j, &r);
+      if (e < n * BPR)
+        *reinterpret_cast<uint16_t*>(t1 + (is_v ? q8_v_scale(HD, r, b) : q8_k_scale(HD, r, b))) = d;
+      __syncwarp();
+    }
+  }
+}
+
+// Calls f<HD, DT>() of the cache's head_dim and type.
+#define LRS_KV_DISPATCH(hd, dtype, CALL)                                      \
+  do {                                                                        \
+    if ((hd) == 128) {                                                        \
+      if ((dtype) == LRS_KV_F32) { CALL(128, LRS_KV_F32); }                   \
+      else if ((dtype) == LRS_KV_BF16) { CALL(128, LRS_KV_BF16); }            \
+      else { CALL(128, LRS_KV_Q8_0); }                                        \
+    } else {                                                                  \
+      if ((dtype) == LRS_KV_F32) { CALL(64, LRS_KV_F32); }                    \
+      else if ((dtype) == LRS_KV_BF16) { CALL(64, LRS_KV_BF16); }             \
+      else { CALL(64, LRS_KV_Q8_0); }                                         \
+    }                                                                         \
+  } while (0)
+
+}  // namespace
+
+cudaError_t launch_kv_store(const KvStoreArgs& a, uint32_t dtype, int hd, int sms, cudaStream_t st) {
+  // few rows: four a CTA, so that the step's rows spread over the SMs
+  const long long big = (a.n + kStoreRows - 1) / kStoreRows * a.c.heads * 2;
+  const int rows = big >= 4ll * sms ? kStoreRows : 4;
+  const bool vec = a.ld % 4 == 0 && reinterpret_cast<uintptr_t>(a.k) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(a.v) % 16 == 0;
+  const dim3 grid((unsigned)((a.n + rows - 1) / rows), a.c.heads, 2);
+#define LRS_CALL(HD, DT) kv_store_kernel<HD, DT><<<grid, 32 * kStoreWarps, 0, st>>>(a, rows, vec)
+  LRS_KV_DISPATCH(hd, dtype, LRS_CALL);
+#undef LRS_CALL
+  return cudaGetLastError();
+}
+
+cudaError_t launch_kv_load(const KvLoadArgs& a, uint32_t dtype, int hd, cudaStream_t st) {
+  const int rpc = 512 / hd;
+  const bool vec = a.ld % 4 == 0 && reinterpret_cast<uintptr_t>(a.k) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(a.v) % 16 == 0;
+  const dim3 grid((unsigned)((a.n + rpc - 1) / rpc), a.c.heads, 2);
+#define LRS_CALL(HD, DT) kv_load_kernel<HD, DT><<<grid, 128, 0, st>>>(a, vec)
+  LRS_KV_DISPATCH(hd, dtype, LRS_CALL);
+#undef LRS_CALL
+  return cudaGetLastError();
+}
+
+}  // namespace lrs
+
+using namespace lrs;
+
+namespace {
+
+// The backend's device for the length of a call.
+class OnDevice {
+ public:
+  explicit OnDevice(int device) {
+    err = cudaGetDevice(&was_);
+    if (err == cudaSuccess && was_ != device) {
+      err = cudaSetDevice(device);
+      moved_ = err == cudaSuccess;
+    }
+  }
+  ~OnDevice() {
+    if (moved_) cudaSetDevice(was_);
+  }
+  cudaError_t err;
+
+ private:
+  int was_ = 0;
+  bool moved_ = false;
+};
+
+int32_t cuda_status(cudaError_t e, const char* what) {
+  return e == cudaSuccess ? (int32_t)LRS_OK
+                          : fail(LRS_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+}
+
+KvView view_of(const lrs_kv_cache& c, int* err) {
+  return KvView{static_cast<uint8_t*>(c.k_pool), static_cast<uint8_t*>(c.v_pool), c.pages,
+                (int)c.n_pages, (int)c.n_seqs, (int)c.max_pages, (int)c.kv_heads, err};
+}
+
+int32_t check_rows(const lrs_kv_cache* c, size_t n, size_t* ld, const char* what) {
+  int32_t rc = lrs_kv_check(c, nullptr);
+  if (rc) return rc;
+  const size_t width = (size_t)c->kv_heads * c->head_dim;
+  if (*ld == 0) *ld = width;
+  if (*ld < width)
+    return fail(LRS_ERR_INVALID, std::string(what) + ": row stride " + std::to_string(*ld) +
+                                     " is below the row's " + std::to_string(width) + " values");
+  if (n > (size_t)INT_MAX) return fail(LRS_ERR_INVALID, std::string(what) + ": too many rows");
+  return LRS_OK;
+}
+
+int32_t check_trees(const lrs_kv_cache* c, const lrs_tree_batch* t, uint32_t n_heads) {
+  int32_t rc = lrs_kv_check(c, nullptr);
+  if (rc) return rc;
+  if (!t) return fail(LRS_ERR_INVALID, "null tree batch");
+  if (n_heads == 0 || n_heads % c->kv_heads)
+    return fail(LRS_ERR_INVALID, "n_heads must be a positive multiple of kv_heads");
+  if (n_heads / c->kv_heads > 64)
+    return fail(LRS_ERR_UNSUPPORTED, "tree attention supports up to 64 query heads per KV head");
+  if (t->n_trees == 0 || t->n_nodes == 0) return LRS_OK;
+  if (!t->seq || !t->ctx || !t->start) return fail(LRS_ERR_INVALID, "null tree array");
+  if (t->max_nodes == 0 || t->max_nodes > LRS_TREE_MAX_NODES)
+    return fail(LRS_ERR_INVALID, "max_nodes must be in 1..=" + std::to_string(LRS_TREE_MAX_NODES));
+  if (t->max_len == 0 || t->max_len > (uint64_t)c->max_pages * LRS_KV_PAGE)
+    return fail(LRS_ERR_INVALID, "max_len " + std::to_string(t->max_len) +
+                                     " is outside the slots' " + std::to_string(c->max_pages) + " pages");
+  if (t->n_trees > 65535u || t->n_nodes > (1u << 24))
+    return fail(LRS_ERR_UNSUPPORTED, "too many trees or nodes");
+  return LRS_OK;
+}
+
+TreeArgs tree_args(const lrs_kv_cache& c, const lrs_tree_batch& t, uint32_t n_heads, int* err) {
+  TreeArgs a{};
+  a.c = view_of(c, err);
+  a.seq = t.seq;
+  a.ctx = t.ctx;
+  a.start = t.start;
+  a.mask = reinterpret_cast<const unsigned long long*>(t.mask);
+  a.n_trees = (int)t.n_trees;
+  a.n_nodes = (int)t.n_nodes;
+  a.max_nodes = (int)t.max_nodes;
+  a.max_len = (int)t.max_len;
+  a.group = (int)(n_heads / c.kv_heads);
+  return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+lrs_status lrs_kv_check(const lrs_kv_cache* c, size_t* tile_bytes) try {
+  if (!c) return fail(LRS_ERR_INVALID, "null cache");
+  if (c->kv_dtype > LRS_KV_Q8_0)
+    return fail(LRS_ERR_UNSUPPORTED, "unknown KV cache type " + std::to_string(c->kv_dtype));
+  if (c->head_dim != 64 && c->head_dim != 128)
+    return fail(LRS_ERR_UNSUPPORTED, "the KV cache operators support head_dim 64 or 128");
+  if (!c->n_pages || !c->n_seqs || !c->max_pages || !c->kv_heads)
+    return fail(LRS_ERR_INVALID, "KV cache: pages, slots and heads must be non-zero");
+  // positions and page numbers are int32 on the device; heads are a grid dimension
+  if (c->n_pages > (uint32_t)INT_MAX || c->n_seqs > (uint32_t)INT_MAX ||
+      c->max_pages > (uint32_t)INT_MAX / LRS_KV_PAGE || c->kv_heads > 65535u)
+    return fail(LRS_ERR_INVALID, "KV cache: too many pages, slots or heads");
+  if (!c->k_pool || !c->v_pool || !c->pages) return fail(LRS_ERR_INVALID, "KV cache: null pool or page table");
+  if (reinterpret_cast<uintptr_t>(c->k_pool) % 16 || reinterpret_cast<uintptr_t>(c->v_pool) % 16)
+    return fail(LRS_ERR_INVALID, "KV cache: pools must be 16-byte aligned");
+  if (tile_bytes) *tile_bytes = kv_tile_bytes(c->kv_dtype, (int)c->head_dim);
+  return LRS_OK;
+} catch (...) {
+  return lrs::status_of_current_exception();
+}
+
+lrs_status lrs_kv_store(lrs_backend* be, const lrs_kv_cache* c, const int32_t* d_seq,
+                        const int32_t* d_pos, size_t n, const float* d_k, const float* d_v,
+                        size_t ld, void* stream) try {
+  int32_t rc = check_rows(c, n, &ld, "lrs_kv_store");
+  if (rc) return rc;
+  if (n == 0) return LRS_OK;
+  if (!be || !d_seq || !d_pos || !d_k || !d_v) return fail(LRS_ERR_INVALID, "null argument");
+  OnDevice on(be->device);
+  if (on.err != cudaSuccess) return cuda_status(on.err, "cudaSetDevice");
+  KvStoreArgs a{view_of(*c, be->d_err), d_seq, d_pos, (long long)n, d_k, d_v, (long long)ld};
+  return cuda_status(launch_kv_store(a, c->kv_dtype, (int)c->head_dim, be->sms,
+                                     stream ? (cudaStream_t)stream : be->stream),
+                     "lrs_kv_store");
+} catch (...) {
+  return lrs::status_of_current_exception();
+}
+
+lrs_status lrs_kv_load(lrs_backend* be, const lrs_kv_cache* c, const int32_t* d_seq,
+                       const int32_t* d_pos, size_t n, float* d_k, float* d_v, size_t ld,
+                       void* stream) try {
+  int32_t rc = check_rows(c, n, &ld, "lrs_kv_load");
+  if (rc) return rc;
+  if (n == 0 || (!d_k && !d_v)) return LRS_OK;
+  if (!be || !d_seq || !d_pos) return fail(LRS_ERR_INVALID, "null argument");
+  OnDevice on(be->device);
+  if (on.err != cudaSuccess) return cuda_status(on.err, "cudaSetDevice");
+  KvLoadArgs a{view_of(*c, be->d_err), d_seq, d_pos, (long long)n, d_k, d_v, (long long)ld};
+  return cuda_status(launch_kv_load(a, c->kv_dtype, (int)c->head_dim,
+                                    stream ? (cudaStream_t)stream : be->stream),
+                     "lrs_kv_load");
+} catch (...) {
+  return lrs::status_of_current_exception();
+}
+
+lrs_status lrs_kv_accept(lrs_backend* be, const lrs_kv_cache* caches, size_t n_caches,
+                         const int32_t* d_seq, const int32_t* d_ctx, const int32_t* d_start,
+                         const int32_t* d_nodes, size_t n_trees, size_t n_nodes, void* stream) try {
+  if (n_caches && !caches) return fail(LRS_ERR_INVALID, "null cache");
+  int32_t rc;
+  for (size_t i = 0; i < n_caches; i++) {
+    if ((rc = lrs_kv_check(&caches[i], nullptr))) return rc;
+    const lrs_kv_cache &x = caches[i], &y = caches[0];
+    if (x.pages != y.pages || x.n_pages != y.n_pages || x.n_seqs != y.n_seqs ||
+        x.max_pages != y.max_pages || x.kv_heads != y.kv_heads || x.head_dim != y.head_dim ||
+        x.kv_dtype != y.kv_dtype)
+      return fail(LRS_ERR_INVALID, "lrs_kv_accept: the caches may differ in their pools only");
+  }
+  if (n_trees > (size_t)INT_MAX || n_nodes > (size_t)INT_MAX)
+    return fail(LRS_ERR_INVALID, "lrs_kv_accept: too many trees or nodes");
+  if (n_caches == 0 || n_trees == 0 || n_nodes == 0) return LRS_OK;
+  if (!be || !d_seq || !d_ctx || !d_start || !d_nodes) return fail(LRS_ERR_INVALID, "null argument");
+  const size_t per_cache = n_trees * caches[0].kv_heads * 2;
+  if (per_cache > (size_t)INT_MAX) return fail(LRS_ERR_INVALID, "lrs_kv_accept: too many trees or nodes");
+  OnDevice on(be->device);
+  if (on.err != cudaSuccess) return cuda_status(on.err, "cudaSetDevice");
+  cudaStream_t st = stream ? (cudaStream_t)stream : be->stream;
+  const size_t most = std::max<size_t>(1, std::min<size_t>(kAcceptCaches, (size_t)INT_MAX / per_cache));
+  for (size_t c0 = 0; c0 < n_caches; c0 += most) {
+    AcceptArgs a{};
+    a.c = view_of(caches[0], be->d_err);
+    a.n_caches = (int)std::min(most, n_caches - c0);
+    for (int i = 0; i < a.n_caches; i++) {
+      a.k[i] = static_cast<uint8_t*>(caches[c0 + i].k_pool);
+      a.v[i] = static_cast<uint8_t*>(caches[c0 + i].v_pool);
+    }
+    a.seq = d_seq;
+    a.ctx = d_ctx;
+    a.start = d_start;
+    a.nodes = d_nodes;
+    a.n_trees = (int)n_trees;
+    a.n_nodes = (int)n_nodes;
+    const unsigned grid = (unsigned)((per_cache * a.n_caches + 3) / 4);
+#define LRS_CALL(HD, DT) kv_accept_kernel<HD, DT><<<grid, 128, 0, st>>>(a)
+    LRS_KV_DISPATCH(caches[0].head_dim, caches[0].kv_dtype, LRS_CALL);
+#undef LRS_CALL
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_status(e, "lrs_kv_accept");
+  }
+  return LRS_OK;
+} catch (...) {
+  return lrs::status_of_current_exception();
+}
+
+lrs_status lrs_tree_attention_workspace(const lrs_backend* be, const lrs_kv_cache* c,
+                                        const lrs_tree_batch* t, uint32_t n_heads, size_t* bytes) try {
+  int32_t rc = check_trees(c, t, n_heads);
+  if (rc) return rc;
+  if (!bytes) return fail(LRS_ERR_INVALID, "null argument");
+  if (!be) return fail(LRS_ERR_INVALID, "null backend");
+  *bytes = tree_attention_workspace_bytes(tree_args(*c, *t, n_heads, nullptr), (int)c->head_dim, be->sms);
+  return LRS_OK;
+} catch (...) {
+  return lrs::status_of_current_exception();
+}
+
+lrs_status lrs_tree_attention(lrs_backend* be, const lrs_kv_cache* c, const lrs_tree_batch* t,
+                              const float* d_q, size_t q_ld, float* d_out, size_t out_ld,
+                              uint32_t n_heads, float scale, void* d_workspace,
+                              size_t workspace_bytes, void* stream) try {
+  int32_t rc = check_trees(c, t, n_heads);
+  if (rc) return rc;
+  const size_t width = (size_t)n_heads * c->head_dim;
+  if (q_ld == 0) q_ld = width;
+  if (out_ld == 0) out_ld = width;
+  if (q_ld < width || out_ld < width)
+    return fail(LRS_ERR_INVALID, "lrs_tree_attention: row stride below the row's " + std::to_string(width) + " values");
+  if (!std::isfinite(scale)) return fail(LRS_ERR_INVALID, "lrs_tree_attention: scale must be finite");
+  if (t->n_trees == 0 || t->n_nodes == 0) return LRS_OK;
+  if (!be || !d_q || !d_out) return fail(LRS_ERR_INVALID, "null argument");
+  TreeArgs a = tree_args(*c, *t, n_heads, be->d_err);
+  const size_t need = tree_attention_workspace_bytes(a, (int)c->head_dim, be->sms);
+  if (workspace_bytes < need || (need && !d_workspace))
+    return fail(LRS_ERR_INVALID, "lrs_tree_attention: workspace of " + std::to_string(workspace_bytes) +
+                                     " bytes, needs " + std::to_string(need));
+  if (reinterpret_cast<uintptr_t>(d_workspace) % 16)
+    return fail(LRS_ERR_INVALID, "lrs_tree_attention: the workspace must be 16-byte aligned");
+  OnDevice on(be->device);
+  if (on.err != cudaSuccess) return cuda_status(on.err, "cudaSetDevice");
+  a.q = d_q;
+  a.out = d_out;
+  a.q_ld = (long long)q_ld;
+  a.out_ld = (long long)out_ld;
+  a.scale = scale;
+  a.workspace = d_workspace;
+  return cuda_status(launch_tree_attention(a, c->kv_dtype, (int)c->head_dim, be->sms,
+                                           stream ? (cudaStream_t)stream : be->stream),
+                     "lrs_tree_attention");
+} catch (...) {
+  return lrs::status_of_current_exception();
+}
+
+}  // extern "C"
