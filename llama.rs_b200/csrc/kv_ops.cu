@@ -437,8 +437,12 @@ int32_t check_trees(const lrs_kv_cache* c, const lrs_tree_batch* t, uint32_t n_h
   if (t->max_len == 0 || t->max_len > (uint64_t)c->max_pages * LRS_KV_PAGE)
     return fail(LRS_ERR_INVALID, "max_len " + std::to_string(t->max_len) +
                                      " is outside the slots' " + std::to_string(c->max_pages) + " pages");
-  if (t->n_trees > 65535u || t->n_nodes > (1u << 24))
-    return fail(LRS_ERR_UNSUPPORTED, "too many trees or nodes");
+  // the kernels number the batch's tiles (128 positions by 16 rows at least) in int32
+  const uint64_t rows = ((uint64_t)t->max_nodes * (n_heads / c->kv_heads) + 15) / 16,
+                 tiles = ((uint64_t)t->max_len + 127) / 128;
+  if (t->n_trees > 65535u || t->n_nodes > (1u << 24) ||
+      rows * tiles > (uint64_t)INT_MAX / ((uint64_t)t->n_trees * c->kv_heads))
+    return fail(LRS_ERR_UNSUPPORTED, "too many trees, nodes or positions");
   return LRS_OK;
 }
 

@@ -49,10 +49,18 @@ namespace {
 
 constexpr int kTilePos = 128;   // positions of a tile: the lanes of an MMA
 constexpr int kMaxRows = 64;    // rows (node, head) of a CTA's unit
-constexpr int kTaThreads = 576; // four groups of four warps, the copies' warp, the MMAs' warp
+// warps: K 0-3, V 4-7, the softmax 8-11 and 12-15 (half of the rows each), O
+// 16-19, the copies 20, the MMAs 21
+constexpr int kWarpV = 4, kWarpS = 8, kWarpO = 16, kWarpCopy = 20, kWarpMma = 21;
+constexpr int kTaThreads = 32 * 22;
+// Registers a thread: 80 at launch; the groups that decode K and V give 8 each to
+// the one that holds O (an increase beyond what was given would wait for good).
+constexpr int kRegs = 80, kRegsKV = 72, kRegsO = 96;
+static_assert(2 * kRegsKV + kRegsO <= 3 * kRegs, "registers");
 constexpr float kShift = 7.0f;  // P = 2^(s - m + kShift)
 constexpr float kLimit = 15.0f; // largest exponent of P before the maximum moves
 constexpr float kUnset = -3e38f;
+constexpr int kSmemMost = 226 * 1024, kSharedBytes = 7680;
 
 template <int HD, int DT, int NR>
 struct TaShape {
@@ -60,10 +68,11 @@ struct TaShape {
   static constexpr int kB = DT == LRS_KV_Q8_0 ? 2 : 3;                        // terms of q, P
   static constexpr bool kF16 = DT == LRS_KV_Q8_0;
   static constexpr int kProducts = DT == LRS_KV_F32 ? 6 : 3;
-  // tensor memory columns
-  static constexpr int kTmK = 0, kTmV = kTmK + kA * HD / 2, kTmS = kTmV + kA * kTilePos / 2;
-  static constexpr int kNS = kTmS + 3 * NR <= 512 ? 2 : 1;  // score buffers
-  static constexpr int kTmO = kTmS + kNS * NR;
+  // tensor memory columns: V is double-buffered where it fits
+  static constexpr int kVCols = kA * kTilePos / 2;
+  static constexpr int kTmK = 0, kTmV = kTmK + kA * HD / 2;
+  static constexpr int kNV = kTmV + 2 * kVCols + 2 * NR <= 512 ? 2 : 1;
+  static constexpr int kTmS = kTmV + kNV * kVCols, kTmO = kTmS + NR;
   static constexpr int kTmCols = kTmO + NR <= 256 ? 256 : 512;
   static_assert(kTmO + NR <= 512, "tensor memory");
   // raw tiles: K rows of f32 / bf16 padded by 16 bytes against bank conflicts
@@ -74,12 +83,16 @@ struct TaShape {
   static constexpr int kSlotK = DT == LRS_KV_Q8_0 ? kTileB : kSlotPos * kRowK;
   static constexpr int kSlotV = kTileB / (kPageSize / kSlotPos);
   // shared memory
-  static constexpr int kQTerm = NR * HD * 2, kPTerm = NR * kTilePos * 2;
-  static constexpr int kOffQ = 0, kOffP = kB * kQTerm, kOffRow = kOffP + kB * kPTerm;
-  static constexpr int kOffRing = kOffRow + 5120;
+  static constexpr int kQTerm = NR * HD * 2, kPTerm = NR * kTilePos * 2, kPBuf = kB * kPTerm;
+  static constexpr int kOffQ = 0, kOffP = kB * kQTerm;
+  // P is double-buffered where two tiles of slots remain beside it
+  static constexpr int kNP =
+      kOffP + 2 * kPBuf + kSharedBytes + 2 * kSlots * (kSlotK + kSlotV) <= kSmemMost ? 2 : 1;
+  static constexpr int kOffRow = kOffP + kNP * kPBuf;
+  static constexpr int kOffRing = kOffRow + kSharedBytes;
   // a K slot has one reader, or two that read one tile's halves: whole tiles of
   // slots keep a slot's readers the same, so that none misses one of its phases
-  static constexpr int kRoom = 226 * 1024 - kOffRing;
+  static constexpr int kRoom = kSmemMost - kOffRing;
   static constexpr int kRing0 = (kRoom / (kSlotK + kSlotV) + kSlots - 1) / kSlots * kSlots;
   static constexpr int kRingK = kRing0 > 8 ? 8 : kRing0;
   static constexpr int kRingV0 = (kRoom - kRingK * kSlotK) / kSlotV;
@@ -91,26 +104,28 @@ struct TaShape {
 
 // The part of shared memory that is not operands (kOffRow).
 struct TaShared {
-  unsigned long long mask[2][kMaxRows];  // per unit parity: the row's node mask
-  long long out[2][kMaxRows];            // offset of the row's output, -1 = no row
-  float fin_m[2][kMaxRows], fin_l[2][kMaxRows];
+  float c[4][kMaxRows];                  // score factor, per unit
+  float nm[kMaxRows];                    // kShift - maximum
+  float f[4][kMaxRows];                  // rescaling of the earlier tiles, per tile
+  float red[2][4][kMaxRows / 2];         // a softmax group's warps meet here
+  float fin_m[2][kMaxRows], fin_l[2][kMaxRows];  // per unit parity: maximum - kShift, sum
+  unsigned long long mask[2][kMaxRows];  // the row's node mask
+  uint32_t vis[2][LRS_TREE_MAX_NODES];   // rows of a softmax group that see a node
+  long long out[2][kMaxRows];            // offset of the row's output
   unsigned vbad[2][4][2];                // nodes whose V is not finite, per warp that reads V
-  float c[kMaxRows], m[kMaxRows];        // score factor, maximum - kShift
-  float f[2][kMaxRows];                  // rescaling of the earlier tiles, per tile parity
-  int moved[2];
-  int fail[2];  // a softmax warp's wait gave up, per tile parity
+  int moved[4][2];
+  int fail[2][2];  // a softmax warp's wait gave up, per tile parity and group
   uint64_t k_full[8], k_empty[8], v_full[8], v_empty[8];
-  uint64_t ak_full, ak_empty, av_full, q_full, p_full, pv_done, o_empty, drain;
-  uint64_t s_full[2], s_empty[2], u_full[2], u_empty[2];
+  uint64_t ak_full, ak_empty, s_full, s_empty, o_full, o_empty, drain;
+  uint64_t av_full[2], av_empty[2], p_full[2], p_empty[2], u_full[2], u_empty[2];
   int abort;
   uint32_t tmem;
   // the schedule
-  long long first, last;  // this CTA's tiles
-  int tree, unit, tile;   // of `first`
-  long long unit0;        // first tile of that unit
+  int first, last;       // this CTA's tiles
+  int tree, unit, tile;  // of `first`
   int active;
 };
-static_assert(sizeof(TaShared) <= 5120, "shared state");
+static_assert(sizeof(TaShared) <= kSharedBytes, "shared state");
 
 __device__ __forceinline__ void ta_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -121,20 +136,27 @@ __device__ __forceinline__ void ta_fence_before() {
 __device__ __forceinline__ void ta_fence_after() {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
-__device__ __forceinline__ void ta_commit(uint64_t* bar) {
+// The warp issues these converged, one lane elected: addresses stay in uniform registers.
+__device__ __forceinline__ void ta_commit(uint32_t bar, uint32_t elected) {
   asm volatile(
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-          smem_u32(bar))
+      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(bar),
+      "r"(elected)
       : "memory");
 }
 // D[tmem] (+)= A[tmem] . B[shared]
 __device__ __forceinline__ void ta_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
-                                       bool accumulate) {
+                                       bool accumulate, uint32_t elected) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(elected)
       : "memory");
+}
+__device__ __forceinline__ uint32_t ta_elect() {
+  uint32_t e;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(e));
+  return e;
 }
 __device__ __forceinline__ uint64_t ta_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
   return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) |
@@ -145,7 +167,7 @@ __device__ __forceinline__ uint32_t ta_idesc(bool f16, bool b_n_major, int n) {
   return (1u << 4) | (f16 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)b_n_major << 16) |
          ((uint32_t)(n >> 3) << 17) | (8u << 24);
 }
-__device__ __forceinline__ void ta_ld16(uint32_t taddr, float (&v)[16]) {
+__device__ __forceinline__ void ta_ld16(uint32_t taddr, float* v) {
   uint32_t r[16];
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
@@ -154,9 +176,34 @@ __device__ __forceinline__ void ta_ld16(uint32_t taddr, float (&v)[16]) {
         "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
         "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
   for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void ta_ld8(uint32_t taddr, float* v) {
+  uint32_t r[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
+                 "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+#pragma unroll
+  for (int i = 0; i < 8; i++) v[i] = __uint_as_float(r[i]);
+}
+// Two f32 operations in one instruction.
+__device__ __forceinline__ float2 ta_fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+      " fma.rn.f32x2 w, x, y, z;\n mov.b64 {%0, %1}, w;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 ta_add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n"
+      " add.rn.f32x2 w, x, y;\n mov.b64 {%0, %1}, w;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 __device__ __forceinline__ void ta_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
@@ -165,6 +212,13 @@ __device__ __forceinline__ void ta_st16(uint32_t taddr, const uint32_t (&r)[16])
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
       "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+// The loaded registers may be used after this: it names them, so that no use moves above it.
+template <int N>
+__device__ __forceinline__ void ta_wait_ld(float (&v)[N]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < N; i++) asm volatile("" : "+f"(v[i]));
 }
 __device__ __forceinline__ void ta_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -189,29 +243,63 @@ __device__ __forceinline__ void ta_group_sync(int id) {
   asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory");
 }
 
+template <int N>
+__device__ __forceinline__ void ta_regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void ta_regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// Tests a barrier's phase; an incomplete one suspends the warp for up to 1 ms, so
+// that waiting warps leave the issue slots and the instruction cache to the others.
+__device__ __forceinline__ bool ta_try_wait(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+      " selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity), "r"(1000000u)
+      : "memory");
+  return done != 0;
+}
+constexpr uint32_t kPolls = 1u << 14;
 // A wait that gives up after a bounded number of polls, or when another role did.
 __device__ __forceinline__ bool ta_wait(TaShared& sh, uint64_t* bar, uint32_t parity) {
-  for (uint32_t i = 0; i < kSpinLimit >> 4; i++) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 63) == 63 && *reinterpret_cast<volatile int*>(&sh.abort)) return false;
+  const uint32_t at = smem_u32(bar);
+#pragma unroll 1
+  for (uint32_t i = 0; i < kPolls; i++) {
+    if (ta_try_wait(at, parity)) return true;
+    if (*reinterpret_cast<volatile int*>(&sh.abort)) return false;
   }
   *reinterpret_cast<volatile int*>(&sh.abort) = 1;
   return false;
 }
+// A position in a ring of N barriers and the parity of its current pass.
+template <int N>
+struct TaRing {
+  uint32_t at = 0, parity = 0;
+  __device__ __forceinline__ void step(uint32_t by = 1) {
+    at += by;
+    if (at >= N) at -= N, parity ^= 1;
+  }
+};
 
 // Two f32 values as `TERMS` 16-bit pairs whose sum they are (to 2^-22, 2^-24).
 template <bool F16, int TERMS>
-__device__ __forceinline__ void ta_split(float a, float b, uint32_t (&t)[TERMS]) {
+__device__ __forceinline__ void ta_split(float2 v, uint32_t (&t)[TERMS]) {
 #pragma unroll
   for (int i = 0; i < TERMS; i++) {
     if constexpr (F16) {
-      const __half2 h = __floats2half2_rn(a, b);
+      const __half2 h = __floats2half2_rn(v.x, v.y);
       t[i] = *reinterpret_cast<const uint32_t*>(&h);
-      if (i + 1 < TERMS) a -= __low2float(h), b -= __high2float(h);
+      if (i + 1 < TERMS) v = ta_add2(v, make_float2(-__low2float(h), -__high2float(h)));
     } else {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
       t[i] = *reinterpret_cast<const uint32_t*>(&h);
-      if (i + 1 < TERMS) a -= __uint_as_float(t[i] << 16), b -= __uint_as_float(t[i] & 0xffff0000u);
+      if (i + 1 < TERMS)
+        v = ta_add2(v, make_float2(-__uint_as_float(t[i] << 16), -__uint_as_float(t[i] & 0xffff0000u)));
     }
   }
 }
@@ -252,9 +340,11 @@ struct TaTree {
     tiles = (len + kTilePos - 1) / kTilePos;
     return true;
   }
-  __device__ __forceinline__ long long total(const TreeArgs& a) const {
-    return (long long)tiles * chunks * a.c.heads;
+  // rows of a chunk: an even share, in whole steps of the MMA's N
+  __device__ __forceinline__ int share(const TreeArgs& a) const {
+    return ((n * a.group + chunks - 1) / chunks + 15) & ~15;
   }
+  __device__ __forceinline__ int total(const TreeArgs& a) const { return tiles * chunks * a.c.heads; }
 };
 
 // Partial results: [2 * CTAs] segments of [kMaxRows] (m, l) and [NR][HD] sums.
@@ -270,7 +360,7 @@ __host__ __device__ constexpr size_t ta_seg_floats() {
 // The units (tree, KV head, chunk of rows) of a CTA, tile range by tile range.
 struct TaIter {
   int tree, unit, tile;  // next unit, its first tile here
-  long long left;        // tiles left
+  int left;              // tiles left
   TaTree t;
   int t0, t1, index;     // the current unit's tiles, its number in this CTA
   int kvh, row0, rows;
@@ -292,12 +382,11 @@ struct TaIter {
       loaded = true;
     }
     kvh = unit / t.chunks;
-    // rows of a chunk: an even share, in whole steps of the MMA's N
-    const int all = t.n * a.group, share = ((all + t.chunks - 1) / t.chunks + 15) & ~15;
+    const int share = t.share(a);
     row0 = (unit % t.chunks) * share;
-    rows = max(0, min(share, all - row0));
+    rows = min(share, t.n * a.group - row0);
     t0 = tile;
-    t1 = (int)min((long long)t.tiles, t0 + left);
+    t1 = min(t.tiles, t0 + left);
     left -= t1 - t0;
     index++;
     unit++;
@@ -306,11 +395,168 @@ struct TaIter {
   }
 };
 
+// A slot's positions of V into tensor memory: lane = column h of the head.  TAIL:
+// positions past the end become zeros, and so do nodes with a value that is not
+// finite, which are noted (their weight may be a zero that must stay one).
+template <int HD, int DT, int NR, bool TAIL>
+__device__ __forceinline__ void decode_v(const uint8_t* raw, uint32_t col, int w, int lane, int p0,
+                                         int ctx, int len, unsigned* vbad) {
+  using S = TaShape<HD, DT, NR>;
+  const int h = w * 32 + lane;
+#pragma unroll 1
+  for (int g = 0; g < S::kSlotPos / 32; g++) {  // 32 positions: 16 columns a term
+    uint32_t x[S::kA][16];
+    if constexpr (DT == LRS_KV_Q8_0) {
+      uint4 d8;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const int r = g * 32 + i * 4;
+        if (i % 2 == 0) d8 = *reinterpret_cast<const uint4*>(raw + q8_v_scale(HD, r, w));
+        uint2 dd = i % 2 ? make_uint2(d8.z, d8.w) : make_uint2(d8.x, d8.y);
+        if constexpr (TAIL) {
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            uint32_t& d = j < 2 ? dd.x : dd.y;
+            const uint32_t keep = j & 1 ? 0x0000ffffu : 0xffff0000u, inf = j & 1 ? 0x7c000000u : 0x7c00u;
+            const int p = p0 + r + j;
+            const bool bad = (d & inf) == inf && p >= ctx;
+            if (p >= len || bad) {
+              d &= keep;
+              if (p < len && lane == 0) atomicOr(&vbad[(p - ctx) >> 5], 1u << ((p - ctx) & 31));
+            }
+          }
+        }
+        const uint32_t cw = *reinterpret_cast<const uint32_t*>(raw + q8_v_code(HD, r, h));
+        uint32_t hi[2], lo[2];
+        ta_q8(cw, ta_u2(dd.x), ta_u2(dd.y), hi, lo);
+        x[0][i * 2] = hi[0], x[0][i * 2 + 1] = hi[1];
+        x[1][i * 2] = lo[0], x[1][i * 2 + 1] = lo[1];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        float f[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const int r = g * 32 + i * 2 + j, p = p0 + r;
+          f[j] = DT == LRS_KV_BF16
+                     ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(raw)[r * HD + h] << 16)
+                     : reinterpret_cast<const float*>(raw)[r * HD + h];
+          if constexpr (TAIL) {
+            const bool bad = (__float_as_uint(f[j]) & 0x7f800000u) == 0x7f800000u && p >= ctx;
+            if (p >= len || bad) {
+              f[j] = 0.0f;
+              if (p < len) atomicOr(&vbad[(p - ctx) >> 5], 1u << ((p - ctx) & 31));
+            }
+          }
+        }
+        uint32_t y[S::kA];
+        ta_split<false, S::kA>(make_float2(f[0], f[1]), y);
+#pragma unroll
+        for (int q = 0; q < S::kA; q++) x[q][i] = y[q];
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < S::kA; q++) ta_st16(col + q * (kTilePos / 2) + g * 16, x[q]);
+  }
+}
+
+// The scores of up to R rows (8 a step) of this lane's position as exponents of
+// P: c * s - maximum + kShift, -inf where the row does not see the position.
+template <int R>
+__device__ __forceinline__ void ta_exponents(float (&s)[R], int steps, const float* c,
+                                             const float* nm, uint32_t vis) {
+#pragma unroll
+  for (int r = 0; r < R; r += 4) {
+    if (r % 8 == 0 && r / 8 >= steps) break;
+    const float4 cc = *reinterpret_cast<const float4*>(c + r), mm = *reinterpret_cast<const float4*>(nm + r);
+    const float2 x = ta_fma2(make_float2(s[r], s[r + 1]), make_float2(cc.x, cc.y), make_float2(mm.x, mm.y));
+    const float2 y = ta_fma2(make_float2(s[r + 2], s[r + 3]), make_float2(cc.z, cc.w), make_float2(mm.z, mm.w));
+    s[r] = x.x, s[r + 1] = x.y, s[r + 2] = y.x, s[r + 3] = y.y;
+  }
+  if (vis != ~0u) {
+#pragma unroll
+    for (int r = 0; r < R; r++)
+      if (!(vis >> r & 1)) s[r] = -INFINITY;
+  }
+}
+
+// q * scale * log2(e) of a unit's rows in terms, K-major core matrices: a warp
+// takes 8 rows, a lane 8 columns of one at a time.  For f16 terms a power of two
+// brings a row's largest magnitude to [2^10, 2^11); c is its inverse.
+template <int HD, int DT, int NR>
+__device__ __forceinline__ void load_q(const TreeArgs& a, const TaIter& it, uint8_t* smem, float* c,
+                                       int w, int lane) {
+  using S = TaShape<HD, DT, NR>;
+  const float qs = a.scale * 1.44269504088896f;
+  const bool vec = a.q_ld % 4 == 0 && reinterpret_cast<uintptr_t>(a.q) % 16 == 0;
+  const int groups = 2 * ((it.rows + 15) >> 4);
+#pragma unroll 1
+  for (int g8 = w; g8 < groups; g8 += 4) {
+    const int gr = g8 * 8 + (lane & 7), row = it.row0 + gr;
+    const float* src = a.q + (size_t)(it.t.s + row / a.group) * a.q_ld +
+                       (size_t)(it.kvh * a.group + row % a.group) * HD + (lane >> 3) * 8;
+    float x[HD / 32][8];
+#pragma unroll
+    for (int j = 0; j < HD / 32; j++) {
+      if (gr >= it.rows) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[j][e] = 0.0f;
+      } else if (vec) {
+        const float4 f0 = *reinterpret_cast<const float4*>(src + j * 32), f1 = *reinterpret_cast<const float4*>(src + j * 32 + 4);
+        x[j][0] = f0.x, x[j][1] = f0.y, x[j][2] = f0.z, x[j][3] = f0.w;
+        x[j][4] = f1.x, x[j][5] = f1.y, x[j][6] = f1.z, x[j][7] = f1.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[j][e] = src[j * 32 + e];
+      }
+    }
+    float mx = 0.0f;
+#pragma unroll
+    for (int j = 0; j < HD / 32; j++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        x[j][e] *= qs;
+        mx = fmaxf(mx, fabsf(x[j][e]));
+      }
+    float up0 = 1.0f, up1 = 1.0f, down = 1.0f;
+    if constexpr (S::kF16) {
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+      const int e = (int)(__float_as_uint(mx) >> 23);
+      if (mx > 0.0f && e < 255) {  // 2^(137 - e), as two factors: it may pass f32's range
+        const int k = 137 - e, k0 = k >> 1;
+        up0 = __uint_as_float((uint32_t)(127 + k0) << 23);
+        up1 = __uint_as_float((uint32_t)(127 + k - k0) << 23);
+        down = ldexpf(1.0f, -k);
+      }
+    }
+    if (lane < 8) c[gr] = down;
+#pragma unroll
+    for (int j = 0; j < HD / 32; j++) {
+      uint32_t y[S::kB][4];
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        float2 v = make_float2(x[j][2 * e], x[j][2 * e + 1]);
+        if constexpr (S::kF16) v = make_float2(v.x * up0 * up1, v.y * up0 * up1);
+        uint32_t z[S::kB];
+        ta_split<S::kF16, S::kB>(v, z);
+#pragma unroll
+        for (int k = 0; k < S::kB; k++) y[k][e] = z[k];
+      }
+      uint8_t* dst = smem + S::kOffQ + g8 * (HD / 8 * 128) + (j * 4 + (lane >> 3)) * 128 + (lane & 7) * 16;
+#pragma unroll
+      for (int k = 0; k < S::kB; k++)
+        *reinterpret_cast<uint4*>(dst + k * S::kQTerm) = make_uint4(y[k][0], y[k][1], y[k][2], y[k][3]);
+    }
+  }
+}
+
 template <int HD, int DT, int NR>
 __global__ void __launch_bounds__(kTaThreads, 1)
     tree_attention_kernel(const __grid_constant__ TreeArgs a) {
   using S = TaShape<HD, DT, NR>;
-  constexpr int kA = S::kA, kB = S::kB;
+  constexpr int kA = S::kA;
   constexpr bool kF16 = S::kF16;
   constexpr int kWarpsD = HD / 32;  // warps that own columns of V
   extern __shared__ __align__(128) uint8_t smem[];
@@ -320,54 +566,55 @@ __global__ void __launch_bounds__(kTaThreads, 1)
 
   // ---- the schedule: every CTA finds its share of all tiles ----
   {
-    __shared__ long long wsum[kTaThreads / 32];
+    __shared__ int wsum[kTaThreads / 32];
     const int per = (a.n_trees + kTaThreads - 1) / kTaThreads;
-    long long mine = 0;
+    int mine = 0;
+    TaTree tr;
     for (int i = 0; i < per; i++) {
       const int t = tid * per + i;
-      TaTree tr;
       if (t < a.n_trees && tr.load(a, t, NR)) mine += tr.total(a);
     }
-    long long incl = mine;
+    int incl = mine;
     for (int o = 1; o < 32; o <<= 1) {
-      const long long x = __shfl_up_sync(0xffffffffu, incl, o);
+      const int x = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += x;
     }
     if (lane == 31) wsum[warp] = incl;
     if (tid == 0) sh.active = 0;
     __syncthreads();
-    long long before = incl - mine, total = 0;
+    int before = incl - mine, total = 0;
     for (int w = 0; w < kTaThreads / 32; w++) {
       if (w < warp) before += wsum[w];
       total += wsum[w];
     }
-    const long long ctas = min((long long)gridDim.x, total), c = blockIdx.x;
+    const int ctas = min((int)gridDim.x, total), c = blockIdx.x;
+    TaDesc d{};
     if (c < ctas) {
-      const long long first = total * c / ctas, last = total * (c + 1) / ctas;
+      // CTA i starts at tile i * (total / ctas) + i * (total % ctas) / ctas
+      const unsigned quot = (unsigned)total / (unsigned)ctas, rem = (unsigned)total % (unsigned)ctas;
+      auto start = [&](int i) { return (int)(quot * i + i * rem / (unsigned)ctas); };
+      const int first = start(c);
       if (before <= first && first < before + mine) {  // the thread that holds the first tile's tree
-        long long at = before;
+        int at = before;
         for (int i = 0; i < per; i++) {
-          TaTree tr;
           const int t = tid * per + i;
-          if (t >= a.n_trees || !tr.load(a, t, NR)) continue;
+          if (t >= a.n_trees || (per > 1 && !tr.load(a, t, NR))) continue;
           if (first < at + tr.total(a)) {
+            const int unit = (first - at) / tr.tiles, unit0 = at + unit * tr.tiles;
             sh.tree = t;
-            sh.unit = (int)((first - at) / tr.tiles);
-            sh.tile = (int)((first - at) % tr.tiles);
-            sh.unit0 = at + (long long)sh.unit * tr.tiles;
+            sh.unit = unit;
+            sh.tile = first - unit0;
             sh.first = first;
-            sh.last = last;
+            sh.last = start(c + 1);
             sh.active = 1;
             // this CTA starts inside a unit: the first such CTA describes it
-            TaDesc d{};
-            if (sh.tile > 0 && total * (c - 1) / ctas <= sh.unit0) {
-              const long long end = sh.unit0 + tr.tiles;
+            if (first > unit0 && start(c - 1) <= unit0) {
               d.nseg = 2;
-              while (total * (c + d.nseg - 1) / ctas < end) d.nseg++;
-              const int all = tr.n * a.group, share = ((all + tr.chunks - 1) / tr.chunks + 15) & ~15;
-              d.kvh = sh.unit / tr.chunks;
-              d.row0 = (sh.unit % tr.chunks) * share;
-              d.rows = max(0, min(share, all - d.row0));
+              while (start(c + d.nseg - 1) < unit0 + tr.tiles) d.nseg++;
+              const int share = tr.share(a);
+              d.kvh = unit / tr.chunks;
+              d.row0 = (unit % tr.chunks) * share;
+              d.rows = min(share, tr.n * a.group - d.row0);
               d.s = tr.s;
             }
             reinterpret_cast<TaDesc*>(a.workspace)[c] = d;
@@ -377,7 +624,6 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         }
       }
     } else if (tid == 0) {
-      TaDesc d{};
       reinterpret_cast<TaDesc*>(a.workspace)[c] = d;
     }
     segs = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + gridDim.x * sizeof(TaDesc));
@@ -391,18 +637,19 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     }
     mbar_init(&sh.ak_full, 4);
     mbar_init(&sh.ak_empty, 1);
-    mbar_init(&sh.av_full, kWarpsD);
-    mbar_init(&sh.q_full, 4);
-    mbar_init(&sh.p_full, 4);
-    mbar_init(&sh.pv_done, 1);
+    mbar_init(&sh.s_full, 1);
+    mbar_init(&sh.s_empty, 8);
+    mbar_init(&sh.o_full, 1);
     mbar_init(&sh.o_empty, kWarpsD);
     mbar_init(&sh.drain, 1);
     for (int i = 0; i < 2; i++) {
-      mbar_init(&sh.s_full[i], 1);
-      mbar_init(&sh.s_empty[i], 4);
-      mbar_init(&sh.u_full[i], 4);
+      mbar_init(&sh.av_full[i], kWarpsD);
+      mbar_init(&sh.av_empty[i], 1);
+      mbar_init(&sh.p_full[i], 8);
+      mbar_init(&sh.p_empty[i], 1);
+      mbar_init(&sh.u_full[i], 8);
       mbar_init(&sh.u_empty[i], kWarpsD);
-      sh.fail[i] = 0;
+      sh.fail[i][0] = sh.fail[i][1] = 0;
     }
     sh.abort = 0;
     fence_barrier_init();
@@ -410,7 +657,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
   __syncthreads();
   pdl_launch_dependents();
   if (!sh.active) return;
-  if (warp == 17) {
+  if (warp == kWarpMma) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(&sh.tmem)),
                  "r"((uint32_t)S::kTmCols)
@@ -420,34 +667,39 @@ __global__ void __launch_bounds__(kTaThreads, 1)
   ta_fence_before();
   __syncthreads();
   ta_fence_after();
-  const uint32_t tmem = sh.tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
   const uint32_t sbase = smem_u32(smem);
   const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;  // this warp's lanes of tensor memory
   TaIter it;
   it.begin(sh);
   bool ok = true;
 
-  if (warp < 4) {
+  if (warp < kWarpV) {
     // ---- K: a lane is a position; its row into tensor memory ----
+    ta_regs_dec<kRegsKV>();
     uint32_t tile = 0;
+    TaRing<S::kRingK> ring;
+    ring.at = warp * 32 / S::kSlotPos;
     while (ok && it.next(a, NR)) {
+      // the last unit's scores are done with q and its factors
+      if (tile > 0) ok = ta_wait(sh, &sh.ak_empty, (tile - 1) & 1);
+      if (!ok) break;
+      load_q<HD, DT, NR>(a, it, smem, sh.c[it.index & 3], warp, lane);
+      fence_proxy_async();
       for (int t = it.t0; t < it.t1 && ok; t++, tile++) {
-        const uint32_t n = tile * S::kSlots + (warp * 32) / S::kSlotPos, slot = n % S::kRingK;
-        ok = ta_wait(sh, &sh.k_full[slot], (n / S::kRingK) & 1);
+        const uint32_t slot = ring.at;
+        ok = ta_wait(sh, &sh.k_full[slot], ring.parity);
+        ring.step(S::kSlots);
         if (ok && tile > 0) ok = ta_wait(sh, &sh.ak_empty, (tile - 1) & 1);
         if (!ok) break;
         ta_fence_after();
         const uint8_t* raw = smem + S::kOffRing + slot * S::kSlotK;
         const int r = (warp * 32 + lane) % S::kSlotPos;
         if constexpr (DT == LRS_KV_Q8_0) {
-          __half d[HD / 32];
-#pragma unroll
-          for (int b = 0; b < HD / 32; b++)
-            d[b] = *reinterpret_cast<const __half*>(raw + q8_k_scale(HD, r, b));
-#pragma unroll
+#pragma unroll 1
           for (int b = 0; b < HD / 32; b++) {  // a block: 16 columns of hi, 16 of lo
             uint32_t hi[16], lo[16];
-            const __half2 d2 = __half2half2(d[b]);
+            const __half2 d2 = __half2half2(*reinterpret_cast<const __half*>(raw + q8_k_scale(HD, r, b)));
 #pragma unroll
             for (int h = 0; h < 2; h++) {
               const uint4 w4 = *reinterpret_cast<const uint4*>(raw + q8_k_code(r, b * 32 + h * 16));
@@ -465,7 +717,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
           }
         } else {
           const uint8_t* row = raw + r * S::kRowK;
-#pragma unroll
+#pragma unroll 1
           for (int b = 0; b < HD / 32; b++) {  // 32 values: 16 columns a term
             uint32_t x[kA][16];
             if constexpr (DT == LRS_KV_BF16) {
@@ -479,10 +731,10 @@ __global__ void __launch_bounds__(kTaThreads, 1)
               for (int i = 0; i < 8; i++) {
                 const float4 f = *reinterpret_cast<const float4*>(row + b * 128 + i * 16);
                 uint32_t y[kA];
-                ta_split<false, kA>(f.x, f.y, y);
+                ta_split<false, kA>(make_float2(f.x, f.y), y);
 #pragma unroll
                 for (int k = 0; k < kA; k++) x[k][i * 2] = y[k];
-                ta_split<false, kA>(f.z, f.w, y);
+                ta_split<false, kA>(make_float2(f.z, f.w), y);
 #pragma unroll
                 for (int k = 0; k < kA; k++) x[k][i * 2 + 1] = y[k];
               }
@@ -500,10 +752,13 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         if (lane == 0) ta_arrive(&sh.ak_full);
       }
     }
-  } else if (warp < 8) {
+  } else if (warp < kWarpS) {
     // ---- V: a lane is a column of the head; positions along its row ----
-    const int w = warp - 4, h = w * 32 + lane;
+    ta_regs_dec<kRegsKV>();
+    const int w = warp - kWarpV;
     uint32_t tile = 0;
+    TaRing<S::kRingV> ring;
+    TaRing<S::kNV> buf;
     while (w < kWarpsD && ok && it.next(a, NR)) {
       // the words of the unit before last have been read
       if (it.index >= 2) ok = ta_wait(sh, &sh.u_empty[it.index & 1], ((it.index >> 1) - 1) & 1);
@@ -511,73 +766,24 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       if (lane < 2) vbad[lane] = 0;
       __syncwarp();
       for (int t = it.t0; t < it.t1 && ok; t++, tile++) {
-        if (tile > 0) ok = ta_wait(sh, &sh.pv_done, (tile - 1) & 1);
+        const uint32_t vb = buf.at;
+        if (tile >= S::kNV) ok = ta_wait(sh, &sh.av_empty[vb], buf.parity ^ 1);
+        buf.step();
         ta_fence_after();
         const bool tail = (t + 1) * kTilePos > it.t.ctx;  // holds nodes, or positions past the end
 #pragma unroll 1
         for (int k = 0; k < S::kSlots && ok; k++) {
-          const uint32_t n = tile * S::kSlots + k, slot = n % S::kRingV;
-          ok = ta_wait(sh, &sh.v_full[slot], (n / S::kRingV) & 1);
+          const uint32_t slot = ring.at;
+          ok = ta_wait(sh, &sh.v_full[slot], ring.parity);
+          ring.step();
           if (!ok) break;
           const uint8_t* raw = smem + S::kOffV + slot * S::kSlotV;
           const int p0 = t * kTilePos + k * S::kSlotPos;
-          const uint32_t col = tmem + lanes + S::kTmV + k * (S::kSlotPos / 2);
-#pragma unroll
-          for (int g = 0; g < S::kSlotPos / 32; g++) {  // 32 positions: 16 columns a term
-            uint32_t x[kA][16];
-            if constexpr (DT == LRS_KV_Q8_0) {
-#pragma unroll
-              for (int i = 0; i < 8; i++) {
-                const int r = g * 32 + i * 4;
-                uint2 dd = *reinterpret_cast<const uint2*>(raw + q8_v_scale(HD, r, w));
-                if (tail) {
-#pragma unroll
-                  for (int j = 0; j < 4; j++) {
-                    uint32_t& d = j < 2 ? dd.x : dd.y;
-                    const uint32_t keep = j & 1 ? 0x0000ffffu : 0xffff0000u, bits = d & ~keep;
-                    const int p = p0 + r + j;
-                    const bool bad = (bits & (j & 1 ? 0x7c000000u : 0x7c00u)) == (j & 1 ? 0x7c000000u : 0x7c00u);
-                    if (p >= it.t.len || (bad && p >= it.t.ctx)) {
-                      d &= keep;
-                      if (p < it.t.len && lane == 0)
-                        atomicOr(&vbad[(p - it.t.ctx) >> 5], 1u << ((p - it.t.ctx) & 31));
-                    }
-                  }
-                }
-                const uint32_t cw = *reinterpret_cast<const uint32_t*>(raw + q8_v_code(HD, r, h));
-                uint32_t hi[2], lo[2];
-                ta_q8(cw, ta_u2(dd.x), ta_u2(dd.y), hi, lo);
-                x[0][i * 2] = hi[0], x[0][i * 2 + 1] = hi[1];
-                x[1][i * 2] = lo[0], x[1][i * 2 + 1] = lo[1];
-              }
-            } else {
-#pragma unroll
-              for (int i = 0; i < 16; i++) {
-                float f[2];
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                  const int r = g * 32 + i * 2 + j, p = p0 + r;
-                  f[j] = DT == LRS_KV_BF16
-                             ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(raw)[r * HD + h] << 16)
-                             : reinterpret_cast<const float*>(raw)[r * HD + h];
-                  if (tail) {
-                    const bool bad = (__float_as_uint(f[j]) & 0x7f800000u) == 0x7f800000u;
-                    if (p >= it.t.len || (bad && p >= it.t.ctx)) {
-                      f[j] = 0.0f;
-                      if (p < it.t.len)
-                        atomicOr(&vbad[(p - it.t.ctx) >> 5], 1u << ((p - it.t.ctx) & 31));
-                    }
-                  }
-                }
-                uint32_t y[kA];
-                ta_split<false, kA>(f[0], f[1], y);
-#pragma unroll
-                for (int q = 0; q < kA; q++) x[q][i] = y[q];
-              }
-            }
-#pragma unroll
-            for (int q = 0; q < kA; q++) ta_st16(col + q * (kTilePos / 2) + g * 16, x[q]);
-          }
+          const uint32_t col = tmem + lanes + S::kTmV + vb * S::kVCols + k * (S::kSlotPos / 2);
+          if (tail)
+            decode_v<HD, DT, NR, true>(raw, col, w, lane, p0, it.t.ctx, it.t.len, vbad);
+          else
+            decode_v<HD, DT, NR, false>(raw, col, w, lane, p0, it.t.ctx, it.t.len, vbad);
           __syncwarp();
           if (lane == 0) ta_arrive(&sh.v_empty[slot]);
         }
@@ -585,274 +791,226 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         ta_wait_st();
         ta_fence_before();
         __syncwarp();
-        if (lane == 0) ta_arrive(&sh.av_full);
+        if (lane == 0) ta_arrive(&sh.av_full[vb]);
       }
     }
-  } else if (warp < 12) {
-    // ---- q, and the softmax: a lane is a position ----
-    const int w = warp - 8, gt = tid - 256;
-    constexpr int kBar = 1;
-    float l[NR];
+  } else if (warp < kWarpO) {
+    // ---- the softmax: a lane is a position, a group of four warps half of the rows ----
+    const int grp = (warp - kWarpS) >> 2, w = warp & 3, gt = w * 32 + lane, bar = 1 + grp;
+    constexpr int R = NR / 2;
+    float2 l[R / 2];
     uint32_t tile = 0;
+    TaRing<S::kNP> buf;
     bool left = false;
     // the four warps meet at barriers: one whose wait gave up goes on (on stale
     // data, in bounds) to the next vote, where they leave together
     while (!left && it.next(a, NR)) {
       const int u = it.index & 1;
+      const int steps = (it.rows + 15) >> 4, base = grp * steps * 8;  // steps of 8 rows from `base`
+      const float* c = sh.c[it.index & 3] + base;
+      float* nm = sh.nm + base;
+      const int my = base + gt;  // the row that this thread keeps, one of the first `mine`
+      const int mine = steps * 8;
+      unsigned long long my_mask = 0;
+      long long my_out = 0;
+      if (gt < mine) {
+        const int row = it.row0 + my, node = row / a.group, g = row % a.group;
+        my_out = (long long)(it.t.s + node) * a.out_ld + (long long)(it.kvh * a.group + g) * HD;
+        if (my < it.rows) {
+          my_mask = a.mask ? a.mask[it.t.s + node] : (node == 63 ? ~0ull : (2ull << node) - 1);
+          if (it.t.n < 64) my_mask &= (1ull << it.t.n) - 1;
+        }
+      }
       if (it.index >= 2) ok = ok && ta_wait(sh, &sh.u_empty[u], ((it.index >> 1) - 1) & 1);
-      const int rows = it.rows, steps = (rows + 15) >> 4;  // MMA rows in steps of 16
-      if (gt < NR) {
-        const int row = it.row0 + gt, node = row / a.group, g = row % a.group;
-        const bool live = gt < rows;
-        sh.out[u][gt] = live ? (long long)(it.t.s + node) * a.out_ld + (long long)(it.kvh * a.group + g) * HD : -1;
-        unsigned long long m = 0;
-        if (live) {
-          m = a.mask ? a.mask[it.t.s + node] : (node == 63 ? ~0ull : (2ull << node) - 1);
-          if (it.t.n < 64) m &= (1ull << it.t.n) - 1;
-        }
-        sh.mask[u][gt] = m;
-        sh.m[gt] = kUnset;
+      if (gt < mine) {
+        sh.out[u][my] = my_out;
+        nm[gt] = -kUnset;
       }
-      // q * scale * log2(e) in terms, K-major core matrices: a warp takes 8 rows,
-      // a lane 8 columns of one at a time
-      const float qs = a.scale * 1.44269504088896f;
-      const bool vec = a.q_ld % 4 == 0 && reinterpret_cast<uintptr_t>(a.q) % 16 == 0;
-      for (int g8 = w; g8 < 2 * steps; g8 += 4) {
-        const int gr = g8 * 8 + (lane & 7), row = it.row0 + gr;
-        const float* src = a.q + (size_t)(it.t.s + row / a.group) * a.q_ld +
-                           (size_t)(it.kvh * a.group + row % a.group) * HD;
-        float x[HD / 32][8];
-        float mx = 0.0f;
+      ta_group_sync(bar);
 #pragma unroll
-        for (int j = 0; j < HD / 32; j++) {
-          const int c = (j * 4 + (lane >> 3)) * 8;
-#pragma unroll
-          for (int e = 0; e < 8; e++) x[j][e] = 0.0f;
-          if (gr < rows) {
-            if (vec) {
-              const float4 f0 = *reinterpret_cast<const float4*>(src + c), f1 = *reinterpret_cast<const float4*>(src + c + 4);
-              x[j][0] = f0.x, x[j][1] = f0.y, x[j][2] = f0.z, x[j][3] = f0.w;
-              x[j][4] = f1.x, x[j][5] = f1.y, x[j][6] = f1.z, x[j][7] = f1.w;
-            } else {
-#pragma unroll
-              for (int e = 0; e < 8; e++) x[j][e] = src[c + e];
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < 8; e++) {
-            x[j][e] *= qs;
-            mx = fmaxf(mx, fabsf(x[j][e]));
-          }
-        }
-        int ex = 0;
-        if constexpr (kF16) {  // the row's largest magnitude to [2^10, 2^11)
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          if (mx > 0.0f && mx < INFINITY) {
-            frexpf(mx, &ex);
-            ex -= 11;
-          }
-        }
-        if (lane < 8) sh.c[gr] = ldexpf(1.0f, ex);
-#pragma unroll
-        for (int j = 0; j < HD / 32; j++) {
-          uint32_t y[kB][4];
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            float f0 = x[j][2 * e], f1 = x[j][2 * e + 1];
-            if constexpr (kF16) f0 = ldexpf(f0, -ex), f1 = ldexpf(f1, -ex);
-            uint32_t z[kB];
-            ta_split<kF16, kB>(f0, f1, z);
-#pragma unroll
-            for (int k = 0; k < kB; k++) y[k][e] = z[k];
-          }
-          uint8_t* dst = smem + S::kOffQ + g8 * (HD / 8 * 128) + (j * 4 + (lane >> 3)) * 128 + (lane & 7) * 16;
-#pragma unroll
-          for (int k = 0; k < kB; k++)
-            *reinterpret_cast<uint4*>(dst + k * S::kQTerm) = make_uint4(y[k][0], y[k][1], y[k][2], y[k][3]);
-        }
-      }
-      fence_proxy_async();
-      ta_group_sync(kBar);
-      if (lane == 0) ta_arrive(&sh.q_full);
-#pragma unroll
-      for (int r = 0; r < NR; r++) l[r] = 0.0f;
+      for (int r = 0; r < R / 2; r++) l[r] = make_float2(0.0f, 0.0f);
+      bool masks = false;
+#pragma unroll 1
       for (int t = it.t0; t < it.t1; t++, tile++) {
-        const int sb = tile % S::kNS, par = tile & 1;
-        ok = ok && ta_wait(sh, &sh.s_full[sb], (tile / S::kNS) & 1);
-        if (!ok) sh.fail[par] = 1;
-        ta_fence_after();
-        const uint32_t st = tmem + lanes + S::kTmS + sb * NR;
         const int p = t * kTilePos + w * 32 + lane;
-        const bool full = (t + 1) * kTilePos <= it.t.ctx;
-        // whether row r sees this lane's position
-        const int node = p - it.t.ctx;
-        auto seen = [&](int r) {
-          return full || node < 0 || (p < it.t.len && (sh.mask[u][r] >> node & 1));
-        };
-        // does a score exceed its row's maximum by more than the margin?
-        float top = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < NR / 16; c++) {
-          if (c >= steps) break;
-          float s[16];
-          ta_ld16(st + c * 16, s);
-#pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const int r = c * 16 + i;
-            const float d = fmaf(s[i], sh.c[r], -sh.m[r]);
-            if (seen(r)) top = fmaxf(top, d);
-          }
-        }
-        const bool move = ta_group_or(kBar, top > kLimit);
-        left = *reinterpret_cast<volatile int*>(&sh.fail[par]) != 0;
-        if (left) break;
-        // the last tile's product has read P, and its O, f and moved may be overwritten
-        if (tile > 0) ok = ok && ta_wait(sh, &sh.pv_done, (tile - 1) & 1);
-        if (move) {
-          // the rows' maxima over the tile: 16 rows by 32 lanes to a row a lane pair
-          float* red = reinterpret_cast<float*>(smem + S::kOffP);
-#pragma unroll
-          for (int c = 0; c < NR / 16; c++) {
-            if (c >= steps) break;
-            float s[16];
-            ta_ld16(st + c * 16, s);
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-              const int r = c * 16 + i;
-              s[i] = seen(r) ? s[i] * sh.c[r] : kUnset;
+        uint32_t vis = ~0u;  // rows that see this lane's position
+        if ((t + 1) * kTilePos > it.t.ctx) {
+          if (!masks) {  // the rows that see each node, from the nodes that each row sees
+            masks = true;
+            if (gt < mine) sh.mask[u][my] = my_mask;
+            ta_group_sync(bar);
+            if (gt < it.t.n) {
+              uint32_t v = 0;
+              for (int r = 0; r < mine; r++) v |= (uint32_t)(sh.mask[u][base + r] >> gt & 1) << r;
+              sh.vis[grp][gt] = v;
             }
-            int row = c * 16;
+            ta_group_sync(bar);
+          }
+          if (p >= it.t.ctx) vis = p < it.t.len ? sh.vis[grp][p - it.t.ctx] : 0;
+        }
+        ok = ok && ta_wait(sh, &sh.s_full, tile & 1);
+        if (!ok) sh.fail[tile & 1][grp] = 1;
+        ta_fence_after();
+        const uint32_t st = tmem + lanes + S::kTmS + base;
+        float s[R];
 #pragma unroll
-            for (int wd = 16, nn = 8; wd >= 2; wd >>= 1, nn >>= 1) {
+        for (int r = 0; r < R; r++) s[r] = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < R / 8; k++)
+          if (k < steps) ta_ld8(st + k * 8, s + k * 8);
+        ta_wait_ld(s);
+        ta_exponents<R>(s, steps, c, nm, vis);
+        // does a score exceed its row's maximum by more than the margin?
+        float top = s[0];
+#pragma unroll
+        for (int r = 1; r < R; r++) top = fmaxf(top, s[r]);
+        const bool move = ta_group_or(bar, top > kLimit);
+        left = *reinterpret_cast<volatile int*>(&sh.fail[tile & 1][grp]) != 0;
+        if (left) break;
+        float* f = sh.f[tile & 3] + base;
+        if (move) {
+          // the rows' maxima over the tile: 8 rows by 32 lanes to a row for four lanes
+#pragma unroll 1
+          for (int k = 0; k < steps; k++) {
+            float x[8];
+            ta_ld8(st + k * 8, x);
+            ta_wait_ld(x);
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = vis >> (k * 8 + i) & 1 ? x[i] * c[k * 8 + i] : kUnset;
+            int row = k * 8;
+#pragma unroll
+            for (int wd = 16, nn = 4; wd >= 4; wd >>= 1, nn >>= 1) {
               const bool up = lane & wd;
 #pragma unroll
-              for (int i = 0; i < 8; i++) {
+              for (int i = 0; i < 4; i++) {
                 if (i < nn) {
-                  const float send = up ? s[i] : s[i + nn], keep = up ? s[i + nn] : s[i];
-                  s[i] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, send, wd));
+                  const float send = up ? x[i] : x[i + nn], keep = up ? x[i + nn] : x[i];
+                  x[i] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, send, wd));
                 }
               }
               if (up) row += nn;
             }
-            s[0] = fmaxf(s[0], __shfl_xor_sync(0xffffffffu, s[0], 1));
-            if (!(lane & 1)) red[w * NR + row] = s[0];
+            x[0] = fmaxf(x[0], __shfl_xor_sync(0xffffffffu, x[0], 2));
+            x[0] = fmaxf(x[0], __shfl_xor_sync(0xffffffffu, x[0], 1));
+            if (!(lane & 3)) sh.red[grp][w][row] = x[0];
           }
-          ta_group_sync(kBar);
-          if (gt < steps * 16) {
-            const float was = sh.m[gt];
-            float mx = fmaxf(fmaxf(red[gt], red[NR + gt]), fmaxf(red[2 * NR + gt], red[3 * NR + gt]));
+          ta_group_sync(bar);
+          if (gt < mine) {
+            const float was = -nm[gt];
+            float mx = fmaxf(fmaxf(sh.red[grp][0][gt], sh.red[grp][1][gt]),
+                             fmaxf(sh.red[grp][2][gt], sh.red[grp][3][gt]));
             mx = mx > kUnset ? fmaxf(was, mx - kShift) : was;
-            sh.f[par][gt] = was == kUnset ? 0.0f : ta_exp2(was - mx);
-            sh.m[gt] = mx;
+            f[gt] = was == kUnset ? 0.0f : ta_exp2(was - mx);
+            nm[gt] = -mx;
           }
-          if (gt == 0) sh.moved[par] = 1;
-          ta_group_sync(kBar);
+          ta_group_sync(bar);
 #pragma unroll
-          for (int r = 0; r < NR; r++)
-            if (r < steps * 16) l[r] *= sh.f[par][r];
-        } else {
-          if (gt == 0) sh.moved[par] = 0;
+          for (int r = 0; r < R / 2; r++)
+            if (r < steps * 4) l[r].x *= f[2 * r], l[r].y *= f[2 * r + 1];
+#pragma unroll
+          for (int k = 0; k < R / 8; k++)
+            if (k < steps) ta_ld8(st + k * 8, s + k * 8);
+          ta_wait_ld(s);
+          ta_exponents<R>(s, steps, c, nm, vis);
+        } else if (gt < mine) {
+          f[gt] = 1.0f;
         }
-        // P = 2^(s - m + 7), its terms N-major: a lane writes 8 rows at once
-#pragma unroll
-        for (int c = 0; c < NR / 16; c++) {
-          if (c >= steps) break;
-          float s[16];
-          ta_ld16(st + c * 16, s);
-#pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const int r = c * 16 + i;
-            s[i] = ta_exp2(fmaf(s[i], sh.c[r], -sh.m[r]));
-            if (!seen(r)) s[i] = 0.0f;
-            l[r] += s[i];
-          }
-#pragma unroll
-          for (int g = 0; g < 2; g++) {
-            uint32_t y[kB][4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-              uint32_t z[kB];
-              ta_split<kF16, kB>(s[g * 8 + 2 * e], s[g * 8 + 2 * e + 1], z);
-#pragma unroll
-              for (int k = 0; k < kB; k++) y[k][e] = z[k];
-            }
-            const int pp = w * 32 + lane;
-            uint8_t* dst = smem + S::kOffP + (pp >> 3) * (NR * 16) + (c * 2 + g) * 128 + (pp & 7) * 16;
-#pragma unroll
-            for (int k = 0; k < kB; k++)
-              *reinterpret_cast<uint4*>(dst + k * S::kPTerm) = make_uint4(y[k][0], y[k][1], y[k][2], y[k][3]);
-          }
-        }
+        if (gt == 0) sh.moved[tile & 3][grp] = move;
         ta_fence_before();
+        __syncwarp();
+        if (lane == 0) ta_arrive(&sh.s_empty);
+        // P in terms, N-major (a lane writes 8 rows at once), and the row sums
+        const uint32_t pb = buf.at;
+        if (tile >= S::kNP) ok = ok && ta_wait(sh, &sh.p_empty[pb], buf.parity ^ 1);
+        buf.step();
+        const int pp = w * 32 + lane;
+        uint8_t* dst = smem + S::kOffP + pb * S::kPBuf + (pp >> 3) * (NR * 16) + (pp & 7) * 16 + base * 16;
+#pragma unroll
+        for (int k = 0; k < R / 8; k++) {
+          if (k >= steps) break;
+          uint32_t y[S::kB][4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const int r = k * 8 + e * 2;
+            const float2 x = make_float2(ta_exp2(s[r]), ta_exp2(s[r + 1]));
+            l[r / 2] = ta_add2(l[r / 2], x);
+            uint32_t z[S::kB];
+            ta_split<kF16, S::kB>(x, z);
+#pragma unroll
+            for (int q = 0; q < S::kB; q++) y[q][e] = z[q];
+          }
+#pragma unroll
+          for (int q = 0; q < S::kB; q++)
+            *reinterpret_cast<uint4*>(dst + q * S::kPTerm + k * 128) =
+                make_uint4(y[q][0], y[q][1], y[q][2], y[q][3]);
+        }
         fence_proxy_async();
         __syncwarp();
-        if (lane == 0) {
-          ta_arrive(&sh.s_empty[sb]);
-          ta_arrive(&sh.p_full);
-        }
+        if (lane == 0) ta_arrive(&sh.p_full[pb]);
       }
       if (left) break;
-      // the rows' sums over the lanes: NR rows by 32 lanes to NR / 32 rows a lane
+      // the rows' sums over the lanes: R rows by 32 lanes to a row a lane (or a few)
       {
+        float* lf = reinterpret_cast<float*>(l);
         int row = 0;
 #pragma unroll
-        for (int wd = 16, nn = NR / 2; wd >= 1; wd >>= 1, nn >>= 1) {
+        for (int wd = 16, nn = R / 2; wd >= 1; wd >>= 1, nn >>= 1) {
           if (nn >= 1) {
             const bool up = lane & wd;
 #pragma unroll
-            for (int i = 0; i < NR / 2; i++) {
+            for (int i = 0; i < R / 2; i++) {
               if (i < nn) {
-                const float send = up ? l[i] : l[i + nn], keep = up ? l[i + nn] : l[i];
-                l[i] = keep + __shfl_xor_sync(0xffffffffu, send, wd);
+                const float send = up ? lf[i] : lf[i + nn], keep = up ? lf[i + nn] : lf[i];
+                lf[i] = keep + __shfl_xor_sync(0xffffffffu, send, wd);
               }
             }
             if (up) row += nn;
           } else {
-            l[0] += __shfl_xor_sync(0xffffffffu, l[0], wd);
+            lf[0] += __shfl_xor_sync(0xffffffffu, lf[0], wd);
           }
         }
-        constexpr int kKeep = NR >= 32 ? NR / 32 : 1;
-        // fin_l as [4 warps] partials would need room: add them one warp at a time
-        for (int k = 0; k < 4; k++) {
-          if (k == w && (NR >= 32 || !(lane & 1))) {
-#pragma unroll
-            for (int i = 0; i < kKeep; i++)
-              sh.fin_l[u][row + i] = (k ? sh.fin_l[u][row + i] : 0.0f) + l[i];
-          }
-          ta_group_sync(kBar);
+        if (!(lane & (32 / R - 1))) sh.red[grp][w][row] = lf[0];
+        ta_group_sync(bar);
+        if (gt < mine) {
+          sh.fin_l[u][my] = (sh.red[grp][0][gt] + sh.red[grp][1][gt]) + (sh.red[grp][2][gt] + sh.red[grp][3][gt]);
+          sh.fin_m[u][my] = -nm[gt];
         }
-        if (gt < NR) sh.fin_m[u][gt] = sh.m[gt];
         __syncwarp();
         if (lane == 0) ta_arrive(&sh.u_full[u]);
+        ta_group_sync(bar);  // red is free again
       }
     }
-  } else if (warp < 16) {
+  } else if (warp < kWarpCopy) {
     // ---- O: a lane is a column; sums of the tiles' products in registers ----
-    const int w = warp - 12, h = w * 32 + lane;
+    ta_regs_inc<kRegsO>();
+    const int w = warp - kWarpO, h = w * 32 + lane;
     uint32_t tile = 0;
     while (w < kWarpsD && ok && it.next(a, NR)) {
       const int u = it.index & 1, steps = (it.rows + 15) >> 4;
       float o[NR];
 #pragma unroll
       for (int r = 0; r < NR; r++) o[r] = 0.0f;
+#pragma unroll 1
       for (int t = it.t0; t < it.t1 && ok; t++, tile++) {
-        ok = ta_wait(sh, &sh.pv_done, tile & 1);
+        ok = ta_wait(sh, &sh.o_full, tile & 1);
         if (!ok) break;
         ta_fence_after();
-        const int par = tile & 1;
-        const bool moved = sh.moved[par] != 0;
+        const bool moved = (sh.moved[tile & 3][0] | sh.moved[tile & 3][1]) != 0;
+        const float* f = sh.f[tile & 3];
 #pragma unroll
         for (int c = 0; c < NR / 16; c++) {
           if (c >= steps) break;
           float x[16];
           ta_ld16(tmem + lanes + S::kTmO + c * 16, x);
+          ta_wait_ld(x);
           if (moved) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) o[c * 16 + i] = fmaf(o[c * 16 + i], sh.f[par][c * 16 + i], x[i]);
-          } else {
+            for (int i = 0; i < 16; i++) o[c * 16 + i] *= f[c * 16 + i];
+          }
 #pragma unroll
-            for (int i = 0; i < 16; i++) o[c * 16 + i] += x[i];
+          for (int i = 0; i < 16; i += 2) {
+            const float2 y = ta_add2(make_float2(o[c * 16 + i], o[c * 16 + i + 1]), make_float2(x[i], x[i + 1]));
+            o[c * 16 + i] = y.x, o[c * 16 + i + 1] = y.y;
           }
         }
         ta_fence_before();
@@ -866,43 +1024,57 @@ __global__ void __launch_bounds__(kTaThreads, 1)
 #pragma unroll
       for (int i = 0; i < kWarpsD; i++) vbad |= sh.vbad[u][i][0] | (unsigned long long)sh.vbad[u][i][1] << 32;
       const bool whole = it.t0 == 0 && it.t1 == it.t.tiles;
-      float* seg = segs + (size_t)(2 * blockIdx.x + (it.t0 == 0)) * ta_seg_floats<HD, NR>();
+      if (vbad) {
 #pragma unroll
-      for (int r = 0; r < NR; r++) {
-        const long long at = sh.out[u][r];
-        if (at >= 0) {
+        for (int r = 0; r < NR; r++)
+          if (sh.mask[u][r] & vbad) o[r] = __int_as_float(0x7fc00000);
+      }
+      if (whole) {
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+          if (r >= it.rows) break;
           const float lr = sh.fin_l[u][r];
-          float x = o[r];
-          if (sh.mask[u][r] & vbad) x = __int_as_float(0x7fc00000);
-          if (whole) {
-            a.out[at + h] = lr == 0.0f ? 0.0f : x / lr;
-          } else {
-            if (w == 0 && lane == 0) seg[2 * r] = sh.fin_m[u][r], seg[2 * r + 1] = lr;
-            seg[2 * NR + r * HD + h] = x;
-          }
+          a.out[sh.out[u][r] + h] = lr == 0.0f ? 0.0f : __fdividef(o[r], lr);
+        }
+      } else {
+        float* seg = segs + (size_t)(2 * blockIdx.x + (it.t0 == 0)) * ta_seg_floats<HD, NR>();
+        if (w == 0)
+          for (int r = lane; r < it.rows; r += 32) seg[2 * r] = sh.fin_m[u][r], seg[2 * r + 1] = sh.fin_l[u][r];
+        seg += 2 * NR + h;
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+          if (r >= it.rows) break;
+          seg[r * HD] = o[r];
         }
       }
       __syncwarp();
       if (lane == 0) ta_arrive(&sh.u_empty[u]);
     }
-  } else if (warp == 16) {
+  } else if (warp == kWarpCopy) {
     // ---- copies: raw K and V tiles of the pages ----
     const uint64_t pol = evict_first_policy();
-    uint32_t n = 0, nk = 0, nv = 0;  // the slot, K and V slots issued
+    uint32_t nk = 0, nv = 0;  // K and V slots issued
+    TaRing<S::kRingK> kr;
+    TaRing<S::kRingV> vr;
     while (ok && it.next(a, NR)) {
       const int used = (it.t.len + kPageSize - 1) / kPageSize;  // the slot's pages that hold positions
+      int from = -1, ids = -1;  // a lane holds page `from + lane`
       for (int t = it.t0; t < it.t1 && ok; t++) {
-        for (int k = 0; k < S::kSlots && ok; k++, n++) {
-          const uint32_t ks = n % S::kRingK, vs = n % S::kRingV;
+        for (int k = 0; k < S::kSlots && ok; k++) {
+          const uint32_t ks = kr.at, vs = vr.at;
           const int p = t * kTilePos + k * S::kSlotPos;
-          int page = -1;
-          if (p / kPageSize < used) page = kv_page(a.c, it.t.seq, p);
+          if (from < 0 || p / kPageSize >= from + 32) {
+            from = p / kPageSize;
+            ids = from + lane < used ? kv_page(a.c, it.t.seq, (from + lane) * kPageSize) : -1;
+          }
+          const int page = __shfl_sync(0xffffffffu, ids, p / kPageSize - from);
           const size_t off = ((size_t)max(page, 0) * a.c.heads + it.kvh) * S::kTileB;
           uint8_t* kd = smem + S::kOffRing + ks * S::kSlotK;
           uint8_t* vd = smem + S::kOffV + vs * S::kSlotV;
           constexpr int kPart = S::kTileB / (kPageSize / S::kSlotPos);  // bytes of the slot's rows
           const size_t part = off + (size_t)(p % kPageSize / S::kSlotPos) * kPart;
-          if (n >= S::kRingK) ok = ta_wait(sh, &sh.k_empty[ks], ((n / S::kRingK) - 1) & 1);
+          if (nk >= S::kRingK) ok = ta_wait(sh, &sh.k_empty[ks], kr.parity ^ 1);
+          kr.step();
           if (!ok) break;
           if (page < 0) {
             if (lane == 0) ta_arrive(&sh.k_full[ks]);
@@ -917,8 +1089,9 @@ __global__ void __launch_bounds__(kTaThreads, 1)
                 tma_load_1d(kd + r * S::kRowK, a.c.k + part + (size_t)r * kRow, kRow, &sh.k_full[ks], pol);
             }
           }
-          nk = n + 1;
-          if (n >= S::kRingV) ok = ta_wait(sh, &sh.v_empty[vs], ((n / S::kRingV) - 1) & 1);
+          nk++;
+          if (nv >= S::kRingV) ok = ta_wait(sh, &sh.v_empty[vs], vr.parity ^ 1);
+          vr.step();
           if (!ok) break;
           if (lane == 0) {
             if (page < 0) {
@@ -928,7 +1101,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
               tma_load_1d(vd, a.c.v + part, kPart, &sh.v_full[vs], pol);
             }
           }
-          nv = n + 1;
+          nv++;
         }
       }
     }
@@ -937,69 +1110,86 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     if (!ok) {
       auto land = [&](uint64_t* full, uint32_t ring, uint32_t issued) {
         for (uint32_t i = issued > ring ? issued - ring : 0; i < issued; i++)
-          for (uint32_t j = 0; j < kSpinLimit >> 4 && !mbar_try_wait(&full[i % ring], (i / ring) & 1); j++) {
+          for (uint32_t j = 0; j < kPolls && !ta_try_wait(smem_u32(&full[i % ring]), (i / ring) & 1); j++) {
           }
       };
       land(sh.k_full, S::kRingK, nk);
       land(sh.v_full, S::kRingV, nv);
     }
-  } else if (lane == 0) {
+  } else {
     // ---- MMAs ----
-    constexpr int kPa[6] = {kA - 1, kA == 3 ? 1 : 0, 0, 1, 0, 0};  // terms of the products, small ones first
-    constexpr int kPb[6] = {0, kA == 3 ? 1 : kB == 2 ? 1 : 1, kA == 3 ? 2 : 0, 0, 1, 0};
-    constexpr int kPaB[3] = {0, 0, 0}, kPbB[3] = {2, 1, 0};  // one term of A
-    auto term_a = [&](int i) { return kA == 1 ? kPaB[i % 3] : kPa[i]; };
-    auto term_b = [&](int i) { return kA == 1 ? kPbB[i % 3] : kPb[i]; };
+    const uint32_t el = ta_elect();
+    const uint32_t bar0 = smem_u32(&sh);
+    auto bar_at = [&](const uint64_t* b) {
+      return bar0 + (uint32_t)(reinterpret_cast<const uint8_t*>(b) - reinterpret_cast<const uint8_t*>(&sh));
+    };
+    // the products' terms (a | b << 4, four bits each), small ones first
+    constexpr uint64_t kTerms = kA == 3   ? 0x001001201102ull
+                                : kA == 2 ? 0x000000001001ull
+                                          : 0x000000001020ull;
+    const uint64_t qdesc = ta_desc(sbase + S::kOffQ, 128, HD / 8 * 128);
+    const uint64_t pdesc = ta_desc(sbase + S::kOffP, NR * 16, 128);
     uint32_t tile = 0, qk = 0;
+    TaRing<S::kNV> vbuf;
+    TaRing<S::kNP> pbuf;
     auto qk_tile = [&](int steps) {  // scores of tile `qk`
-      const int sb = qk % S::kNS;
       bool good = ta_wait(sh, &sh.ak_full, qk & 1);
-      if (good && qk >= S::kNS) good = ta_wait(sh, &sh.s_empty[sb], ((qk / S::kNS) - 1) & 1);
+      if (good && qk > 0) good = ta_wait(sh, &sh.s_empty, (qk - 1) & 1);
       if (!good) return false;
       ta_fence_after();
-      const uint32_t d = tmem + S::kTmS + sb * NR, idesc = ta_idesc(kF16, false, steps * 16);
+      const uint32_t d = tmem + S::kTmS, idesc = ta_idesc(kF16, false, steps * 16);
+#pragma unroll 1
+      for (int i = 0; i < S::kProducts; i++) {
+        const uint32_t ta = (uint32_t)(kTerms >> (8 * i)) & 15, tb = (uint32_t)(kTerms >> (8 * i + 4)) & 15;
+        const uint32_t at = tmem + S::kTmK + ta * (HD / 2);
+        const uint64_t qd = qdesc + tb * (S::kQTerm >> 4);
 #pragma unroll
-      for (int i = 0; i < S::kProducts; i++)
-#pragma unroll
-        for (int k = 0; k < HD / 16; k++)
-          ta_mma(d, tmem + S::kTmK + term_a(i) * (HD / 2) + k * 8,
-                 ta_desc(sbase + S::kOffQ + term_b(i) * S::kQTerm + k * 256, 128, HD / 8 * 128), idesc,
-                 (i | k) != 0);
-      ta_commit(&sh.ak_empty);
-      ta_commit(&sh.s_full[sb]);
+        for (int k = 0; k < HD / 16; k++) ta_mma(d, at + k * 8, qd + k * 16, idesc, (i | k) != 0, el);
+      }
+      ta_commit(bar_at(&sh.ak_empty), el);
+      ta_commit(bar_at(&sh.s_full), el);
       qk++;
       return true;
     };
     while (ok && it.next(a, NR)) {
       const int steps = (it.rows + 15) >> 4;
-      ok = ta_wait(sh, &sh.q_full, it.index & 1) && qk_tile(steps);
+      ok = qk_tile(steps);
+#pragma unroll 1
       for (int t = it.t0; t < it.t1 && ok; t++, tile++) {
         if (t + 1 < it.t1) ok = qk_tile(steps);
-        ok = ok && ta_wait(sh, &sh.av_full, tile & 1) && ta_wait(sh, &sh.p_full, tile & 1);
+        const uint32_t vb = vbuf.at, pb = pbuf.at;
+        ok = ok && ta_wait(sh, &sh.av_full[vb], vbuf.parity) && ta_wait(sh, &sh.p_full[pb], pbuf.parity);
+        vbuf.step();
+        pbuf.step();
         if (ok && tile > 0) ok = ta_wait(sh, &sh.o_empty, (tile - 1) & 1);
         if (!ok) break;
         ta_fence_after();
-        const uint32_t d = tmem + S::kTmO, idesc = ta_idesc(kF16, true, steps * 16);
-#pragma unroll
-        for (int i = 0; i < S::kProducts; i++)
+        const uint32_t d = tmem + S::kTmO, idesc = ta_idesc(kF16, true, steps * 16), av = tmem + S::kTmV + vb * S::kVCols;
+        const uint64_t pd = pdesc + (uint64_t)(pb * (S::kPBuf >> 4));
+#pragma unroll 1
+        for (int i = 0; i < S::kProducts; i++) {
+          const uint32_t ta = (uint32_t)(kTerms >> (8 * i)) & 15, tb = (uint32_t)(kTerms >> (8 * i + 4)) & 15;
+          const uint32_t at = av + ta * (kTilePos / 2);
+          const uint64_t pt = pd + tb * (S::kPTerm >> 4);
 #pragma unroll
           for (int k = 0; k < kTilePos / 16; k++)
-            ta_mma(d, tmem + S::kTmV + term_a(i) * (kTilePos / 2) + k * 8,
-                   ta_desc(sbase + S::kOffP + term_b(i) * S::kPTerm + k * 2 * (NR * 16), NR * 16, 128), idesc,
-                   (i | k) != 0);
-        ta_commit(&sh.pv_done);
+            ta_mma(d, at + k * 8, pt + k * 2 * NR, idesc, (i | k) != 0, el);
+        }
+        ta_commit(bar_at(&sh.o_full), el);
+        ta_commit(bar_at(&sh.av_empty[vb]), el);
+        ta_commit(bar_at(&sh.p_empty[pb]), el);
       }
     }
     if (!ok) {  // MMAs in flight end before their memory goes away
-      ta_commit(&sh.drain);
-      for (uint32_t j = 0; j < kSpinLimit >> 4; j++)
-        if (mbar_try_wait(&sh.drain, 0)) break;
+      ta_commit(bar_at(&sh.drain), el);
+      for (uint32_t j = 0; j < kPolls && !ta_try_wait(smem_u32(&sh.drain), 0); j++) {
+      }
     }
   }
   if (!ok) atomicExch(a.c.err, LRS_ERR_DEVICE_TIMEOUT);
   ta_fence_before();
   __syncthreads();
-  if (warp == 17) {
+  if (warp == kWarpMma) {
     ta_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
                  "r"((uint32_t)S::kTmCols)
