@@ -103,26 +103,35 @@ struct TaShape {
 };
 
 // The part of shared memory that is not operands (kOffRow).
+// A unit: the rows of one (tree, KV head, chunk of rows) and its tiles here.
+struct TaUnit {
+  int t0, t1, tiles;  // tiles t0..t1 of `tiles`; t1 = 0 ends the list
+  int ctx, len, s, n, kvh, row0, rows;
+};
+constexpr int kUnits = 4;  // units announced ahead
+
 struct TaShared {
-  float c[4][kMaxRows];                  // score factor, per unit
+  float c[kUnits][kMaxRows];             // score factor, per unit
   float nm[kMaxRows];                    // kShift - maximum
   float f[4][kMaxRows];                  // rescaling of the earlier tiles, per tile
   float red[2][4][kMaxRows / 2];         // a softmax group's warps meet here
-  float fin_m[2][kMaxRows], fin_l[2][kMaxRows];  // per unit parity: maximum - kShift, sum
+  float fin[2][kMaxRows];                // per unit parity: the factor of a row's output
   unsigned long long mask[2][kMaxRows];  // the row's node mask
   uint32_t vis[2][LRS_TREE_MAX_NODES];   // rows of a softmax group that see a node
-  long long out[2][kMaxRows];            // offset of the row's output
+  float* out[2][kMaxRows];               // the row's output
   unsigned vbad[2][4][2];                // nodes whose V is not finite, per warp that reads V
   int moved[4][2];
   int fail[2][2];  // a softmax warp's wait gave up, per tile parity and group
+  TaUnit unit[kUnits];
   uint64_t k_full[8], k_empty[8], v_full[8], v_empty[8];
   uint64_t ak_full, ak_empty, s_full, s_empty, o_full, o_empty, drain;
   uint64_t av_full[2], av_empty[2], p_full[2], p_empty[2], u_full[2], u_empty[2];
+  uint64_t unit_full[kUnits], unit_empty[kUnits];
   int abort;
   uint32_t tmem;
   // the schedule
-  int first, last;       // this CTA's tiles
-  int tree, unit, tile;  // of `first`
+  int first, last;              // this CTA's tiles
+  int tree, unit0, tile;        // of `first`: tree, unit of the tree, tile of the unit
   int active;
 };
 static_assert(sizeof(TaShared) <= kSharedBytes, "shared state");
@@ -357,50 +366,62 @@ __host__ __device__ constexpr size_t ta_seg_floats() {
   return 2 * NR + (size_t)NR * HD;
 }
 
-// The units (tree, KV head, chunk of rows) of a CTA, tile range by tile range.
-struct TaIter {
-  int tree, unit, tile;  // next unit, its first tile here
-  int left;              // tiles left
-  TaTree t;
-  int t0, t1, index;     // the current unit's tiles, its number in this CTA
-  int kvh, row0, rows;
-  bool loaded;
-  __device__ __forceinline__ void begin(const TaShared& sh) {
-    tree = sh.tree;
-    unit = sh.unit;
-    tile = sh.tile;
-    left = sh.last - sh.first;
-    index = -1;
-    loaded = false;
-  }
-  __device__ __forceinline__ bool next(const TreeArgs& a, int nr) {
-    if (left <= 0) return false;
-    while (!loaded || unit >= t.chunks * a.c.heads) {
-      if (loaded) tree++, unit = 0;
-      if (tree >= a.n_trees) return false;  // the arrays changed under the kernel
-      t.load(a, tree, nr);
-      loaded = true;
-    }
-    kvh = unit / t.chunks;
-    const int share = t.share(a);
-    row0 = (unit % t.chunks) * share;
-    rows = min(share, t.n * a.group - row0);
-    t0 = tile;
-    t1 = min(t.tiles, t0 + left);
-    left -= t1 - t0;
+// The units as a warp takes them from the list.
+struct TaFeed {
+  TaUnit u;
+  int index = -1;  // number of the unit in this CTA
+  TaRing<kUnits> ring;
+  // False at the end of the list, or (ok = false) when the wait gave up.
+  __device__ __forceinline__ bool next(TaShared& sh, int lane, bool& ok) {
+    ok = ok && ta_wait(sh, &sh.unit_full[ring.at], ring.parity);
+    if (!ok) return false;
+    u = sh.unit[ring.at];
+    __syncwarp();
+    if (lane == 0) ta_arrive(&sh.unit_empty[ring.at]);
+    ring.step();
     index++;
-    unit++;
-    tile = 0;
-    return true;
+    return u.t1 > 0;
   }
 };
 
-// A slot's positions of V into tensor memory: lane = column h of the head.  TAIL:
-// positions past the end become zeros, and so do nodes with a value that is not
-// finite, which are noted (their weight may be a zero that must stay one).
-template <int HD, int DT, int NR, bool TAIL>
-__device__ __forceinline__ void decode_v(const uint8_t* raw, uint32_t col, int w, int lane, int p0,
-                                         int ctx, int len, unsigned* vbad) {
+// The last tile's positions of V past the end, and nodes with a value that is not
+// finite, become zeros (their weight may be a zero that must stay one); the
+// nodes are noted.  A warp mends its own columns of the raw slot.
+template <int HD, int DT, int POS>
+__device__ __forceinline__ void mend_v(uint8_t* raw, int w, int lane, int p0, int ctx, int len, unsigned* vbad) {
+  if constexpr (DT == LRS_KV_Q8_0) {
+    uint16_t* d = reinterpret_cast<uint16_t*>(raw + q8_v_scale(HD, 0, w));
+#pragma unroll 1
+    for (int r = lane; r < POS; r += 32) {
+      const int p = p0 + r;
+      const bool bad = p >= ctx && (d[r] & 0x7c00) == 0x7c00;
+      if (p >= len || bad) {
+        d[r] = 0;
+        if (p < len) atomicOr(&vbad[(p - ctx) >> 5], 1u << ((p - ctx) & 31));
+      }
+    }
+  } else {
+    const int h = w * 32 + lane;
+#pragma unroll 1
+    for (int r = max(0, ctx - p0); r < POS; r++) {
+      const int p = p0 + r;
+      uint16_t* b = reinterpret_cast<uint16_t*>(raw) + r * HD + h;
+      uint32_t* f = reinterpret_cast<uint32_t*>(raw) + r * HD + h;
+      const bool bad = DT == LRS_KV_BF16 ? (*b & 0x7f80) == 0x7f80 : (*f & 0x7f800000u) == 0x7f800000u;
+      if (p >= len || bad) {
+        if (DT == LRS_KV_BF16) *b = 0;
+        else *f = 0;
+        if (p < len) atomicOr(&vbad[(p - ctx) >> 5], 1u << ((p - ctx) & 31));
+      }
+    }
+  }
+  fence_proxy_async();  // the slot is refilled by copies later
+  __syncwarp();
+}
+
+// A slot's positions of V into tensor memory: lane = column of the head.
+template <int HD, int DT, int NR>
+__device__ __forceinline__ void decode_v(const uint8_t* raw, uint32_t col, int w, int lane) {
   using S = TaShape<HD, DT, NR>;
   const int h = w * 32 + lane;
 #pragma unroll 1
@@ -412,48 +433,26 @@ __device__ __forceinline__ void decode_v(const uint8_t* raw, uint32_t col, int w
       for (int i = 0; i < 8; i++) {
         const int r = g * 32 + i * 4;
         if (i % 2 == 0) d8 = *reinterpret_cast<const uint4*>(raw + q8_v_scale(HD, r, w));
-        uint2 dd = i % 2 ? make_uint2(d8.z, d8.w) : make_uint2(d8.x, d8.y);
-        if constexpr (TAIL) {
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            uint32_t& d = j < 2 ? dd.x : dd.y;
-            const uint32_t keep = j & 1 ? 0x0000ffffu : 0xffff0000u, inf = j & 1 ? 0x7c000000u : 0x7c00u;
-            const int p = p0 + r + j;
-            const bool bad = (d & inf) == inf && p >= ctx;
-            if (p >= len || bad) {
-              d &= keep;
-              if (p < len && lane == 0) atomicOr(&vbad[(p - ctx) >> 5], 1u << ((p - ctx) & 31));
-            }
-          }
-        }
         const uint32_t cw = *reinterpret_cast<const uint32_t*>(raw + q8_v_code(HD, r, h));
         uint32_t hi[2], lo[2];
-        ta_q8(cw, ta_u2(dd.x), ta_u2(dd.y), hi, lo);
+        ta_q8(cw, ta_u2(i % 2 ? d8.z : d8.x), ta_u2(i % 2 ? d8.w : d8.y), hi, lo);
         x[0][i * 2] = hi[0], x[0][i * 2 + 1] = hi[1];
         x[1][i * 2] = lo[0], x[1][i * 2 + 1] = lo[1];
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 16; i++) {
-        float f[2];
+        const int r = g * 32 + i * 2;
+        if constexpr (DT == LRS_KV_BF16) {
+          const uint16_t* b = reinterpret_cast<const uint16_t*>(raw) + r * HD + h;
+          x[0][i] = (uint32_t)b[0] | (uint32_t)b[HD] << 16;
+        } else {
+          const float* f = reinterpret_cast<const float*>(raw) + r * HD + h;
+          uint32_t y[S::kA];
+          ta_split<false, S::kA>(make_float2(f[0], f[HD]), y);
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-          const int r = g * 32 + i * 2 + j, p = p0 + r;
-          f[j] = DT == LRS_KV_BF16
-                     ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(raw)[r * HD + h] << 16)
-                     : reinterpret_cast<const float*>(raw)[r * HD + h];
-          if constexpr (TAIL) {
-            const bool bad = (__float_as_uint(f[j]) & 0x7f800000u) == 0x7f800000u && p >= ctx;
-            if (p >= len || bad) {
-              f[j] = 0.0f;
-              if (p < len) atomicOr(&vbad[(p - ctx) >> 5], 1u << ((p - ctx) & 31));
-            }
-          }
+          for (int q = 0; q < S::kA; q++) x[q][i] = y[q];
         }
-        uint32_t y[S::kA];
-        ta_split<false, S::kA>(make_float2(f[0], f[1]), y);
-#pragma unroll
-        for (int q = 0; q < S::kA; q++) x[q][i] = y[q];
       }
     }
 #pragma unroll
@@ -485,7 +484,7 @@ __device__ __forceinline__ void ta_exponents(float (&s)[R], int steps, const flo
 // takes 8 rows, a lane 8 columns of one at a time.  For f16 terms a power of two
 // brings a row's largest magnitude to [2^10, 2^11); c is its inverse.
 template <int HD, int DT, int NR>
-__device__ __forceinline__ void load_q(const TreeArgs& a, const TaIter& it, uint8_t* smem, float* c,
+__device__ __forceinline__ void load_q(const TreeArgs& a, const TaUnit& it, uint8_t* smem, float* c,
                                        int w, int lane) {
   using S = TaShape<HD, DT, NR>;
   const float qs = a.scale * 1.44269504088896f;
@@ -494,7 +493,7 @@ __device__ __forceinline__ void load_q(const TreeArgs& a, const TaIter& it, uint
 #pragma unroll 1
   for (int g8 = w; g8 < groups; g8 += 4) {
     const int gr = g8 * 8 + (lane & 7), row = it.row0 + gr;
-    const float* src = a.q + (size_t)(it.t.s + row / a.group) * a.q_ld +
+    const float* src = a.q + (size_t)(it.s + row / a.group) * a.q_ld +
                        (size_t)(it.kvh * a.group + row % a.group) * HD + (lane >> 3) * 8;
     float x[HD / 32][8];
 #pragma unroll
@@ -570,11 +569,13 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     const int per = (a.n_trees + kTaThreads - 1) / kTaThreads;
     int mine = 0;
     TaTree tr;
+#pragma unroll 1
     for (int i = 0; i < per; i++) {
       const int t = tid * per + i;
       if (t < a.n_trees && tr.load(a, t, NR)) mine += tr.total(a);
     }
     int incl = mine;
+#pragma unroll 1
     for (int o = 1; o < 32; o <<= 1) {
       const int x = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += x;
@@ -583,6 +584,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     if (tid == 0) sh.active = 0;
     __syncthreads();
     int before = incl - mine, total = 0;
+#pragma unroll 1
     for (int w = 0; w < kTaThreads / 32; w++) {
       if (w < warp) before += wsum[w];
       total += wsum[w];
@@ -596,13 +598,14 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       const int first = start(c);
       if (before <= first && first < before + mine) {  // the thread that holds the first tile's tree
         int at = before;
+#pragma unroll 1
         for (int i = 0; i < per; i++) {
           const int t = tid * per + i;
           if (t >= a.n_trees || (per > 1 && !tr.load(a, t, NR))) continue;
           if (first < at + tr.total(a)) {
             const int unit = (first - at) / tr.tiles, unit0 = at + unit * tr.tiles;
             sh.tree = t;
-            sh.unit = unit;
+            sh.unit0 = unit;
             sh.tile = first - unit0;
             sh.first = first;
             sh.last = start(c + 1);
@@ -610,6 +613,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
             // this CTA starts inside a unit: the first such CTA describes it
             if (first > unit0 && start(c - 1) <= unit0) {
               d.nseg = 2;
+#pragma unroll 1
               while (start(c + d.nseg - 1) < unit0 + tr.tiles) d.nseg++;
               const int share = tr.share(a);
               d.kvh = unit / tr.chunks;
@@ -629,6 +633,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     segs = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + gridDim.x * sizeof(TaDesc));
   }
   if (tid == 0) {
+#pragma unroll 1
     for (int i = 0; i < 8; i++) {
       mbar_init(&sh.k_full[i], 1);
       mbar_init(&sh.k_empty[i], S::kSlotPos / 32);
@@ -651,6 +656,11 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       mbar_init(&sh.u_empty[i], kWarpsD);
       sh.fail[i][0] = sh.fail[i][1] = 0;
     }
+#pragma unroll 1
+    for (int i = 0; i < kUnits; i++) {
+      mbar_init(&sh.unit_full[i], 1);
+      mbar_init(&sh.unit_empty[i], 4 + 8 + 2 * kWarpsD + 1);  // the warps that take units
+    }
     sh.abort = 0;
     fence_barrier_init();
   }
@@ -670,8 +680,8 @@ __global__ void __launch_bounds__(kTaThreads, 1)
   const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
   const uint32_t sbase = smem_u32(smem);
   const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;  // this warp's lanes of tensor memory
-  TaIter it;
-  it.begin(sh);
+  TaFeed feed;
+  const TaUnit& it = feed.u;
   bool ok = true;
 
   if (warp < kWarpV) {
@@ -680,11 +690,11 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     uint32_t tile = 0;
     TaRing<S::kRingK> ring;
     ring.at = warp * 32 / S::kSlotPos;
-    while (ok && it.next(a, NR)) {
+    while (feed.next(sh, lane, ok)) {
       // the last unit's scores are done with q and its factors
       if (tile > 0) ok = ta_wait(sh, &sh.ak_empty, (tile - 1) & 1);
       if (!ok) break;
-      load_q<HD, DT, NR>(a, it, smem, sh.c[it.index & 3], warp, lane);
+      load_q<HD, DT, NR>(a, it, smem, sh.c[feed.index % kUnits], warp, lane);
       fence_proxy_async();
       for (int t = it.t0; t < it.t1 && ok; t++, tile++) {
         const uint32_t slot = ring.at;
@@ -759,31 +769,30 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     uint32_t tile = 0;
     TaRing<S::kRingV> ring;
     TaRing<S::kNV> buf;
-    while (w < kWarpsD && ok && it.next(a, NR)) {
+    while (w < kWarpsD && feed.next(sh, lane, ok)) {
       // the words of the unit before last have been read
-      if (it.index >= 2) ok = ta_wait(sh, &sh.u_empty[it.index & 1], ((it.index >> 1) - 1) & 1);
-      unsigned* vbad = sh.vbad[it.index & 1][w];
+      const int par = feed.index & 1;
+      if (feed.index >= 2) ok = ta_wait(sh, &sh.u_empty[par], ((feed.index >> 1) - 1) & 1);
+      unsigned* vbad = sh.vbad[par][w];
       if (lane < 2) vbad[lane] = 0;
       __syncwarp();
+#pragma unroll 1
       for (int t = it.t0; t < it.t1 && ok; t++, tile++) {
         const uint32_t vb = buf.at;
         if (tile >= S::kNV) ok = ta_wait(sh, &sh.av_empty[vb], buf.parity ^ 1);
         buf.step();
         ta_fence_after();
-        const bool tail = (t + 1) * kTilePos > it.t.ctx;  // holds nodes, or positions past the end
 #pragma unroll 1
         for (int k = 0; k < S::kSlots && ok; k++) {
           const uint32_t slot = ring.at;
           ok = ta_wait(sh, &sh.v_full[slot], ring.parity);
           ring.step();
           if (!ok) break;
-          const uint8_t* raw = smem + S::kOffV + slot * S::kSlotV;
+          uint8_t* raw = smem + S::kOffV + slot * S::kSlotV;
           const int p0 = t * kTilePos + k * S::kSlotPos;
-          const uint32_t col = tmem + lanes + S::kTmV + vb * S::kVCols + k * (S::kSlotPos / 2);
-          if (tail)
-            decode_v<HD, DT, NR, true>(raw, col, w, lane, p0, it.t.ctx, it.t.len, vbad);
-          else
-            decode_v<HD, DT, NR, false>(raw, col, w, lane, p0, it.t.ctx, it.t.len, vbad);
+          if (p0 + S::kSlotPos > it.ctx)  // holds nodes, or positions past the end
+            mend_v<HD, DT, S::kSlotPos>(raw, w, lane, p0, it.ctx, it.len, vbad);
+          decode_v<HD, DT, NR>(raw, tmem + lanes + S::kTmV + vb * S::kVCols + k * (S::kSlotPos / 2), w, lane);
           __syncwarp();
           if (lane == 0) ta_arrive(&sh.v_empty[slot]);
         }
@@ -801,74 +810,79 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     float2 l[R / 2];
     uint32_t tile = 0;
     TaRing<S::kNP> buf;
-    bool left = false;
     // the four warps meet at barriers: one whose wait gave up goes on (on stale
     // data, in bounds) to the next vote, where they leave together
-    while (!left && it.next(a, NR)) {
-      const int u = it.index & 1;
+    for (;;) {
+      const bool more = feed.next(sh, lane, ok);
+      const int u = feed.index & 1;
       const int steps = (it.rows + 15) >> 4, base = grp * steps * 8;  // steps of 8 rows from `base`
-      const float* c = sh.c[it.index & 3] + base;
+      const float* c = sh.c[feed.index % kUnits] + base;
       float* nm = sh.nm + base;
       const int my = base + gt;  // the row that this thread keeps, one of the first `mine`
       const int mine = steps * 8;
+      const bool whole = it.t0 == 0 && it.t1 == it.tiles;
+      float* seg = segs + (size_t)(2 * blockIdx.x + (it.t0 == 0)) * ta_seg_floats<HD, NR>();
       unsigned long long my_mask = 0;
-      long long my_out = 0;
-      if (gt < mine) {
+      float* my_out = nullptr;
+      if (more && gt < mine && my < it.rows) {
         const int row = it.row0 + my, node = row / a.group, g = row % a.group;
-        my_out = (long long)(it.t.s + node) * a.out_ld + (long long)(it.kvh * a.group + g) * HD;
-        if (my < it.rows) {
-          my_mask = a.mask ? a.mask[it.t.s + node] : (node == 63 ? ~0ull : (2ull << node) - 1);
-          if (it.t.n < 64) my_mask &= (1ull << it.t.n) - 1;
-        }
+        my_out = whole ? a.out + (size_t)(it.s + node) * a.out_ld + (size_t)(it.kvh * a.group + g) * HD
+                       : seg + 2 * NR + my * HD;
+        my_mask = a.mask ? a.mask[it.s + node] : (node == 63 ? ~0ull : (2ull << node) - 1);
+        if (it.n < 64) my_mask &= (1ull << it.n) - 1;
       }
-      if (it.index >= 2) ok = ok && ta_wait(sh, &sh.u_empty[u], ((it.index >> 1) - 1) & 1);
-      if (gt < mine) {
+      if (more && feed.index >= 2) ok = ok && ta_wait(sh, &sh.u_empty[u], ((feed.index >> 1) - 1) & 1);
+      if (more && gt < mine) {
         sh.out[u][my] = my_out;
         nm[gt] = -kUnset;
       }
-      ta_group_sync(bar);
+      if (ta_group_or(bar, !more || !ok)) break;
 #pragma unroll
       for (int r = 0; r < R / 2; r++) l[r] = make_float2(0.0f, 0.0f);
-      bool masks = false;
+      bool masks = false, left = false;
 #pragma unroll 1
       for (int t = it.t0; t < it.t1; t++, tile++) {
         const int p = t * kTilePos + w * 32 + lane;
         uint32_t vis = ~0u;  // rows that see this lane's position
-        if ((t + 1) * kTilePos > it.t.ctx) {
+        if ((t + 1) * kTilePos > it.ctx) {
           if (!masks) {  // the rows that see each node, from the nodes that each row sees
             masks = true;
             if (gt < mine) sh.mask[u][my] = my_mask;
             ta_group_sync(bar);
-            if (gt < it.t.n) {
+            if (gt < it.n) {
               uint32_t v = 0;
+#pragma unroll 1
               for (int r = 0; r < mine; r++) v |= (uint32_t)(sh.mask[u][base + r] >> gt & 1) << r;
               sh.vis[grp][gt] = v;
             }
             ta_group_sync(bar);
           }
-          if (p >= it.t.ctx) vis = p < it.t.len ? sh.vis[grp][p - it.t.ctx] : 0;
+          if (p >= it.ctx) vis = p < it.len ? sh.vis[grp][p - it.ctx] : 0;
         }
         ok = ok && ta_wait(sh, &sh.s_full, tile & 1);
         if (!ok) sh.fail[tile & 1][grp] = 1;
         ta_fence_after();
         const uint32_t st = tmem + lanes + S::kTmS + base;
         float s[R];
-#pragma unroll
-        for (int r = 0; r < R; r++) s[r] = -INFINITY;
-#pragma unroll
-        for (int k = 0; k < R / 8; k++)
-          if (k < steps) ta_ld8(st + k * 8, s + k * 8);
-        ta_wait_ld(s);
-        ta_exponents<R>(s, steps, c, nm, vis);
-        // does a score exceed its row's maximum by more than the margin?
-        float top = s[0];
-#pragma unroll
-        for (int r = 1; r < R; r++) top = fmaxf(top, s[r]);
-        const bool move = ta_group_or(bar, top > kLimit);
-        left = *reinterpret_cast<volatile int*>(&sh.fail[tile & 1][grp]) != 0;
-        if (left) break;
         float* f = sh.f[tile & 3] + base;
-        if (move) {
+        bool move = false;
+#pragma unroll 1
+        for (;;) {
+#pragma unroll
+          for (int r = 0; r < R; r++) s[r] = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < R / 8; k++)
+            if (k < steps) ta_ld8(st + k * 8, s + k * 8);
+          ta_wait_ld(s);
+          ta_exponents<R>(s, steps, c, nm, vis);
+          if (move) break;
+          // does a score exceed its row's maximum by more than the margin?
+          float top = s[0];
+#pragma unroll
+          for (int r = 1; r < R; r++) top = fmaxf(top, s[r]);
+          move = ta_group_or(bar, top > kLimit);
+          left = *reinterpret_cast<volatile int*>(&sh.fail[tile & 1][grp]) != 0;
+          if (left || !move) break;
           // the rows' maxima over the tile: 8 rows by 32 lanes to a row for four lanes
 #pragma unroll 1
           for (int k = 0; k < steps; k++) {
@@ -907,14 +921,9 @@ __global__ void __launch_bounds__(kTaThreads, 1)
 #pragma unroll
           for (int r = 0; r < R / 2; r++)
             if (r < steps * 4) l[r].x *= f[2 * r], l[r].y *= f[2 * r + 1];
-#pragma unroll
-          for (int k = 0; k < R / 8; k++)
-            if (k < steps) ta_ld8(st + k * 8, s + k * 8);
-          ta_wait_ld(s);
-          ta_exponents<R>(s, steps, c, nm, vis);
-        } else if (gt < mine) {
-          f[gt] = 1.0f;
         }
+        if (left) break;
+        if (!move && gt < mine) f[gt] = 1.0f;
         if (gt == 0) sh.moved[tile & 3][grp] = move;
         ta_fence_before();
         __syncwarp();
@@ -972,8 +981,9 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         if (!(lane & (32 / R - 1))) sh.red[grp][w][row] = lf[0];
         ta_group_sync(bar);
         if (gt < mine) {
-          sh.fin_l[u][my] = (sh.red[grp][0][gt] + sh.red[grp][1][gt]) + (sh.red[grp][2][gt] + sh.red[grp][3][gt]);
-          sh.fin_m[u][my] = -nm[gt];
+          const float sum = (sh.red[grp][0][gt] + sh.red[grp][1][gt]) + (sh.red[grp][2][gt] + sh.red[grp][3][gt]);
+          sh.fin[u][my] = !whole ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+          if (!whole && my < it.rows) seg[2 * my] = -nm[gt], seg[2 * my + 1] = sum;
         }
         __syncwarp();
         if (lane == 0) ta_arrive(&sh.u_full[u]);
@@ -985,8 +995,8 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     ta_regs_inc<kRegsO>();
     const int w = warp - kWarpO, h = w * 32 + lane;
     uint32_t tile = 0;
-    while (w < kWarpsD && ok && it.next(a, NR)) {
-      const int u = it.index & 1, steps = (it.rows + 15) >> 4;
+    while (w < kWarpsD && feed.next(sh, lane, ok)) {
+      const int u = feed.index & 1, steps = (it.rows + 15) >> 4;
       float o[NR];
 #pragma unroll
       for (int r = 0; r < NR; r++) o[r] = 0.0f;
@@ -1018,34 +1028,20 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         if (lane == 0) ta_arrive(&sh.o_empty);
       }
       if (!ok) break;
-      ok = ta_wait(sh, &sh.u_full[u], (it.index >> 1) & 1);
+      ok = ta_wait(sh, &sh.u_full[u], (feed.index >> 1) & 1);
       if (!ok) break;
       unsigned long long vbad = 0;
 #pragma unroll
       for (int i = 0; i < kWarpsD; i++) vbad |= sh.vbad[u][i][0] | (unsigned long long)sh.vbad[u][i][1] << 32;
-      const bool whole = it.t0 == 0 && it.t1 == it.t.tiles;
       if (vbad) {
 #pragma unroll
         for (int r = 0; r < NR; r++)
           if (sh.mask[u][r] & vbad) o[r] = __int_as_float(0x7fc00000);
       }
-      if (whole) {
 #pragma unroll
-        for (int r = 0; r < NR; r++) {
-          if (r >= it.rows) break;
-          const float lr = sh.fin_l[u][r];
-          a.out[sh.out[u][r] + h] = lr == 0.0f ? 0.0f : __fdividef(o[r], lr);
-        }
-      } else {
-        float* seg = segs + (size_t)(2 * blockIdx.x + (it.t0 == 0)) * ta_seg_floats<HD, NR>();
-        if (w == 0)
-          for (int r = lane; r < it.rows; r += 32) seg[2 * r] = sh.fin_m[u][r], seg[2 * r + 1] = sh.fin_l[u][r];
-        seg += 2 * NR + h;
-#pragma unroll
-        for (int r = 0; r < NR; r++) {
-          if (r >= it.rows) break;
-          seg[r * HD] = o[r];
-        }
+      for (int r = 0; r < NR; r++) {
+        if (r % 16 == 0 && r >= it.rows) break;
+        if (r < it.rows) sh.out[u][r][h] = o[r] * sh.fin[u][r];
       }
       __syncwarp();
       if (lane == 0) ta_arrive(&sh.u_empty[u]);
@@ -1056,19 +1052,53 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     uint32_t nk = 0, nv = 0;  // K and V slots issued
     TaRing<S::kRingK> kr;
     TaRing<S::kRingV> vr;
-    while (ok && it.next(a, NR)) {
-      const int used = (it.t.len + kPageSize - 1) / kPageSize;  // the slot's pages that hold positions
+    TaRing<kUnits> list;
+    TaTree tr;
+    int tree = sh.tree, unit = sh.unit0, tile = sh.tile, left = sh.last - sh.first;
+    bool loaded = false;
+#pragma unroll 1
+    for (uint32_t index = 0; ok; index++) {
+      // the next unit (the last entry of the list is empty)
+      while (left > 0 && (!loaded || unit >= tr.chunks * a.c.heads)) {
+        if (loaded) tree++, unit = 0;
+        if (tree >= a.n_trees) left = 0;  // the arrays changed under the kernel
+        else tr.load(a, tree, NR);
+        loaded = true;
+      }
+      TaUnit un{};
+      if (left > 0) {
+        const int share = tr.share(a);
+        un.t0 = tile, un.t1 = min(tr.tiles, tile + left), un.tiles = tr.tiles;
+        un.ctx = tr.ctx, un.len = tr.len, un.s = tr.s, un.n = tr.n;
+        un.kvh = unit / tr.chunks;
+        un.row0 = unit % tr.chunks * share;
+        un.rows = min(share, tr.n * a.group - un.row0);
+        left -= un.t1 - un.t0;
+        unit++;
+        tile = 0;
+      }
+      if (index >= kUnits) ok = ta_wait(sh, &sh.unit_empty[list.at], list.parity ^ 1);
+      if (!ok) break;
+      if (lane == 0) {
+        sh.unit[list.at] = un;
+        ta_arrive(&sh.unit_full[list.at]);
+      }
+      list.step();
+      if (un.t1 == 0) break;
+      const int used = (un.len + kPageSize - 1) / kPageSize;  // the slot's pages that hold positions
       int from = -1, ids = -1;  // a lane holds page `from + lane`
-      for (int t = it.t0; t < it.t1 && ok; t++) {
+#pragma unroll 1
+      for (int t = un.t0; t < un.t1 && ok; t++) {
+#pragma unroll 1
         for (int k = 0; k < S::kSlots && ok; k++) {
           const uint32_t ks = kr.at, vs = vr.at;
           const int p = t * kTilePos + k * S::kSlotPos;
           if (from < 0 || p / kPageSize >= from + 32) {
             from = p / kPageSize;
-            ids = from + lane < used ? kv_page(a.c, it.t.seq, (from + lane) * kPageSize) : -1;
+            ids = from + lane < used ? kv_page(a.c, tr.seq, (from + lane) * kPageSize) : -1;
           }
           const int page = __shfl_sync(0xffffffffu, ids, p / kPageSize - from);
-          const size_t off = ((size_t)max(page, 0) * a.c.heads + it.kvh) * S::kTileB;
+          const size_t off = ((size_t)max(page, 0) * a.c.heads + un.kvh) * S::kTileB;
           uint8_t* kd = smem + S::kOffRing + ks * S::kSlotK;
           uint8_t* vd = smem + S::kOffV + vs * S::kSlotV;
           constexpr int kPart = S::kTileB / (kPageSize / S::kSlotPos);  // bytes of the slot's rows
@@ -1151,7 +1181,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       qk++;
       return true;
     };
-    while (ok && it.next(a, NR)) {
+    while (feed.next(sh, lane, ok)) {
       const int steps = (it.rows + 15) >> 4;
       ok = qk_tile(steps);
 #pragma unroll 1
