@@ -49,9 +49,10 @@ namespace {
 
 constexpr int kTilePos = 128;   // positions of a tile: the lanes of an MMA
 constexpr int kMaxRows = 64;    // rows (node, head) of a CTA's unit
-// warps: K 0-3, V 4-7, the softmax 8-11 and 12-15 (half of the rows each), O
-// 16-19, the copies 20, the MMAs 21
-constexpr int kWarpV = 4, kWarpS = 8, kWarpO = 16, kWarpCopy = 20, kWarpMma = 21;
+// warps: K 0-3, V 4-7, the softmax 8-11, V (up to 32 rows: half of the positions
+// each) or the softmax (64: half of the rows each) 12-15, O 16-19, the copies 20,
+// the MMAs 21
+constexpr int kWarpV = 4, kWarpS = 8, kWarp2 = 12, kWarpO = 16, kWarpCopy = 20, kWarpMma = 21;
 constexpr int kTaThreads = 32 * 22;
 // Registers a thread: 80 at launch; the groups that decode K and V give 8 each to
 // the one that holds O (an increase beyond what was given would wait for good).
@@ -67,6 +68,8 @@ struct TaShape {
   static constexpr int kA = DT == LRS_KV_F32 ? 3 : DT == LRS_KV_BF16 ? 1 : 2;  // terms of K, V
   static constexpr int kB = DT == LRS_KV_Q8_0 ? 2 : 3;                        // terms of q, P
   static constexpr bool kF16 = DT == LRS_KV_Q8_0;
+  static constexpr int kSG = NR == 64 ? 2 : 1, kVG = 3 - kSG;  // softmax groups, V groups
+  static constexpr int kR = NR / kSG;                          // rows of a softmax group
   static constexpr int kProducts = DT == LRS_KV_F32 ? 6 : 3;
   // tensor memory columns: V is double-buffered where it fits
   static constexpr int kVCols = kA * kTilePos / 2;
@@ -90,16 +93,18 @@ struct TaShape {
       kOffP + 2 * kPBuf + kSharedBytes + 2 * kSlots * (kSlotK + kSlotV) <= kSmemMost ? 2 : 1;
   static constexpr int kOffRow = kOffP + kNP * kPBuf;
   static constexpr int kOffRing = kOffRow + kSharedBytes;
-  // a K slot has one reader, or two that read one tile's halves: whole tiles of
-  // slots keep a slot's readers the same, so that none misses one of its phases
+  // where a tile's slots have different readers, whole tiles of slots keep a
+  // slot's readers the same, so that none misses one of its phases
   static constexpr int kRoom = kSmemMost - kOffRing;
-  static constexpr int kRing0 = (kRoom / (kSlotK + kSlotV) + kSlots - 1) / kSlots * kSlots;
+  static constexpr int kTiles = kRoom / (kSlots * (kSlotK + kSlotV));
+  static constexpr int kRing0 = kVG == 2 ? kTiles * kSlots : (kRoom / (kSlotK + kSlotV) + kSlots - 1) / kSlots * kSlots;
   static constexpr int kRingK = kRing0 > 8 ? 8 : kRing0;
-  static constexpr int kRingV0 = (kRoom - kRingK * kSlotK) / kSlotV;
+  static constexpr int kRingV0 = kVG == 2 ? kRingK : (kRoom - kRingK * kSlotK) / kSlotV;
   static constexpr int kRingV = kRingV0 > 8 ? 8 : kRingV0;
   static constexpr int kOffV = kOffRing + kRingK * kSlotK;
   static constexpr int kSmem = kOffV + kRingV * kSlotV;
-  static_assert(kRingK % kSlots == 0 && kRingV >= 2 && kSlotK % 16 == 0 && kSlotV % 16 == 0, "ring");
+  static_assert(kRingK % kSlots == 0 && kRingK >= kSlots && kRingV >= 2 && kSmem <= kSmemMost &&
+                kSlotK % 16 == 0 && kSlotV % 16 == 0, "ring");
 };
 
 // The part of shared memory that is not operands (kOffRow).
@@ -114,12 +119,12 @@ struct TaShared {
   float c[kUnits][kMaxRows];             // score factor, per unit
   float nm[kMaxRows];                    // kShift - maximum
   float f[4][kMaxRows];                  // rescaling of the earlier tiles, per tile
-  float red[2][4][kMaxRows / 2];         // a softmax group's warps meet here
+  float red[2][4][32];                  // a softmax group's warps meet here
   float fin[2][kMaxRows];                // per unit parity: the factor of a row's output
   unsigned long long mask[2][kMaxRows];  // the row's node mask
   uint32_t vis[2][LRS_TREE_MAX_NODES];   // rows of a softmax group that see a node
   float* out[2][kMaxRows];               // the row's output
-  unsigned vbad[2][4][2];                // nodes whose V is not finite, per warp that reads V
+  unsigned vbad[2][8][2];                // nodes whose V is not finite, per warp that reads V
   int moved[4][2];
   int fail[2][2];  // a softmax warp's wait gave up, per tile parity and group
   TaUnit unit[kUnits];
@@ -560,7 +565,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
   constexpr int kWarpsD = HD / 32;  // warps that own columns of V
   extern __shared__ __align__(128) uint8_t smem[];
   TaShared& sh = *reinterpret_cast<TaShared*>(smem + S::kOffRow);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   float* segs = static_cast<float*>(a.workspace);
 
   // ---- the schedule: every CTA finds its share of all tiles ----
@@ -643,23 +648,23 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     mbar_init(&sh.ak_full, 4);
     mbar_init(&sh.ak_empty, 1);
     mbar_init(&sh.s_full, 1);
-    mbar_init(&sh.s_empty, 8);
+    mbar_init(&sh.s_empty, 4 * S::kSG);
     mbar_init(&sh.o_full, 1);
     mbar_init(&sh.o_empty, kWarpsD);
     mbar_init(&sh.drain, 1);
     for (int i = 0; i < 2; i++) {
-      mbar_init(&sh.av_full[i], kWarpsD);
+      mbar_init(&sh.av_full[i], S::kVG * kWarpsD);
       mbar_init(&sh.av_empty[i], 1);
-      mbar_init(&sh.p_full[i], 8);
+      mbar_init(&sh.p_full[i], 4 * S::kSG);
       mbar_init(&sh.p_empty[i], 1);
-      mbar_init(&sh.u_full[i], 8);
+      mbar_init(&sh.u_full[i], 4 * S::kSG);
       mbar_init(&sh.u_empty[i], kWarpsD);
       sh.fail[i][0] = sh.fail[i][1] = 0;
     }
 #pragma unroll 1
     for (int i = 0; i < kUnits; i++) {
       mbar_init(&sh.unit_full[i], 1);
-      mbar_init(&sh.unit_empty[i], 4 + 8 + 2 * kWarpsD + 1);  // the warps that take units
+      mbar_init(&sh.unit_empty[i], 4 + 4 * S::kSG + (S::kVG + 1) * kWarpsD + 1);  // the warps that take units
     }
     sh.abort = 0;
     fence_barrier_init();
@@ -762,18 +767,20 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         if (lane == 0) ta_arrive(&sh.ak_full);
       }
     }
-  } else if (warp < kWarpS) {
+  } else if (warp < kWarpS || (S::kVG == 2 && warp >= kWarp2 && warp < kWarpO)) {
     // ---- V: a lane is a column of the head; positions along its row ----
     ta_regs_dec<kRegsKV>();
-    const int w = warp - kWarpV;
+    const int w = warp & 3, vg = warp >= kWarp2;
+    constexpr int kMine = S::kSlots / S::kVG;  // slots of a tile
     uint32_t tile = 0;
     TaRing<S::kRingV> ring;
+    ring.at = vg * kMine;
     TaRing<S::kNV> buf;
     while (w < kWarpsD && feed.next(sh, lane, ok)) {
       // the words of the unit before last have been read
       const int par = feed.index & 1;
       if (feed.index >= 2) ok = ta_wait(sh, &sh.u_empty[par], ((feed.index >> 1) - 1) & 1);
-      unsigned* vbad = sh.vbad[par][w];
+      unsigned* vbad = sh.vbad[par][vg * 4 + w];
       if (lane < 2) vbad[lane] = 0;
       __syncwarp();
 #pragma unroll 1
@@ -783,10 +790,10 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         buf.step();
         ta_fence_after();
 #pragma unroll 1
-        for (int k = 0; k < S::kSlots && ok; k++) {
+        for (int k = vg * kMine; k < (vg + 1) * kMine && ok; k++) {
           const uint32_t slot = ring.at;
           ok = ta_wait(sh, &sh.v_full[slot], ring.parity);
-          ring.step();
+          ring.step(k + 1 == (vg + 1) * kMine ? S::kSlots - kMine + 1 : 1);
           if (!ok) break;
           uint8_t* raw = smem + S::kOffV + slot * S::kSlotV;
           const int p0 = t * kTilePos + k * S::kSlotPos;
@@ -806,7 +813,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
   } else if (warp < kWarpO) {
     // ---- the softmax: a lane is a position, a group of four warps half of the rows ----
     const int grp = (warp - kWarpS) >> 2, w = warp & 3, gt = w * 32 + lane, bar = 1 + grp;
-    constexpr int R = NR / 2;
+    constexpr int R = S::kR;
     float2 l[R / 2];
     uint32_t tile = 0;
     TaRing<S::kNP> buf;
@@ -815,7 +822,8 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     for (;;) {
       const bool more = feed.next(sh, lane, ok);
       const int u = feed.index & 1;
-      const int steps = (it.rows + 15) >> 4, base = grp * steps * 8;  // steps of 8 rows from `base`
+      // steps of 8 rows from `base`
+      const int steps = NR == 16 ? 2 : ((it.rows + 15) >> 4) * (2 / S::kSG), base = grp * steps * 8;
       const float* c = sh.c[feed.index % kUnits] + base;
       float* nm = sh.nm + base;
       const int my = base + gt;  // the row that this thread keeps, one of the first `mine`
@@ -1005,7 +1013,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         ok = ta_wait(sh, &sh.o_full, tile & 1);
         if (!ok) break;
         ta_fence_after();
-        const bool moved = (sh.moved[tile & 3][0] | sh.moved[tile & 3][1]) != 0;
+        const bool moved = (sh.moved[tile & 3][0] | (S::kSG == 2 ? sh.moved[tile & 3][1] : 0)) != 0;
         const float* f = sh.f[tile & 3];
 #pragma unroll
         for (int c = 0; c < NR / 16; c++) {
@@ -1032,7 +1040,10 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       if (!ok) break;
       unsigned long long vbad = 0;
 #pragma unroll
-      for (int i = 0; i < kWarpsD; i++) vbad |= sh.vbad[u][i][0] | (unsigned long long)sh.vbad[u][i][1] << 32;
+      for (int i = 0; i < kWarpsD; i++)
+#pragma unroll
+        for (int g = 0; g < S::kVG; g++)
+          vbad |= sh.vbad[u][g * 4 + i][0] | (unsigned long long)sh.vbad[u][g * 4 + i][1] << 32;
       if (vbad) {
 #pragma unroll
         for (int r = 0; r < NR; r++)
@@ -1165,10 +1176,10 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     auto qk_tile = [&](int steps) {  // scores of tile `qk`
       bool good = ta_wait(sh, &sh.ak_full, qk & 1);
       if (good && qk > 0) good = ta_wait(sh, &sh.s_empty, (qk - 1) & 1);
-      if (!good) return false;
+      if (!__all_sync(0xffffffffu, good)) return false;
       ta_fence_after();
       const uint32_t d = tmem + S::kTmS, idesc = ta_idesc(kF16, false, steps * 16);
-#pragma unroll 1
+#pragma unroll
       for (int i = 0; i < S::kProducts; i++) {
         const uint32_t ta = (uint32_t)(kTerms >> (8 * i)) & 15, tb = (uint32_t)(kTerms >> (8 * i + 4)) & 15;
         const uint32_t at = tmem + S::kTmK + ta * (HD / 2);
@@ -1182,21 +1193,23 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       return true;
     };
     while (feed.next(sh, lane, ok)) {
-      const int steps = (it.rows + 15) >> 4;
+      const int steps = NR == 16 ? 1 : (__shfl_sync(0xffffffffu, it.rows, 0) + 15) >> 4;
+      const int tiles = __shfl_sync(0xffffffffu, it.t1 - it.t0, 0);
       ok = qk_tile(steps);
 #pragma unroll 1
-      for (int t = it.t0; t < it.t1 && ok; t++, tile++) {
-        if (t + 1 < it.t1) ok = qk_tile(steps);
+      for (int t = 0; t < tiles && ok; t++, tile++) {
+        if (t + 1 < tiles) ok = qk_tile(steps);
         const uint32_t vb = vbuf.at, pb = pbuf.at;
         ok = ok && ta_wait(sh, &sh.av_full[vb], vbuf.parity) && ta_wait(sh, &sh.p_full[pb], pbuf.parity);
         vbuf.step();
         pbuf.step();
         if (ok && tile > 0) ok = ta_wait(sh, &sh.o_empty, (tile - 1) & 1);
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         ta_fence_after();
         const uint32_t d = tmem + S::kTmO, idesc = ta_idesc(kF16, true, steps * 16), av = tmem + S::kTmV + vb * S::kVCols;
         const uint64_t pd = pdesc + (uint64_t)(pb * (S::kPBuf >> 4));
-#pragma unroll 1
+#pragma unroll
         for (int i = 0; i < S::kProducts; i++) {
           const uint32_t ta = (uint32_t)(kTerms >> (8 * i)) & 15, tb = (uint32_t)(kTerms >> (8 * i + 4)) & 15;
           const uint32_t at = av + ta * (kTilePos / 2);
