@@ -54,10 +54,10 @@ constexpr int kMaxRows = 64;    // rows (node, head) of a CTA's unit
 // the MMAs 21
 constexpr int kWarpV = 4, kWarpS = 8, kWarp2 = 12, kWarpO = 16, kWarpCopy = 20, kWarpMma = 21;
 constexpr int kTaThreads = 32 * 22;
-// Registers a thread: 80 at launch; the groups that decode K and V give 8 each to
-// the one that holds O (an increase beyond what was given would wait for good).
-constexpr int kRegs = 80, kRegsKV = 72, kRegsO = 96;
-static_assert(2 * kRegsKV + kRegsO <= 3 * kRegs, "registers");
+// Registers a thread: 80 at launch; the groups that decode K and V give 24 each,
+// the softmax and O take 16 each (increases beyond what was given would wait for good).
+constexpr int kRegs = 80, kRegsKV = 56, kRegsS = 96, kRegsO = 96;
+static_assert(2 * kRegsKV + 2 * kRegsS + kRegsO <= 5 * kRegs && 3 * kRegsKV + kRegsS + kRegsO <= 5 * kRegs, "registers");
 constexpr float kShift = 7.0f;  // P = 2^(s - m + kShift)
 constexpr float kLimit = 15.0f; // largest exponent of P before the maximum moves
 constexpr float kUnset = -3e38f;
@@ -117,7 +117,7 @@ constexpr int kUnits = 4;  // units announced ahead
 
 struct TaShared {
   float c[kUnits][kMaxRows];             // score factor, per unit
-  float nm[kMaxRows];                    // kShift - maximum
+  float nm[kMaxRows];                    // kShift - maximum (0 before the row has one)
   float f[4][kMaxRows];                  // rescaling of the earlier tiles, per tile
   float red[2][4][32];                  // a softmax group's warps meet here
   float fin[2][kMaxRows];                // per unit parity: the factor of a row's output
@@ -234,8 +234,18 @@ __device__ __forceinline__ void ta_wait_ld(float (&v)[N]) {
 #pragma unroll
   for (int i = 0; i < N; i++) asm volatile("" : "+f"(v[i]));
 }
+__device__ __forceinline__ void ta_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 __device__ __forceinline__ void ta_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ta_max(float x) {  // over the warp's lanes
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
 }
 __device__ __forceinline__ float ta_exp2(float x) {
   float y;
@@ -429,10 +439,10 @@ template <int HD, int DT, int NR>
 __device__ __forceinline__ void decode_v(const uint8_t* raw, uint32_t col, int w, int lane) {
   using S = TaShape<HD, DT, NR>;
   const int h = w * 32 + lane;
+  if constexpr (DT == LRS_KV_Q8_0) {
 #pragma unroll 1
-  for (int g = 0; g < S::kSlotPos / 32; g++) {  // 32 positions: 16 columns a term
-    uint32_t x[S::kA][16];
-    if constexpr (DT == LRS_KV_Q8_0) {
+    for (int g = 0; g < S::kSlotPos / 32; g++) {  // 32 positions: 16 columns a term
+      uint32_t x[2][16];
       uint4 d8;
 #pragma unroll
       for (int i = 0; i < 8; i++) {
@@ -444,10 +454,16 @@ __device__ __forceinline__ void decode_v(const uint8_t* raw, uint32_t col, int w
         x[0][i * 2] = hi[0], x[0][i * 2 + 1] = hi[1];
         x[1][i * 2] = lo[0], x[1][i * 2 + 1] = lo[1];
       }
-    } else {
 #pragma unroll
-      for (int i = 0; i < 16; i++) {
-        const int r = g * 32 + i * 2;
+      for (int q = 0; q < 2; q++) ta_st16(col + q * (kTilePos / 2) + g * 16, x[q]);
+    }
+  } else {
+#pragma unroll 1
+    for (int g = 0; g < S::kSlotPos / 16; g++) {  // 16 positions: 8 columns a term
+      uint32_t x[S::kA][8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const int r = g * 16 + i * 2;
         if constexpr (DT == LRS_KV_BF16) {
           const uint16_t* b = reinterpret_cast<const uint16_t*>(raw) + r * HD + h;
           x[0][i] = (uint32_t)b[0] | (uint32_t)b[HD] << 16;
@@ -459,9 +475,9 @@ __device__ __forceinline__ void decode_v(const uint8_t* raw, uint32_t col, int w
           for (int q = 0; q < S::kA; q++) x[q][i] = y[q];
         }
       }
-    }
 #pragma unroll
-    for (int q = 0; q < S::kA; q++) ta_st16(col + q * (kTilePos / 2) + g * 16, x[q]);
+      for (int q = 0; q < S::kA; q++) ta_st8(col + q * (kTilePos / 2) + g * 8, x[q]);
+    }
   }
 }
 
@@ -733,18 +749,18 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         } else {
           const uint8_t* row = raw + r * S::kRowK;
 #pragma unroll 1
-          for (int b = 0; b < HD / 32; b++) {  // 32 values: 16 columns a term
-            uint32_t x[kA][16];
+          for (int b = 0; b < HD / 16; b++) {  // 16 values: 8 columns a term
+            uint32_t x[kA][8];
             if constexpr (DT == LRS_KV_BF16) {
 #pragma unroll
-              for (int i = 0; i < 4; i++) {
-                const uint4 w = *reinterpret_cast<const uint4*>(row + b * 64 + i * 16);
+              for (int i = 0; i < 2; i++) {
+                const uint4 w = *reinterpret_cast<const uint4*>(row + b * 32 + i * 16);
                 x[0][i * 4] = w.x, x[0][i * 4 + 1] = w.y, x[0][i * 4 + 2] = w.z, x[0][i * 4 + 3] = w.w;
               }
             } else {
 #pragma unroll
-              for (int i = 0; i < 8; i++) {
-                const float4 f = *reinterpret_cast<const float4*>(row + b * 128 + i * 16);
+              for (int i = 0; i < 4; i++) {
+                const float4 f = *reinterpret_cast<const float4*>(row + b * 64 + i * 16);
                 uint32_t y[kA];
                 ta_split<false, kA>(make_float2(f.x, f.y), y);
 #pragma unroll
@@ -756,7 +772,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
             }
 #pragma unroll
             for (int k = 0; k < kA; k++)
-              ta_st16(tmem + lanes + S::kTmK + k * HD / 2 + b * 16, x[k]);
+              ta_st8(tmem + lanes + S::kTmK + k * HD / 2 + b * 8, x[k]);
           }
         }
         __syncwarp();
@@ -812,6 +828,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     }
   } else if (warp < kWarpO) {
     // ---- the softmax: a lane is a position, a group of four warps half of the rows ----
+    ta_regs_inc<kRegsS>();
     const int grp = (warp - kWarpS) >> 2, w = warp & 3, gt = w * 32 + lane, bar = 1 + grp;
     constexpr int R = S::kR;
     float2 l[R / 2];
@@ -830,24 +847,25 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       const int mine = steps * 8;
       const bool whole = it.t0 == 0 && it.t1 == it.tiles;
       float* seg = segs + (size_t)(2 * blockIdx.x + (it.t0 == 0)) * ta_seg_floats<HD, NR>();
-      unsigned long long my_mask = 0;
+      unsigned long long row_mask = 0;  // of row base + lane
       float* my_out = nullptr;
-      if (more && gt < mine && my < it.rows) {
-        const int row = it.row0 + my, node = row / a.group, g = row % a.group;
+      if (more && base + lane < it.rows) {
+        const int row = it.row0 + base + lane, node = row / a.group, g = row % a.group;
         my_out = whole ? a.out + (size_t)(it.s + node) * a.out_ld + (size_t)(it.kvh * a.group + g) * HD
                        : seg + 2 * NR + my * HD;
-        my_mask = a.mask ? a.mask[it.s + node] : (node == 63 ? ~0ull : (2ull << node) - 1);
-        if (it.n < 64) my_mask &= (1ull << it.n) - 1;
+        row_mask = a.mask ? a.mask[it.s + node] : (node == 63 ? ~0ull : (2ull << node) - 1);
+        if (it.n < 64) row_mask &= (1ull << it.n) - 1;
       }
       if (more && feed.index >= 2) ok = ok && ta_wait(sh, &sh.u_empty[u], ((feed.index >> 1) - 1) & 1);
       if (more && gt < mine) {
         sh.out[u][my] = my_out;
-        nm[gt] = -kUnset;
+        nm[gt] = 0.0f;
       }
       if (ta_group_or(bar, !more || !ok)) break;
 #pragma unroll
       for (int r = 0; r < R / 2; r++) l[r] = make_float2(0.0f, 0.0f);
-      bool masks = false, left = false;
+      bool masks = false, left = false, unset = true;  // unset: a row may have no maximum yet
+      float max_of = kUnset;                           // this thread's row's, + kShift as in nm
 #pragma unroll 1
       for (int t = it.t0; t < it.t1; t++, tile++) {
         const int p = t * kTilePos + w * 32 + lane;
@@ -855,13 +873,11 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         if ((t + 1) * kTilePos > it.ctx) {
           if (!masks) {  // the rows that see each node, from the nodes that each row sees
             masks = true;
-            if (gt < mine) sh.mask[u][my] = my_mask;
-            ta_group_sync(bar);
-            if (gt < it.n) {
-              uint32_t v = 0;
+            if (gt < mine) sh.mask[u][my] = row_mask;
 #pragma unroll 1
-              for (int r = 0; r < mine; r++) v |= (uint32_t)(sh.mask[u][base + r] >> gt & 1) << r;
-              sh.vis[grp][gt] = v;
+            for (int j = w; j < it.n; j += 4) {
+              const uint32_t v = __ballot_sync(0xffffffffu, lane < mine && (row_mask >> j & 1));
+              if (lane == 0) sh.vis[grp][j] = v;
             }
             ta_group_sync(bar);
           }
@@ -873,72 +889,63 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         const uint32_t st = tmem + lanes + S::kTmS + base;
         float s[R];
         float* f = sh.f[tile & 3] + base;
-        bool move = false;
-#pragma unroll 1
-        for (;;) {
 #pragma unroll
-          for (int r = 0; r < R; r++) s[r] = -INFINITY;
+        for (int r = 0; r < R; r++) s[r] = -INFINITY;
 #pragma unroll
-          for (int k = 0; k < R / 8; k++)
-            if (k < steps) ta_ld8(st + k * 8, s + k * 8);
-          ta_wait_ld(s);
-          ta_exponents<R>(s, steps, c, nm, vis);
-          if (move) break;
-          // does a score exceed its row's maximum by more than the margin?
-          float top = s[0];
-#pragma unroll
-          for (int r = 1; r < R; r++) top = fmaxf(top, s[r]);
-          move = ta_group_or(bar, top > kLimit);
-          left = *reinterpret_cast<volatile int*>(&sh.fail[tile & 1][grp]) != 0;
-          if (left || !move) break;
-          // the rows' maxima over the tile: 8 rows by 32 lanes to a row for four lanes
-#pragma unroll 1
-          for (int k = 0; k < steps; k++) {
-            float x[8];
-            ta_ld8(st + k * 8, x);
-            ta_wait_ld(x);
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = vis >> (k * 8 + i) & 1 ? x[i] * c[k * 8 + i] : kUnset;
-            int row = k * 8;
-#pragma unroll
-            for (int wd = 16, nn = 4; wd >= 4; wd >>= 1, nn >>= 1) {
-              const bool up = lane & wd;
-#pragma unroll
-              for (int i = 0; i < 4; i++) {
-                if (i < nn) {
-                  const float send = up ? x[i] : x[i + nn], keep = up ? x[i + nn] : x[i];
-                  x[i] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, send, wd));
-                }
-              }
-              if (up) row += nn;
-            }
-            x[0] = fmaxf(x[0], __shfl_xor_sync(0xffffffffu, x[0], 2));
-            x[0] = fmaxf(x[0], __shfl_xor_sync(0xffffffffu, x[0], 1));
-            if (!(lane & 3)) sh.red[grp][w][row] = x[0];
-          }
-          ta_group_sync(bar);
-          if (gt < mine) {
-            const float was = -nm[gt];
-            float mx = fmaxf(fmaxf(sh.red[grp][0][gt], sh.red[grp][1][gt]),
-                             fmaxf(sh.red[grp][2][gt], sh.red[grp][3][gt]));
-            mx = mx > kUnset ? fmaxf(was, mx - kShift) : was;
-            f[gt] = was == kUnset ? 0.0f : ta_exp2(was - mx);
-            nm[gt] = -mx;
-          }
-          ta_group_sync(bar);
-#pragma unroll
-          for (int r = 0; r < R / 2; r++)
-            if (r < steps * 4) l[r].x *= f[2 * r], l[r].y *= f[2 * r + 1];
-        }
-        if (left) break;
-        if (!move && gt < mine) f[gt] = 1.0f;
-        if (gt == 0) sh.moved[tile & 3][grp] = move;
+        for (int k = 0; k < R / 8; k++)
+          if (k < steps) ta_ld8(st + k * 8, s + k * 8);
+        ta_wait_ld(s);
         ta_fence_before();
         __syncwarp();
-        if (lane == 0) ta_arrive(&sh.s_empty);
+        if (lane == 0) ta_arrive(&sh.s_empty);  // the next tile's scores may come
+        ta_exponents<R>(s, steps, c, nm, vis);
+        // does a score exceed its row's maximum by more than the margin?
+        float top = s[0];
+#pragma unroll
+        for (int r = 1; r < R; r++) top = fmaxf(top, s[r]);
+        const bool move = ta_group_or(bar, unset || top > kLimit);
+        left = *reinterpret_cast<volatile int*>(&sh.fail[tile & 1][grp]) != 0;
+        if (left) break;
+        if (move) {
+          // the rows' largest exponents over the tile, to kShift
+          float mx = -INFINITY;
+#pragma unroll
+          for (int r = 0; r < R; r++) {
+            const float v = ta_max(s[r]);
+            if (lane == r) mx = v;
+          }
+          if (lane < R) sh.red[grp][w][lane] = mx;
+          ta_group_sync(bar);
+          bool none = false;
+          if (gt < mine) {
+            mx = fmaxf(fmaxf(sh.red[grp][0][gt], sh.red[grp][1][gt]), fmaxf(sh.red[grp][2][gt], sh.red[grp][3][gt]));
+            // a row without a maximum takes the tile's, the others a larger one
+            float by = max_of == kUnset ? mx - kShift : fmaxf(mx - kShift, 0.0f);
+            if (!(mx > -INFINITY)) by = 0.0f;
+            f[gt] = max_of == kUnset ? 0.0f : ta_exp2(-by);
+            sh.red[grp][0][gt] = -by;
+            if (mx > -INFINITY) max_of = (max_of == kUnset ? 0.0f : max_of) + by;
+            none = max_of == kUnset;
+            nm[gt] = none ? 0.0f : -max_of;
+          }
+          unset = ta_group_or(bar, none);
+#pragma unroll
+          for (int r = 0; r < R; r += 2) {
+            if (r < steps * 8) {
+              const float2 g = *reinterpret_cast<const float2*>(f + r);
+              const float2 d = ta_add2(make_float2(s[r], s[r + 1]), *reinterpret_cast<const float2*>(&sh.red[grp][0][r]));
+              s[r] = d.x, s[r + 1] = d.y;
+              l[r / 2].x *= g.x, l[r / 2].y *= g.y;
+            }
+          }
+        } else if (gt < mine) {
+          f[gt] = 1.0f;
+        }
+        if (gt == 0) sh.moved[tile & 3][grp] = move;
         // P in terms, N-major (a lane writes 8 rows at once), and the row sums
         const uint32_t pb = buf.at;
-        if (tile >= S::kNP) ok = ok && ta_wait(sh, &sh.p_empty[pb], buf.parity ^ 1);
+        // (of two buffers the older product had ended before these scores came)
+        if (S::kNP == 1 && tile >= 1) ok = ok && ta_wait(sh, &sh.p_empty[pb], buf.parity ^ 1);
         buf.step();
         const int pp = w * 32 + lane;
         uint8_t* dst = smem + S::kOffP + pb * S::kPBuf + (pp >> 3) * (NR * 16) + (pp & 7) * 16 + base * 16;
@@ -991,7 +998,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         if (gt < mine) {
           const float sum = (sh.red[grp][0][gt] + sh.red[grp][1][gt]) + (sh.red[grp][2][gt] + sh.red[grp][3][gt]);
           sh.fin[u][my] = !whole ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
-          if (!whole && my < it.rows) seg[2 * my] = -nm[gt], seg[2 * my + 1] = sum;
+          if (!whole && my < it.rows) seg[2 * my] = max_of, seg[2 * my + 1] = sum;
         }
         __syncwarp();
         if (lane == 0) ta_arrive(&sh.u_full[u]);
