@@ -49,27 +49,29 @@ namespace {
 
 constexpr int kTilePos = 128;   // positions of a tile: the lanes of an MMA
 constexpr int kMaxRows = 64;    // rows (node, head) of a CTA's unit
-// warps: K 0-3, V 4-7, the softmax 8-11, V (up to 32 rows: half of the positions
-// each) or the softmax (64: half of the rows each) 12-15, O 16-19, the copies 20,
-// the MMAs 21
-constexpr int kWarpV = 4, kWarpS = 8, kWarp2 = 12, kWarpO = 16, kWarpCopy = 20, kWarpMma = 21;
-constexpr int kTaThreads = 32 * 22;
-// Registers a thread: 80 at launch; the groups that decode K and V give 24 each,
-// the softmax and O take 16 each (increases beyond what was given would wait for good).
-constexpr int kRegs = 80, kRegsKV = 56, kRegsS = 96, kRegsO = 96;
-static_assert(2 * kRegsKV + 2 * kRegsS + kRegsO <= 5 * kRegs && 3 * kRegsKV + kRegsS + kRegsO <= 5 * kRegs, "registers");
 constexpr float kShift = 7.0f;  // P = 2^(s - m + kShift)
 constexpr float kLimit = 15.0f; // largest exponent of P before the maximum moves
 constexpr float kUnset = -3e38f;
-constexpr int kSmemMost = 226 * 1024, kSharedBytes = 7680;
+constexpr int kSmemMost = 226 * 1024, kSharedBytes = 8192;
 
 template <int HD, int DT, int NR>
 struct TaShape {
   static constexpr int kA = DT == LRS_KV_F32 ? 3 : DT == LRS_KV_BF16 ? 1 : 2;  // terms of K, V
   static constexpr int kB = DT == LRS_KV_Q8_0 ? 2 : 3;                        // terms of q, P
   static constexpr bool kF16 = DT == LRS_KV_Q8_0;
-  static constexpr int kSG = NR == 64 ? 2 : 1, kVG = 3 - kSG;  // softmax groups, V groups
-  static constexpr int kR = NR / kSG;                          // rows of a softmax group
+  // Groups of four warps: K, V (up to 32 rows two, half of the positions each),
+  // the softmax (16 rows each), O; then a warp for the copies and one for the MMAs.
+  static constexpr int kSG = NR / 16, kVG = NR == 64 ? 1 : 2;
+  static constexpr int kWarpV = 4, kWarpS = kWarpV + 4 * kVG, kWarpO = kWarpS + 4 * kSG;
+  static constexpr int kWarpCopy = kWarpO + 4, kWarpMma = kWarpCopy + 1;
+  static constexpr int kThreads = 32 * (kWarpMma + 1);
+  // Registers a thread: at launch, K and V, the softmax, O (increases beyond what
+  // the others gave would wait for good).
+  static constexpr int kRegs = NR == 64 ? 64 : NR == 32 ? 72 : 80;
+  static constexpr int kRegsKV = NR == 64 ? 48 : 56, kRegsS = NR == 64 ? 64 : NR == 32 ? 72 : 80;
+  static constexpr int kRegsO = 96;
+  static_assert((1 + kVG) * kRegsKV + kSG * kRegsS + kRegsO <= (2 + kVG + kSG) * kRegs, "registers");
+  static_assert(kRegsS == kRegs && kRegsKV < kRegs && kRegsO > kRegs, "the roles' changes of registers");
   static constexpr int kProducts = DT == LRS_KV_F32 ? 6 : 3;
   // tensor memory columns: V is double-buffered where it fits
   static constexpr int kVCols = kA * kTilePos / 2;
@@ -119,14 +121,14 @@ struct TaShared {
   float c[kUnits][kMaxRows];             // score factor, per unit
   float nm[kMaxRows];                    // kShift - maximum (0 before the row has one)
   float f[4][kMaxRows];                  // rescaling of the earlier tiles, per tile
-  float red[2][4][32];                  // a softmax group's warps meet here
+  float red[4][4][16];                  // a softmax group's warps meet here
   float fin[2][kMaxRows];                // per unit parity: the factor of a row's output
   unsigned long long mask[2][kMaxRows];  // the row's node mask
-  uint32_t vis[2][LRS_TREE_MAX_NODES];   // rows of a softmax group that see a node
+  uint32_t vis[4][LRS_TREE_MAX_NODES];   // rows of a softmax group that see a node
   float* out[2][kMaxRows];               // the row's output
   unsigned vbad[2][8][2];                // nodes whose V is not finite, per warp that reads V
-  int moved[4][2];
-  int fail[2][2];  // a softmax warp's wait gave up, per tile parity and group
+  int moved[4][4];  // per tile and softmax group
+  int fail[2][4];  // a softmax warp's wait gave up, per tile parity and group
   TaUnit unit[kUnits];
   uint64_t k_full[8], k_empty[8], v_full[8], v_empty[8];
   uint64_t ak_full, ak_empty, s_full, s_empty, o_full, o_empty, drain;
@@ -193,15 +195,6 @@ __device__ __forceinline__ void ta_ld16(uint32_t taddr, float* v) {
 #pragma unroll
   for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
 }
-__device__ __forceinline__ void ta_ld8(uint32_t taddr, float* v) {
-  uint32_t r[8];
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
-                 "=r"(r[6]), "=r"(r[7])
-               : "r"(taddr));
-#pragma unroll
-  for (int i = 0; i < 8; i++) v[i] = __uint_as_float(r[i]);
-}
 // Two f32 operations in one instruction.
 __device__ __forceinline__ float2 ta_fma2(float2 a, float2 b, float2 c) {
   float2 d;
@@ -218,14 +211,6 @@ __device__ __forceinline__ float2 ta_add2(float2 a, float2 b) {
       : "=f"(d.x), "=f"(d.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
-}
-__device__ __forceinline__ void ta_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
-      "%14,%15,%16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
 }
 // The loaded registers may be used after this: it names them, so that no use moves above it.
 template <int N>
@@ -276,26 +261,26 @@ __device__ __forceinline__ void ta_regs_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-// Tests a barrier's phase; an incomplete one suspends the warp for up to 1 ms, so
-// that waiting warps leave the issue slots and the instruction cache to the others.
+// Tests a barrier's phase; an incomplete one suspends the warp for a while.
 __device__ __forceinline__ bool ta_try_wait(uint32_t bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
       " selp.u32 %0, 1, 0, p;\n}"
       : "=r"(done)
-      : "r"(bar), "r"(parity), "r"(1000000u)
+      : "r"(bar), "r"(parity)
       : "memory");
   return done != 0;
 }
-constexpr uint32_t kPolls = 1u << 14;
+constexpr uint32_t kPolls = 1u << 20;
 // A wait that gives up after a bounded number of polls, or when another role did.
 __device__ __forceinline__ bool ta_wait(TaShared& sh, uint64_t* bar, uint32_t parity) {
   const uint32_t at = smem_u32(bar);
+  if (ta_try_wait(at, parity)) return true;
 #pragma unroll 1
   for (uint32_t i = 0; i < kPolls; i++) {
     if (ta_try_wait(at, parity)) return true;
-    if (*reinterpret_cast<volatile int*>(&sh.abort)) return false;
+    if ((i & 255) == 255 && *reinterpret_cast<volatile int*>(&sh.abort)) return false;
   }
   *reinterpret_cast<volatile int*>(&sh.abort) = 1;
   return false;
@@ -441,12 +426,12 @@ __device__ __forceinline__ void decode_v(const uint8_t* raw, uint32_t col, int w
   const int h = w * 32 + lane;
   if constexpr (DT == LRS_KV_Q8_0) {
 #pragma unroll 1
-    for (int g = 0; g < S::kSlotPos / 32; g++) {  // 32 positions: 16 columns a term
-      uint32_t x[2][16];
+    for (int g = 0; g < S::kSlotPos / 16; g++) {  // 16 positions: 8 columns a term
+      uint32_t x[2][8];
       uint4 d8;
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const int r = g * 32 + i * 4;
+      for (int i = 0; i < 4; i++) {
+        const int r = g * 16 + i * 4;
         if (i % 2 == 0) d8 = *reinterpret_cast<const uint4*>(raw + q8_v_scale(HD, r, w));
         const uint32_t cw = *reinterpret_cast<const uint32_t*>(raw + q8_v_code(HD, r, h));
         uint32_t hi[2], lo[2];
@@ -455,7 +440,7 @@ __device__ __forceinline__ void decode_v(const uint8_t* raw, uint32_t col, int w
         x[1][i * 2] = lo[0], x[1][i * 2 + 1] = lo[1];
       }
 #pragma unroll
-      for (int q = 0; q < 2; q++) ta_st16(col + q * (kTilePos / 2) + g * 16, x[q]);
+      for (int q = 0; q < 2; q++) ta_st8(col + q * (kTilePos / 2) + g * 8, x[q]);
     }
   } else {
 #pragma unroll 1
@@ -481,22 +466,27 @@ __device__ __forceinline__ void decode_v(const uint8_t* raw, uint32_t col, int w
   }
 }
 
-// The scores of up to R rows (8 a step) of this lane's position as exponents of
-// P: c * s - maximum + kShift, -inf where the row does not see the position.
-template <int R>
-__device__ __forceinline__ void ta_exponents(float (&s)[R], int steps, const float* c,
-                                             const float* nm, uint32_t vis) {
+// The scores of 16 rows of this lane's position as exponents of P:
+// c * s - maximum + kShift (c is 1 but for f16), -inf where the row does not see it.
+template <bool SCALED>
+__device__ __forceinline__ void ta_exponents(float (&s)[16], const float* c, const float* nm, uint32_t vis) {
 #pragma unroll
-  for (int r = 0; r < R; r += 4) {
-    if (r % 8 == 0 && r / 8 >= steps) break;
-    const float4 cc = *reinterpret_cast<const float4*>(c + r), mm = *reinterpret_cast<const float4*>(nm + r);
-    const float2 x = ta_fma2(make_float2(s[r], s[r + 1]), make_float2(cc.x, cc.y), make_float2(mm.x, mm.y));
-    const float2 y = ta_fma2(make_float2(s[r + 2], s[r + 3]), make_float2(cc.z, cc.w), make_float2(mm.z, mm.w));
+  for (int r = 0; r < 16; r += 4) {
+    const float4 mm = *reinterpret_cast<const float4*>(nm + r);
+    float2 x = make_float2(s[r], s[r + 1]), y = make_float2(s[r + 2], s[r + 3]);
+    if constexpr (SCALED) {
+      const float4 cc = *reinterpret_cast<const float4*>(c + r);
+      x = ta_fma2(x, make_float2(cc.x, cc.y), make_float2(mm.x, mm.y));
+      y = ta_fma2(y, make_float2(cc.z, cc.w), make_float2(mm.z, mm.w));
+    } else {
+      x = ta_add2(x, make_float2(mm.x, mm.y));
+      y = ta_add2(y, make_float2(mm.z, mm.w));
+    }
     s[r] = x.x, s[r + 1] = x.y, s[r + 2] = y.x, s[r + 3] = y.y;
   }
-  if (vis != ~0u) {
+  if (vis != 0xffffu) {
 #pragma unroll
-    for (int r = 0; r < R; r++)
+    for (int r = 0; r < 16; r++)
       if (!(vis >> r & 1)) s[r] = -INFINITY;
   }
 }
@@ -573,7 +563,7 @@ __device__ __forceinline__ void load_q(const TreeArgs& a, const TaUnit& it, uint
 }
 
 template <int HD, int DT, int NR>
-__global__ void __launch_bounds__(kTaThreads, 1)
+__global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
     tree_attention_kernel(const __grid_constant__ TreeArgs a) {
   using S = TaShape<HD, DT, NR>;
   constexpr int kA = S::kA;
@@ -586,8 +576,8 @@ __global__ void __launch_bounds__(kTaThreads, 1)
 
   // ---- the schedule: every CTA finds its share of all tiles ----
   {
-    __shared__ int wsum[kTaThreads / 32];
-    const int per = (a.n_trees + kTaThreads - 1) / kTaThreads;
+    __shared__ int wsum[S::kThreads / 32];
+    const int per = (a.n_trees + S::kThreads - 1) / S::kThreads;
     int mine = 0;
     TaTree tr;
 #pragma unroll 1
@@ -606,7 +596,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     __syncthreads();
     int before = incl - mine, total = 0;
 #pragma unroll 1
-    for (int w = 0; w < kTaThreads / 32; w++) {
+    for (int w = 0; w < S::kThreads / 32; w++) {
       if (w < warp) before += wsum[w];
       total += wsum[w];
     }
@@ -675,7 +665,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       mbar_init(&sh.p_empty[i], 1);
       mbar_init(&sh.u_full[i], 4 * S::kSG);
       mbar_init(&sh.u_empty[i], kWarpsD);
-      sh.fail[i][0] = sh.fail[i][1] = 0;
+      sh.fail[i][0] = sh.fail[i][1] = sh.fail[i][2] = sh.fail[i][3] = 0;
     }
 #pragma unroll 1
     for (int i = 0; i < kUnits; i++) {
@@ -688,7 +678,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
   __syncthreads();
   pdl_launch_dependents();
   if (!sh.active) return;
-  if (warp == kWarpMma) {
+  if (warp == S::kWarpMma) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(&sh.tmem)),
                  "r"((uint32_t)S::kTmCols)
@@ -705,9 +695,9 @@ __global__ void __launch_bounds__(kTaThreads, 1)
   const TaUnit& it = feed.u;
   bool ok = true;
 
-  if (warp < kWarpV) {
+  if (warp < S::kWarpV) {
     // ---- K: a lane is a position; its row into tensor memory ----
-    ta_regs_dec<kRegsKV>();
+    ta_regs_dec<S::kRegsKV>();
     uint32_t tile = 0;
     TaRing<S::kRingK> ring;
     ring.at = warp * 32 / S::kSlotPos;
@@ -728,23 +718,20 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         const int r = (warp * 32 + lane) % S::kSlotPos;
         if constexpr (DT == LRS_KV_Q8_0) {
 #pragma unroll 1
-          for (int b = 0; b < HD / 32; b++) {  // a block: 16 columns of hi, 16 of lo
-            uint32_t hi[16], lo[16];
-            const __half2 d2 = __half2half2(*reinterpret_cast<const __half*>(raw + q8_k_scale(HD, r, b)));
+          for (int b = 0; b < HD / 16; b++) {  // 16 values: 8 columns of hi, 8 of lo
+            uint32_t hi[8], lo[8];
+            const __half2 d2 = __half2half2(*reinterpret_cast<const __half*>(raw + q8_k_scale(HD, r, b >> 1)));
+            const uint4 w4 = *reinterpret_cast<const uint4*>(raw + q8_k_code(r, b * 16));
+            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-              const uint4 w4 = *reinterpret_cast<const uint4*>(raw + q8_k_code(r, b * 32 + h * 16));
-              const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-              for (int i = 0; i < 4; i++) {
-                uint32_t x[2], y[2];
-                ta_q8(w[i], d2, d2, x, y);
-                hi[h * 8 + i * 2] = x[0], hi[h * 8 + i * 2 + 1] = x[1];
-                lo[h * 8 + i * 2] = y[0], lo[h * 8 + i * 2 + 1] = y[1];
-              }
+            for (int i = 0; i < 4; i++) {
+              uint32_t x[2], y[2];
+              ta_q8(w[i], d2, d2, x, y);
+              hi[i * 2] = x[0], hi[i * 2 + 1] = x[1];
+              lo[i * 2] = y[0], lo[i * 2 + 1] = y[1];
             }
-            ta_st16(tmem + lanes + S::kTmK + b * 16, hi);
-            ta_st16(tmem + lanes + S::kTmK + HD / 2 + b * 16, lo);
+            ta_st8(tmem + lanes + S::kTmK + b * 8, hi);
+            ta_st8(tmem + lanes + S::kTmK + HD / 2 + b * 8, lo);
           }
         } else {
           const uint8_t* row = raw + r * S::kRowK;
@@ -783,10 +770,10 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         if (lane == 0) ta_arrive(&sh.ak_full);
       }
     }
-  } else if (warp < kWarpS || (S::kVG == 2 && warp >= kWarp2 && warp < kWarpO)) {
+  } else if (warp < S::kWarpS) {
     // ---- V: a lane is a column of the head; positions along its row ----
-    ta_regs_dec<kRegsKV>();
-    const int w = warp & 3, vg = warp >= kWarp2;
+    ta_regs_dec<S::kRegsKV>();
+    const int w = warp & 3, vg = (warp - S::kWarpV) >> 2;
     constexpr int kMine = S::kSlots / S::kVG;  // slots of a tile
     uint32_t tile = 0;
     TaRing<S::kRingV> ring;
@@ -826,12 +813,12 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         if (lane == 0) ta_arrive(&sh.av_full[vb]);
       }
     }
-  } else if (warp < kWarpO) {
-    // ---- the softmax: a lane is a position, a group of four warps half of the rows ----
-    ta_regs_inc<kRegsS>();
-    const int grp = (warp - kWarpS) >> 2, w = warp & 3, gt = w * 32 + lane, bar = 1 + grp;
-    constexpr int R = S::kR;
-    float2 l[R / 2];
+  } else if (warp < S::kWarpO) {
+    // ---- the softmax: a lane is a position, a group of four warps 16 of the rows ----
+    const int grp = (warp - S::kWarpS) >> 2, w = warp & 3, gt = w * 32 + lane, bar = 1 + grp;
+    const int base = grp * 16, my = base + gt;  // threads 0..15 keep a row each
+    float* nm = sh.nm + base;
+    float2 l[8];
     uint32_t tile = 0;
     TaRing<S::kNP> buf;
     // the four warps meet at barriers: one whose wait gave up goes on (on stale
@@ -839,44 +826,39 @@ __global__ void __launch_bounds__(kTaThreads, 1)
     for (;;) {
       const bool more = feed.next(sh, lane, ok);
       const int u = feed.index & 1;
-      // steps of 8 rows from `base`
-      const int steps = NR == 16 ? 2 : ((it.rows + 15) >> 4) * (2 / S::kSG), base = grp * steps * 8;
       const float* c = sh.c[feed.index % kUnits] + base;
-      float* nm = sh.nm + base;
-      const int my = base + gt;  // the row that this thread keeps, one of the first `mine`
-      const int mine = steps * 8;
-      const bool whole = it.t0 == 0 && it.t1 == it.tiles;
+      const bool whole = it.t0 == 0 && it.t1 == it.tiles, idle = base >= it.rows;  // idle: no rows here
       float* seg = segs + (size_t)(2 * blockIdx.x + (it.t0 == 0)) * ta_seg_floats<HD, NR>();
       unsigned long long row_mask = 0;  // of row base + lane
       float* my_out = nullptr;
-      if (more && base + lane < it.rows) {
+      if (more && lane < 16 && base + lane < it.rows) {
         const int row = it.row0 + base + lane, node = row / a.group, g = row % a.group;
         my_out = whole ? a.out + (size_t)(it.s + node) * a.out_ld + (size_t)(it.kvh * a.group + g) * HD
-                       : seg + 2 * NR + my * HD;
+                       : seg + 2 * NR + (base + lane) * HD;
         row_mask = a.mask ? a.mask[it.s + node] : (node == 63 ? ~0ull : (2ull << node) - 1);
         if (it.n < 64) row_mask &= (1ull << it.n) - 1;
       }
       if (more && feed.index >= 2) ok = ok && ta_wait(sh, &sh.u_empty[u], ((feed.index >> 1) - 1) & 1);
-      if (more && gt < mine) {
+      if (more && gt < 16) {
         sh.out[u][my] = my_out;
         nm[gt] = 0.0f;
       }
       if (ta_group_or(bar, !more || !ok)) break;
 #pragma unroll
-      for (int r = 0; r < R / 2; r++) l[r] = make_float2(0.0f, 0.0f);
+      for (int r = 0; r < 8; r++) l[r] = make_float2(0.0f, 0.0f);
       bool masks = false, left = false, unset = true;  // unset: a row may have no maximum yet
-      float max_of = kUnset;                           // this thread's row's, + kShift as in nm
+      float max_of = kUnset;                           // this thread's row's, - kShift
 #pragma unroll 1
       for (int t = it.t0; t < it.t1; t++, tile++) {
         const int p = t * kTilePos + w * 32 + lane;
-        uint32_t vis = ~0u;  // rows that see this lane's position
+        uint32_t vis = 0xffffu;  // rows that see this lane's position
         if ((t + 1) * kTilePos > it.ctx) {
           if (!masks) {  // the rows that see each node, from the nodes that each row sees
             masks = true;
-            if (gt < mine) sh.mask[u][my] = row_mask;
+            if (gt < 16) sh.mask[u][my] = row_mask;
 #pragma unroll 1
             for (int j = w; j < it.n; j += 4) {
-              const uint32_t v = __ballot_sync(0xffffffffu, lane < mine && (row_mask >> j & 1));
+              const uint32_t v = __ballot_sync(0xffffffffu, row_mask >> j & 1);
               if (lane == 0) sh.vis[grp][j] = v;
             }
             ta_group_sync(bar);
@@ -886,38 +868,33 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         ok = ok && ta_wait(sh, &sh.s_full, tile & 1);
         if (!ok) sh.fail[tile & 1][grp] = 1;
         ta_fence_after();
-        const uint32_t st = tmem + lanes + S::kTmS + base;
-        float s[R];
+        float s[16];
         float* f = sh.f[tile & 3] + base;
-#pragma unroll
-        for (int r = 0; r < R; r++) s[r] = -INFINITY;
-#pragma unroll
-        for (int k = 0; k < R / 8; k++)
-          if (k < steps) ta_ld8(st + k * 8, s + k * 8);
+        ta_ld16(tmem + lanes + S::kTmS + base, s);
         ta_wait_ld(s);
         ta_fence_before();
         __syncwarp();
         if (lane == 0) ta_arrive(&sh.s_empty);  // the next tile's scores may come
-        ta_exponents<R>(s, steps, c, nm, vis);
+        ta_exponents<kF16>(s, c, nm, vis);
         // does a score exceed its row's maximum by more than the margin?
         float top = s[0];
 #pragma unroll
-        for (int r = 1; r < R; r++) top = fmaxf(top, s[r]);
-        const bool move = ta_group_or(bar, unset || top > kLimit);
+        for (int r = 1; r < 16; r++) top = fmaxf(top, s[r]);
+        const bool move = ta_group_or(bar, !idle && (unset || top > kLimit));
         left = *reinterpret_cast<volatile int*>(&sh.fail[tile & 1][grp]) != 0;
         if (left) break;
         if (move) {
           // the rows' largest exponents over the tile, to kShift
           float mx = -INFINITY;
 #pragma unroll
-          for (int r = 0; r < R; r++) {
+          for (int r = 0; r < 16; r++) {
             const float v = ta_max(s[r]);
             if (lane == r) mx = v;
           }
-          if (lane < R) sh.red[grp][w][lane] = mx;
+          if (lane < 16) sh.red[grp][w][lane] = mx;
           ta_group_sync(bar);
           bool none = false;
-          if (gt < mine) {
+          if (gt < 16) {
             mx = fmaxf(fmaxf(sh.red[grp][0][gt], sh.red[grp][1][gt]), fmaxf(sh.red[grp][2][gt], sh.red[grp][3][gt]));
             // a row without a maximum takes the tile's, the others a larger one
             float by = max_of == kUnset ? mx - kShift : fmaxf(mx - kShift, 0.0f);
@@ -930,15 +907,13 @@ __global__ void __launch_bounds__(kTaThreads, 1)
           }
           unset = ta_group_or(bar, none);
 #pragma unroll
-          for (int r = 0; r < R; r += 2) {
-            if (r < steps * 8) {
-              const float2 g = *reinterpret_cast<const float2*>(f + r);
-              const float2 d = ta_add2(make_float2(s[r], s[r + 1]), *reinterpret_cast<const float2*>(&sh.red[grp][0][r]));
-              s[r] = d.x, s[r + 1] = d.y;
-              l[r / 2].x *= g.x, l[r / 2].y *= g.y;
-            }
+          for (int r = 0; r < 16; r += 2) {
+            const float2 g = *reinterpret_cast<const float2*>(f + r);
+            const float2 d = ta_add2(make_float2(s[r], s[r + 1]), *reinterpret_cast<const float2*>(&sh.red[grp][0][r]));
+            s[r] = d.x, s[r + 1] = d.y;
+            l[r / 2].x *= g.x, l[r / 2].y *= g.y;
           }
-        } else if (gt < mine) {
+        } else if (gt < 16) {
           f[gt] = 1.0f;
         }
         if (gt == 0) sh.moved[tile & 3][grp] = move;
@@ -949,66 +924,62 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         buf.step();
         const int pp = w * 32 + lane;
         uint8_t* dst = smem + S::kOffP + pb * S::kPBuf + (pp >> 3) * (NR * 16) + (pp & 7) * 16 + base * 16;
+        if (!idle) {
 #pragma unroll
-        for (int k = 0; k < R / 8; k++) {
-          if (k >= steps) break;
-          uint32_t y[S::kB][4];
+          for (int k = 0; k < 2; k++) {
+            uint32_t y[S::kB][4];
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const int r = k * 8 + e * 2;
-            const float2 x = make_float2(ta_exp2(s[r]), ta_exp2(s[r + 1]));
-            l[r / 2] = ta_add2(l[r / 2], x);
-            uint32_t z[S::kB];
-            ta_split<kF16, S::kB>(x, z);
+            for (int e = 0; e < 4; e++) {
+              const int r = k * 8 + e * 2;
+              const float2 x = make_float2(ta_exp2(s[r]), ta_exp2(s[r + 1]));
+              l[r / 2] = ta_add2(l[r / 2], x);
+              uint32_t z[S::kB];
+              ta_split<kF16, S::kB>(x, z);
 #pragma unroll
-            for (int q = 0; q < S::kB; q++) y[q][e] = z[q];
+              for (int q = 0; q < S::kB; q++) y[q][e] = z[q];
+            }
+#pragma unroll
+            for (int q = 0; q < S::kB; q++)
+              *reinterpret_cast<uint4*>(dst + q * S::kPTerm + k * 128) =
+                  make_uint4(y[q][0], y[q][1], y[q][2], y[q][3]);
           }
-#pragma unroll
-          for (int q = 0; q < S::kB; q++)
-            *reinterpret_cast<uint4*>(dst + q * S::kPTerm + k * 128) =
-                make_uint4(y[q][0], y[q][1], y[q][2], y[q][3]);
+          fence_proxy_async();
         }
-        fence_proxy_async();
         __syncwarp();
         if (lane == 0) ta_arrive(&sh.p_full[pb]);
       }
       if (left) break;
-      // the rows' sums over the lanes: R rows by 32 lanes to a row a lane (or a few)
-      {
-        float* lf = reinterpret_cast<float*>(l);
-        int row = 0;
+      // the rows' sums over the lanes: 16 rows by 32 lanes to a row a lane pair
+      float* lf = reinterpret_cast<float*>(l);
+      int row = 0;
 #pragma unroll
-        for (int wd = 16, nn = R / 2; wd >= 1; wd >>= 1, nn >>= 1) {
-          if (nn >= 1) {
-            const bool up = lane & wd;
+      for (int wd = 16, nn = 8; wd >= 2; wd >>= 1, nn >>= 1) {
+        const bool up = lane & wd;
 #pragma unroll
-            for (int i = 0; i < R / 2; i++) {
-              if (i < nn) {
-                const float send = up ? lf[i] : lf[i + nn], keep = up ? lf[i + nn] : lf[i];
-                lf[i] = keep + __shfl_xor_sync(0xffffffffu, send, wd);
-              }
-            }
-            if (up) row += nn;
-          } else {
-            lf[0] += __shfl_xor_sync(0xffffffffu, lf[0], wd);
+        for (int i = 0; i < 8; i++) {
+          if (i < nn) {
+            const float send = up ? lf[i] : lf[i + nn], keep = up ? lf[i + nn] : lf[i];
+            lf[i] = keep + __shfl_xor_sync(0xffffffffu, send, wd);
           }
         }
-        if (!(lane & (32 / R - 1))) sh.red[grp][w][row] = lf[0];
-        ta_group_sync(bar);
-        if (gt < mine) {
-          const float sum = (sh.red[grp][0][gt] + sh.red[grp][1][gt]) + (sh.red[grp][2][gt] + sh.red[grp][3][gt]);
-          sh.fin[u][my] = !whole ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
-          if (!whole && my < it.rows) seg[2 * my] = max_of, seg[2 * my + 1] = sum;
-        }
-        __syncwarp();
-        if (lane == 0) ta_arrive(&sh.u_full[u]);
-        ta_group_sync(bar);  // red is free again
+        if (up) row += nn;
       }
+      lf[0] += __shfl_xor_sync(0xffffffffu, lf[0], 1);
+      if (!(lane & 1)) sh.red[grp][w][row] = lf[0];
+      ta_group_sync(bar);
+      if (gt < 16) {
+        const float sum = (sh.red[grp][0][gt] + sh.red[grp][1][gt]) + (sh.red[grp][2][gt] + sh.red[grp][3][gt]);
+        sh.fin[u][my] = !whole ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+        if (!whole && my < it.rows) seg[2 * my] = max_of, seg[2 * my + 1] = sum;
+      }
+      __syncwarp();
+      if (lane == 0) ta_arrive(&sh.u_full[u]);
+      ta_group_sync(bar);  // red is free again
     }
-  } else if (warp < kWarpCopy) {
+  } else if (warp < S::kWarpCopy) {
     // ---- O: a lane is a column; sums of the tiles' products in registers ----
-    ta_regs_inc<kRegsO>();
-    const int w = warp - kWarpO, h = w * 32 + lane;
+    ta_regs_inc<S::kRegsO>();
+    const int w = warp - S::kWarpO, h = w * 32 + lane;
     uint32_t tile = 0;
     while (w < kWarpsD && feed.next(sh, lane, ok)) {
       const int u = feed.index & 1, steps = (it.rows + 15) >> 4;
@@ -1020,7 +991,9 @@ __global__ void __launch_bounds__(kTaThreads, 1)
         ok = ta_wait(sh, &sh.o_full, tile & 1);
         if (!ok) break;
         ta_fence_after();
-        const bool moved = (sh.moved[tile & 3][0] | (S::kSG == 2 ? sh.moved[tile & 3][1] : 0)) != 0;
+        int moved = 0;
+#pragma unroll
+        for (int g = 0; g < S::kSG; g++) moved |= sh.moved[tile & 3][g];
         const float* f = sh.f[tile & 3];
 #pragma unroll
         for (int c = 0; c < NR / 16; c++) {
@@ -1064,7 +1037,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
       __syncwarp();
       if (lane == 0) ta_arrive(&sh.u_empty[u]);
     }
-  } else if (warp == kWarpCopy) {
+  } else if (warp == S::kWarpCopy) {
     // ---- copies: raw K and V tiles of the pages ----
     const uint64_t pol = evict_first_policy();
     uint32_t nk = 0, nv = 0;  // K and V slots issued
@@ -1239,7 +1212,7 @@ __global__ void __launch_bounds__(kTaThreads, 1)
   if (!ok) atomicExch(a.c.err, LRS_ERR_DEVICE_TIMEOUT);
   ta_fence_before();
   __syncthreads();
-  if (warp == kWarpMma) {
+  if (warp == S::kWarpMma) {
     ta_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
                  "r"((uint32_t)S::kTmCols)
@@ -1294,7 +1267,7 @@ cudaError_t launch(const TreeArgs& a, int sms, cudaStream_t st) {
   cudaError_t e = set_smem_once(attr, (const void*)tree_attention_kernel<HD, DT, NR>, S::kSmem);
   if (e != cudaSuccess) return e;
   const int ctas = grid_ctas(a, sms);
-  tree_attention_kernel<HD, DT, NR><<<ctas, kTaThreads, S::kSmem, st>>>(a);
+  tree_attention_kernel<HD, DT, NR><<<ctas, S::kThreads, S::kSmem, st>>>(a);
   e = cudaGetLastError();
   // units of one tile are never shared
   if (e != cudaSuccess || ctas < 2 || a.max_len <= kTilePos) return e;
