@@ -68,10 +68,10 @@ struct TaShape {
   // Registers a thread: at launch, K and V, the softmax, O (increases beyond what
   // the others gave would wait for good).
   static constexpr int kRegs = NR == 64 ? 64 : NR == 32 ? 72 : 80;
-  static constexpr int kRegsKV = NR == 64 ? 48 : 56, kRegsS = NR == 64 ? 64 : NR == 32 ? 72 : 80;
+  static constexpr int kRegsKV = 64, kRegsS = NR == 64 ? 56 : NR == 32 ? 64 : 80;
   static constexpr int kRegsO = 96;
   static_assert((1 + kVG) * kRegsKV + kSG * kRegsS + kRegsO <= (2 + kVG + kSG) * kRegs, "registers");
-  static_assert(kRegsS == kRegs && kRegsKV < kRegs && kRegsO > kRegs, "the roles' changes of registers");
+  static_assert(kRegsS <= kRegs && kRegsKV <= kRegs && kRegsO > kRegs, "the roles' changes of registers");
   static constexpr int kProducts = DT == LRS_KV_F32 ? 6 : 3;
   // tensor memory columns: V is double-buffered where it fits
   static constexpr int kVCols = kA * kTilePos / 2;
@@ -131,7 +131,8 @@ struct TaShared {
   int fail[2][4];  // a softmax warp's wait gave up, per tile parity and group
   TaUnit unit[kUnits];
   uint64_t k_full[8], k_empty[8], v_full[8], v_empty[8];
-  uint64_t ak_full, ak_empty, s_full, s_empty, o_full, o_empty, drain;
+  uint64_t ak_full[2], ak_empty[2];  // K's halves of the columns
+  uint64_t s_full, s_empty, o_full, o_empty, drain;
   uint64_t av_full[2], av_empty[2], p_full[2], p_empty[2], u_full[2], u_empty[2];
   uint64_t unit_full[kUnits], unit_empty[kUnits];
   int abort;
@@ -160,13 +161,30 @@ __device__ __forceinline__ void ta_commit(uint32_t bar, uint32_t elected) {
       "r"(elected)
       : "memory");
 }
-// D[tmem] (+)= A[tmem] . B[shared]
-__device__ __forceinline__ void ta_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
-                                       bool accumulate, uint32_t elected) {
+// Four steps of K of D[tmem] (+)= A[tmem] . B[shared]; B advances by `step` (in 16 bytes).
+__device__ __forceinline__ void ta_mma4(uint32_t d, uint32_t a, uint64_t b, uint32_t step, uint32_t idesc,
+                                        bool accumulate, uint32_t elected) {
   asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
-      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(elected)
+      "{\n .reg .pred p, q, t;\n .reg .b32 a1, a2, a3;\n .reg .b64 s, b1, b2, b3;\n"
+      " setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n setp.eq.b32 t, 0, 0;\n"
+      " cvt.u64.u32 s, %6;\n add.u64 b1, %2, s;\n add.u64 b2, b1, s;\n add.u64 b3, b2, s;\n"
+      " add.u32 a1, %1, 8;\n add.u32 a2, %1, 16;\n add.u32 a3, %1, 24;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, t;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, t;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, t;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(elected), "r"(step)
+      : "memory");
+}
+__device__ __forceinline__ void ta_mma2(uint32_t d, uint32_t a, uint64_t b, uint32_t step, uint32_t idesc,
+                                        bool accumulate, uint32_t elected) {
+  asm volatile(
+      "{\n .reg .pred p, q, t;\n .reg .b32 a1;\n .reg .b64 s, b1;\n"
+      " setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n setp.eq.b32 t, 0, 0;\n"
+      " cvt.u64.u32 s, %6;\n add.u64 b1, %2, s;\n add.u32 a1, %1, 8;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, t;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(elected), "r"(step)
       : "memory");
 }
 __device__ __forceinline__ uint32_t ta_elect() {
@@ -272,15 +290,27 @@ __device__ __forceinline__ bool ta_try_wait(uint32_t bar, uint32_t parity) {
       : "memory");
   return done != 0;
 }
+// A run of tests, as few instructions as waiting warps may take from the others.
+__device__ __forceinline__ bool ta_try_many(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p, q;\n .reg .u32 n;\n mov.u32 n, 2048;\n"
+      "AGAIN:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra DONE;\n"
+      " sub.u32 n, n, 1;\n setp.ne.u32 q, n, 0;\n @q bra AGAIN;\n"
+      "DONE:\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
 constexpr uint32_t kPolls = 1u << 20;
 // A wait that gives up after a bounded number of polls, or when another role did.
 __device__ __forceinline__ bool ta_wait(TaShared& sh, uint64_t* bar, uint32_t parity) {
   const uint32_t at = smem_u32(bar);
-  if (ta_try_wait(at, parity)) return true;
 #pragma unroll 1
-  for (uint32_t i = 0; i < kPolls; i++) {
-    if (ta_try_wait(at, parity)) return true;
-    if ((i & 255) == 255 && *reinterpret_cast<volatile int*>(&sh.abort)) return false;
+  for (uint32_t i = 0; i < kPolls / 2048; i++) {
+    if (ta_try_many(at, parity)) return true;
+    if (*reinterpret_cast<volatile int*>(&sh.abort)) return false;
   }
   *reinterpret_cast<volatile int*>(&sh.abort) = 1;
   return false;
@@ -419,6 +449,62 @@ __device__ __forceinline__ void mend_v(uint8_t* raw, int w, int lane, int p0, in
   __syncwarp();
 }
 
+// Half of the columns of a position's K into tensor memory: lane = position, row r of the slot.
+template <int HD, int DT, int NR>
+__device__ __forceinline__ void decode_k(const uint8_t* raw, uint32_t at, int r, int half) {
+  using S = TaShape<HD, DT, NR>;
+  constexpr int kSteps = HD / 32;  // of 16 values: 8 columns a term
+  at += half * kSteps * 8;
+  if constexpr (DT == LRS_KV_Q8_0) {
+    const uint8_t* code = raw + q8_k_code(r, half * kSteps * 16);
+    const uint8_t* scale = raw + q8_k_scale(HD, r, half * kSteps / 2);
+    uint4 w4 = *reinterpret_cast<const uint4*>(code);
+#pragma unroll 1
+    for (int b = 0; b < kSteps; b++) {
+      uint32_t hi[8], lo[8];
+      const __half2 d2 = __half2half2(*reinterpret_cast<const __half*>(scale + (b >> 1) * 2));
+      const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+      if (b + 1 < kSteps) w4 = *reinterpret_cast<const uint4*>(code + (b + 1) * kPageSize * 16);
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        uint32_t x[2], y[2];
+        ta_q8(w[i], d2, d2, x, y);
+        hi[i * 2] = x[0], hi[i * 2 + 1] = x[1];
+        lo[i * 2] = y[0], lo[i * 2 + 1] = y[1];
+      }
+      ta_st8(at + b * 8, hi);
+      ta_st8(at + HD / 2 + b * 8, lo);
+    }
+  } else {
+    const uint8_t* row = raw + r * S::kRowK + half * kSteps * (DT == LRS_KV_BF16 ? 32 : 64);
+#pragma unroll 1
+    for (int b = 0; b < kSteps; b++) {
+      uint32_t x[S::kA][8];
+      if constexpr (DT == LRS_KV_BF16) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          const uint4 w = *reinterpret_cast<const uint4*>(row + b * 32 + i * 16);
+          x[0][i * 4] = w.x, x[0][i * 4 + 1] = w.y, x[0][i * 4 + 2] = w.z, x[0][i * 4 + 3] = w.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float4 f = *reinterpret_cast<const float4*>(row + b * 64 + i * 16);
+          uint32_t y[S::kA];
+          ta_split<false, S::kA>(make_float2(f.x, f.y), y);
+#pragma unroll
+          for (int k = 0; k < S::kA; k++) x[k][i * 2] = y[k];
+          ta_split<false, S::kA>(make_float2(f.z, f.w), y);
+#pragma unroll
+          for (int k = 0; k < S::kA; k++) x[k][i * 2 + 1] = y[k];
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < S::kA; k++) ta_st8(at + k * HD / 2 + b * 8, x[k]);
+    }
+  }
+}
+
 // A slot's positions of V into tensor memory: lane = column of the head.
 template <int HD, int DT, int NR>
 __device__ __forceinline__ void decode_v(const uint8_t* raw, uint32_t col, int w, int lane) {
@@ -484,7 +570,7 @@ __device__ __forceinline__ void ta_exponents(float (&s)[16], const float* c, con
     }
     s[r] = x.x, s[r + 1] = x.y, s[r + 2] = y.x, s[r + 3] = y.y;
   }
-  if (vis != 0xffffu) {
+  if (__builtin_expect(vis != 0xffffu, 0)) {
 #pragma unroll
     for (int r = 0; r < 16; r++)
       if (!(vis >> r & 1)) s[r] = -INFINITY;
@@ -574,6 +660,48 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   float* segs = static_cast<float*>(a.workspace);
 
+  // barriers and tensor memory, beside the schedule
+  if (tid == 32) {
+#pragma unroll 1
+    for (int i = 0; i < 8; i++) {
+      mbar_init(&sh.k_full[i], 1);
+      mbar_init(&sh.k_empty[i], S::kSlotPos / 32);
+      mbar_init(&sh.v_full[i], 1);
+      mbar_init(&sh.v_empty[i], kWarpsD);
+    }
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&sh.ak_full[i], 4);
+      mbar_init(&sh.ak_empty[i], 1);
+    }
+    mbar_init(&sh.s_full, 1);
+    mbar_init(&sh.s_empty, 4 * S::kSG);
+    mbar_init(&sh.o_full, 1);
+    mbar_init(&sh.o_empty, kWarpsD);
+    mbar_init(&sh.drain, 1);
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&sh.av_full[i], S::kVG * kWarpsD);
+      mbar_init(&sh.av_empty[i], 1);
+      mbar_init(&sh.p_full[i], 4 * S::kSG);
+      mbar_init(&sh.p_empty[i], 1);
+      mbar_init(&sh.u_full[i], 4 * S::kSG);
+      mbar_init(&sh.u_empty[i], kWarpsD);
+      sh.fail[i][0] = sh.fail[i][1] = sh.fail[i][2] = sh.fail[i][3] = 0;
+    }
+#pragma unroll 1
+    for (int i = 0; i < kUnits; i++) {
+      mbar_init(&sh.unit_full[i], 1);
+      mbar_init(&sh.unit_empty[i], 4 + 4 * S::kSG + (S::kVG + 1) * kWarpsD + 1);  // the warps that take units
+    }
+    sh.abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == S::kWarpMma) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&sh.tmem)),
+                 "r"((uint32_t)S::kTmCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
   // ---- the schedule: every CTA finds its share of all tiles ----
   {
     __shared__ int wsum[S::kThreads / 32];
@@ -594,12 +722,14 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
     if (lane == 31) wsum[warp] = incl;
     if (tid == 0) sh.active = 0;
     __syncthreads();
-    int before = incl - mine, total = 0;
+    int sums = lane < S::kThreads / 32 ? wsum[lane] : 0;
 #pragma unroll 1
-    for (int w = 0; w < S::kThreads / 32; w++) {
-      if (w < warp) before += wsum[w];
-      total += wsum[w];
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, sums, o);
+      if (lane >= o) sums += x;
     }
+    const int total = __shfl_sync(0xffffffffu, sums, 31);
+    const int before = __shfl_sync(0xffffffffu, sums, max(warp - 1, 0)) * (warp > 0) + incl - mine;
     const int ctas = min((int)gridDim.x, total), c = blockIdx.x;
     TaDesc d{};
     if (c < ctas) {
@@ -643,67 +773,33 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
     }
     segs = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + gridDim.x * sizeof(TaDesc));
   }
-  if (tid == 0) {
-#pragma unroll 1
-    for (int i = 0; i < 8; i++) {
-      mbar_init(&sh.k_full[i], 1);
-      mbar_init(&sh.k_empty[i], S::kSlotPos / 32);
-      mbar_init(&sh.v_full[i], 1);
-      mbar_init(&sh.v_empty[i], kWarpsD);
-    }
-    mbar_init(&sh.ak_full, 4);
-    mbar_init(&sh.ak_empty, 1);
-    mbar_init(&sh.s_full, 1);
-    mbar_init(&sh.s_empty, 4 * S::kSG);
-    mbar_init(&sh.o_full, 1);
-    mbar_init(&sh.o_empty, kWarpsD);
-    mbar_init(&sh.drain, 1);
-    for (int i = 0; i < 2; i++) {
-      mbar_init(&sh.av_full[i], S::kVG * kWarpsD);
-      mbar_init(&sh.av_empty[i], 1);
-      mbar_init(&sh.p_full[i], 4 * S::kSG);
-      mbar_init(&sh.p_empty[i], 1);
-      mbar_init(&sh.u_full[i], 4 * S::kSG);
-      mbar_init(&sh.u_empty[i], kWarpsD);
-      sh.fail[i][0] = sh.fail[i][1] = sh.fail[i][2] = sh.fail[i][3] = 0;
-    }
-#pragma unroll 1
-    for (int i = 0; i < kUnits; i++) {
-      mbar_init(&sh.unit_full[i], 1);
-      mbar_init(&sh.unit_empty[i], 4 + 4 * S::kSG + (S::kVG + 1) * kWarpsD + 1);  // the warps that take units
-    }
-    sh.abort = 0;
-    fence_barrier_init();
-  }
-  __syncthreads();
-  pdl_launch_dependents();
-  if (!sh.active) return;
-  if (warp == S::kWarpMma) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                     smem_u32(&sh.tmem)),
-                 "r"((uint32_t)S::kTmCols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
   ta_fence_before();
   __syncthreads();
   ta_fence_after();
+  pdl_launch_dependents();
   const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
   const uint32_t sbase = smem_u32(smem);
   const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;  // this warp's lanes of tensor memory
   TaFeed feed;
   const TaUnit& it = feed.u;
   bool ok = true;
+  if (!sh.active) {
+    if (warp == S::kWarpMma)
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                   "r"((uint32_t)S::kTmCols)
+                   : "memory");
+    return;
+  }
 
   if (warp < S::kWarpV) {
     // ---- K: a lane is a position; its row into tensor memory ----
-    ta_regs_dec<S::kRegsKV>();
+    if constexpr (S::kRegsKV < S::kRegs) ta_regs_dec<S::kRegsKV>();
     uint32_t tile = 0;
     TaRing<S::kRingK> ring;
     ring.at = warp * 32 / S::kSlotPos;
     while (feed.next(sh, lane, ok)) {
       // the last unit's scores are done with q and its factors
-      if (tile > 0) ok = ta_wait(sh, &sh.ak_empty, (tile - 1) & 1);
+      if (tile > 0) ok = ta_wait(sh, &sh.ak_empty[1], (tile - 1) & 1);
       if (!ok) break;
       load_q<HD, DT, NR>(a, it, smem, sh.c[feed.index % kUnits], warp, lane);
       fence_proxy_async();
@@ -711,68 +807,26 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
         const uint32_t slot = ring.at;
         ok = ta_wait(sh, &sh.k_full[slot], ring.parity);
         ring.step(S::kSlots);
-        if (ok && tile > 0) ok = ta_wait(sh, &sh.ak_empty, (tile - 1) & 1);
-        if (!ok) break;
-        ta_fence_after();
         const uint8_t* raw = smem + S::kOffRing + slot * S::kSlotK;
         const int r = (warp * 32 + lane) % S::kSlotPos;
-        if constexpr (DT == LRS_KV_Q8_0) {
 #pragma unroll 1
-          for (int b = 0; b < HD / 16; b++) {  // 16 values: 8 columns of hi, 8 of lo
-            uint32_t hi[8], lo[8];
-            const __half2 d2 = __half2half2(*reinterpret_cast<const __half*>(raw + q8_k_scale(HD, r, b >> 1)));
-            const uint4 w4 = *reinterpret_cast<const uint4*>(raw + q8_k_code(r, b * 16));
-            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-              uint32_t x[2], y[2];
-              ta_q8(w[i], d2, d2, x, y);
-              hi[i * 2] = x[0], hi[i * 2 + 1] = x[1];
-              lo[i * 2] = y[0], lo[i * 2 + 1] = y[1];
-            }
-            ta_st8(tmem + lanes + S::kTmK + b * 8, hi);
-            ta_st8(tmem + lanes + S::kTmK + HD / 2 + b * 8, lo);
-          }
-        } else {
-          const uint8_t* row = raw + r * S::kRowK;
-#pragma unroll 1
-          for (int b = 0; b < HD / 16; b++) {  // 16 values: 8 columns a term
-            uint32_t x[kA][8];
-            if constexpr (DT == LRS_KV_BF16) {
-#pragma unroll
-              for (int i = 0; i < 2; i++) {
-                const uint4 w = *reinterpret_cast<const uint4*>(row + b * 32 + i * 16);
-                x[0][i * 4] = w.x, x[0][i * 4 + 1] = w.y, x[0][i * 4 + 2] = w.z, x[0][i * 4 + 3] = w.w;
-              }
-            } else {
-#pragma unroll
-              for (int i = 0; i < 4; i++) {
-                const float4 f = *reinterpret_cast<const float4*>(row + b * 64 + i * 16);
-                uint32_t y[kA];
-                ta_split<false, kA>(make_float2(f.x, f.y), y);
-#pragma unroll
-                for (int k = 0; k < kA; k++) x[k][i * 2] = y[k];
-                ta_split<false, kA>(make_float2(f.z, f.w), y);
-#pragma unroll
-                for (int k = 0; k < kA; k++) x[k][i * 2 + 1] = y[k];
-              }
-            }
-#pragma unroll
-            for (int k = 0; k < kA; k++)
-              ta_st8(tmem + lanes + S::kTmK + k * HD / 2 + b * 8, x[k]);
-          }
+        for (int half = 0; half < 2; half++) {
+          if (ok && tile > 0) ok = ta_wait(sh, &sh.ak_empty[half], (tile - 1) & 1);
+          if (!ok) break;
+          ta_fence_after();
+          decode_k<HD, DT, NR>(raw, tmem + lanes + S::kTmK, r, half);
+          __syncwarp();
+          if (half && lane == 0) ta_arrive(&sh.k_empty[slot]);
+          ta_wait_st();
+          ta_fence_before();
+          __syncwarp();
+          if (lane == 0) ta_arrive(&sh.ak_full[half]);
         }
-        __syncwarp();
-        if (lane == 0) ta_arrive(&sh.k_empty[slot]);
-        ta_wait_st();
-        ta_fence_before();
-        __syncwarp();
-        if (lane == 0) ta_arrive(&sh.ak_full);
       }
     }
   } else if (warp < S::kWarpS) {
     // ---- V: a lane is a column of the head; positions along its row ----
-    ta_regs_dec<S::kRegsKV>();
+    if constexpr (S::kRegsKV < S::kRegs) ta_regs_dec<S::kRegsKV>();
     const int w = warp & 3, vg = (warp - S::kWarpV) >> 2;
     constexpr int kMine = S::kSlots / S::kVG;  // slots of a tile
     uint32_t tile = 0;
@@ -800,7 +854,7 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
           if (!ok) break;
           uint8_t* raw = smem + S::kOffV + slot * S::kSlotV;
           const int p0 = t * kTilePos + k * S::kSlotPos;
-          if (p0 + S::kSlotPos > it.ctx)  // holds nodes, or positions past the end
+          if (__builtin_expect(p0 + S::kSlotPos > it.ctx, 0))  // holds nodes, or positions past the end
             mend_v<HD, DT, S::kSlotPos>(raw, w, lane, p0, it.ctx, it.len, vbad);
           decode_v<HD, DT, NR>(raw, tmem + lanes + S::kTmV + vb * S::kVCols + k * (S::kSlotPos / 2), w, lane);
           __syncwarp();
@@ -815,6 +869,7 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
     }
   } else if (warp < S::kWarpO) {
     // ---- the softmax: a lane is a position, a group of four warps 16 of the rows ----
+    if constexpr (S::kRegsS < S::kRegs) ta_regs_dec<S::kRegsS>();
     const int grp = (warp - S::kWarpS) >> 2, w = warp & 3, gt = w * 32 + lane, bar = 1 + grp;
     const int base = grp * 16, my = base + gt;  // threads 0..15 keep a row each
     float* nm = sh.nm + base;
@@ -852,7 +907,7 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
       for (int t = it.t0; t < it.t1; t++, tile++) {
         const int p = t * kTilePos + w * 32 + lane;
         uint32_t vis = 0xffffu;  // rows that see this lane's position
-        if ((t + 1) * kTilePos > it.ctx) {
+        if (__builtin_expect((t + 1) * kTilePos > it.ctx, 0)) {
           if (!masks) {  // the rows that see each node, from the nodes that each row sees
             masks = true;
             if (gt < 16) sh.mask[u][my] = row_mask;
@@ -866,7 +921,7 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
           if (p >= it.ctx) vis = p < it.len ? sh.vis[grp][p - it.ctx] : 0;
         }
         ok = ok && ta_wait(sh, &sh.s_full, tile & 1);
-        if (!ok) sh.fail[tile & 1][grp] = 1;
+        if (__builtin_expect(!ok, 0)) sh.fail[tile & 1][grp] = 1;
         ta_fence_after();
         float s[16];
         float* f = sh.f[tile & 3] + base;
@@ -882,8 +937,8 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
         for (int r = 1; r < 16; r++) top = fmaxf(top, s[r]);
         const bool move = ta_group_or(bar, !idle && (unset || top > kLimit));
         left = *reinterpret_cast<volatile int*>(&sh.fail[tile & 1][grp]) != 0;
-        if (left) break;
-        if (move) {
+        if (__builtin_expect(left, 0)) break;
+        if (__builtin_expect(move, 0)) {
           // the rows' largest exponents over the tile, to kShift
           float mx = -INFINITY;
 #pragma unroll
@@ -994,17 +1049,20 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
         int moved = 0;
 #pragma unroll
         for (int g = 0; g < S::kSG; g++) moved |= sh.moved[tile & 3][g];
-        const float* f = sh.f[tile & 3];
+        if (__builtin_expect(moved, 0)) {
+          const float* f = sh.f[tile & 3];
+#pragma unroll
+          for (int r = 0; r < NR; r++) {
+            if (r % 16 == 0 && r / 16 >= steps) break;
+            o[r] *= f[r];
+          }
+        }
 #pragma unroll
         for (int c = 0; c < NR / 16; c++) {
           if (c >= steps) break;
           float x[16];
           ta_ld16(tmem + lanes + S::kTmO + c * 16, x);
           ta_wait_ld(x);
-          if (moved) {
-#pragma unroll
-            for (int i = 0; i < 16; i++) o[c * 16 + i] *= f[c * 16 + i];
-          }
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
             const float2 y = ta_add2(make_float2(o[c * 16 + i], o[c * 16 + i + 1]), make_float2(x[i], x[i + 1]));
@@ -1024,7 +1082,7 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
 #pragma unroll
         for (int g = 0; g < S::kVG; g++)
           vbad |= sh.vbad[u][g * 4 + i][0] | (unsigned long long)sh.vbad[u][g * 4 + i][1] << 32;
-      if (vbad) {
+      if (__builtin_expect(vbad != 0, 0)) {
 #pragma unroll
         for (int r = 0; r < NR; r++)
           if (sh.mask[u][r] & vbad) o[r] = __int_as_float(0x7fc00000);
@@ -1154,20 +1212,25 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
     TaRing<S::kNV> vbuf;
     TaRing<S::kNP> pbuf;
     auto qk_tile = [&](int steps) {  // scores of tile `qk`
-      bool good = ta_wait(sh, &sh.ak_full, qk & 1);
-      if (good && qk > 0) good = ta_wait(sh, &sh.s_empty, (qk - 1) & 1);
-      if (!__all_sync(0xffffffffu, good)) return false;
-      ta_fence_after();
       const uint32_t d = tmem + S::kTmS, idesc = ta_idesc(kF16, false, steps * 16);
 #pragma unroll
-      for (int i = 0; i < S::kProducts; i++) {
-        const uint32_t ta = (uint32_t)(kTerms >> (8 * i)) & 15, tb = (uint32_t)(kTerms >> (8 * i + 4)) & 15;
-        const uint32_t at = tmem + S::kTmK + ta * (HD / 2);
-        const uint64_t qd = qdesc + tb * (S::kQTerm >> 4);
+      for (int half = 0; half < 2; half++) {
+        bool good = ta_wait(sh, &sh.ak_full[half], qk & 1);
+        if (half == 0 && good && qk > 0) good = ta_wait(sh, &sh.s_empty, (qk - 1) & 1);
+        if (!__all_sync(0xffffffffu, good)) return false;
+        ta_fence_after();
 #pragma unroll
-        for (int k = 0; k < HD / 16; k++) ta_mma(d, at + k * 8, qd + k * 16, idesc, (i | k) != 0, el);
+        for (int i = 0; i < S::kProducts; i++) {
+          const uint32_t ta = (uint32_t)(kTerms >> (8 * i)) & 15, tb = (uint32_t)(kTerms >> (8 * i + 4)) & 15;
+          const uint32_t at = tmem + S::kTmK + ta * (HD / 2);
+          const uint64_t qd = qdesc + tb * (S::kQTerm >> 4);
+          const uint32_t ah = at + half * (HD / 4);
+          const uint64_t qh = qd + half * (HD / 2);
+          if constexpr (HD == 128) ta_mma4(d, ah, qh, 16, idesc, (half | i) != 0, el);
+          else ta_mma2(d, ah, qh, 16, idesc, (half | i) != 0, el);
+        }
+        ta_commit(bar_at(&sh.ak_empty[half]), el);
       }
-      ta_commit(bar_at(&sh.ak_empty), el);
       ta_commit(bar_at(&sh.s_full), el);
       qk++;
       return true;
@@ -1194,9 +1257,8 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
           const uint32_t ta = (uint32_t)(kTerms >> (8 * i)) & 15, tb = (uint32_t)(kTerms >> (8 * i + 4)) & 15;
           const uint32_t at = av + ta * (kTilePos / 2);
           const uint64_t pt = pd + tb * (S::kPTerm >> 4);
-#pragma unroll
-          for (int k = 0; k < kTilePos / 16; k++)
-            ta_mma(d, at + k * 8, pt + k * 2 * NR, idesc, (i | k) != 0, el);
+          ta_mma4(d, at, pt, 2 * NR, idesc, i != 0, el);
+          ta_mma4(d, at + 32, pt + 8 * NR, 2 * NR, idesc, true, el);
         }
         ta_commit(bar_at(&sh.o_full), el);
         ta_commit(bar_at(&sh.av_empty[vb]), el);
@@ -1220,32 +1282,32 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
   }
 }
 
-// Merges the segments of the units that several CTAs share: block (c, y) the
-// unit that CTA c is the second one of, rows y, y + gridDim.y, ...
+// Merges the segments of the units that several CTAs share: block (c, y) rows
+// 4 y .. 4 y + 3 of the unit that CTA c is the second one of.
 template <int HD, int NR>
-__global__ void __launch_bounds__(HD) tree_combine_kernel(const __grid_constant__ TreeArgs a, int ctas) {
+__global__ void __launch_bounds__(HD * 4) tree_combine_kernel(const __grid_constant__ TreeArgs a, int ctas) {
   pdl_wait();
-  const int c = blockIdx.x + 1, h = threadIdx.x;
+  const int c = blockIdx.x + 1, h = threadIdx.x % HD, r = blockIdx.y * 4 + threadIdx.x / HD;
   const TaDesc d = reinterpret_cast<const TaDesc*>(a.workspace)[c];
+  if (d.nseg == 0 || r >= d.rows) return;
+  constexpr size_t kSeg = ta_seg_floats<HD, NR>();
   const float* segs = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.workspace) + ctas * sizeof(TaDesc));
-  for (int r = blockIdx.y; d.nseg > 0 && r < d.rows; r += gridDim.y) {
-    auto seg = [&](int i) {
-      return segs + (size_t)(i == 0 ? 2 * (c - 1) + 1 : 2 * (c + i - 1)) * ta_seg_floats<HD, NR>();
-    };
-    float m = kUnset;
-    for (int i = 0; i < d.nseg; i++) m = fmaxf(m, seg(i)[2 * r]);
-    float l = 0.0f, o = 0.0f;
-    for (int i = 0; i < d.nseg; i++) {
-      const float* s = seg(i);
-      const float f = s[2 * r] == kUnset ? 0.0f : exp2f(s[2 * r] - m);
-      if (s[2 * r] == kUnset) continue;
-      l = fmaf(s[2 * r + 1], f, l);
-      o = fmaf(s[2 * NR + r * HD + h], f, o);
-    }
-    const int row = d.row0 + r;
-    a.out[(size_t)(d.s + row / a.group) * a.out_ld +
-          ((size_t)d.kvh * a.group + row % a.group) * HD + h] = l == 0.0f ? 0.0f : o / l;
+  // the first segment ends CTA c - 1, the others start CTAs c, c + 1, ...
+  const float* first = segs + (2 * (size_t)(c - 1) + 1) * kSeg;
+  const float* next = segs + 2 * (size_t)c * kSeg;
+  float m = first[2 * r], l = m == kUnset ? 0.0f : first[2 * r + 1], o = m == kUnset ? 0.0f : first[2 * NR + r * HD + h];
+#pragma unroll 4
+  for (int i = 1; i < d.nseg; i++, next += 2 * kSeg) {
+    const float mi = next[2 * r], li = next[2 * r + 1], oi = next[2 * NR + r * HD + h];
+    if (mi == kUnset) continue;
+    const float top = fmaxf(m, mi), f = m == kUnset ? 0.0f : exp2f(m - top), g = exp2f(mi - top);
+    l = l * f + li * g;
+    o = o * f + oi * g;
+    m = top;
   }
+  const int row = d.row0 + r;
+  a.out[(size_t)(d.s + row / a.group) * a.out_ld + ((size_t)d.kvh * a.group + row % a.group) * HD + h] =
+      l == 0.0f ? 0.0f : o / l;
 }
 
 // Rows a unit: the smallest of 16, 32, 64 that holds a tree's rows.
@@ -1273,7 +1335,7 @@ cudaError_t launch(const TreeArgs& a, int sms, cudaStream_t st) {
   if (e != cudaSuccess || ctas < 2 || a.max_len <= kTilePos) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas - 1, NR / 4);
-  cfg.blockDim = dim3(HD);
+  cfg.blockDim = dim3(HD * 4);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
