@@ -222,6 +222,14 @@ __device__ __forceinline__ float2 ta_fma2(float2 a, float2 b, float2 c) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
   return d;
 }
+__device__ __forceinline__ float2 ta_mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n"
+      " mul.rn.f32x2 w, x, y;\n mov.b64 {%0, %1}, w;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
 __device__ __forceinline__ float2 ta_add2(float2 a, float2 b) {
   float2 d;
   asm("{\n .reg .b64 x, y, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n"
@@ -459,11 +467,13 @@ __device__ __forceinline__ void decode_k(const uint8_t* raw, uint32_t at, int r,
     const uint8_t* code = raw + q8_k_code(r, half * kSteps * 16);
     const uint8_t* scale = raw + q8_k_scale(HD, r, half * kSteps / 2);
     uint4 w4 = *reinterpret_cast<const uint4*>(code);
+    __half d1 = *reinterpret_cast<const __half*>(scale);
 #pragma unroll 1
-    for (int b = 0; b < kSteps; b++) {
+    for (int b = 0; b < kSteps; b++) {  // the next step's words are under way
       uint32_t hi[8], lo[8];
-      const __half2 d2 = __half2half2(*reinterpret_cast<const __half*>(scale + (b >> 1) * 2));
+      const __half2 d2 = __half2half2(d1);
       const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+      d1 = *reinterpret_cast<const __half*>(scale + ((b + 1 < kSteps ? b + 1 : b) >> 1) * 2);
       if (b + 1 < kSteps) w4 = *reinterpret_cast<const uint4*>(code + (b + 1) * kPageSize * 16);
 #pragma unroll
       for (int i = 0; i < 4; i++) {
@@ -511,17 +521,28 @@ __device__ __forceinline__ void decode_v(const uint8_t* raw, uint32_t col, int w
   using S = TaShape<HD, DT, NR>;
   const int h = w * 32 + lane;
   if constexpr (DT == LRS_KV_Q8_0) {
+    // 16 positions a step (8 columns a term); the next step's words are under way
+    const uint8_t* code = raw + q8_v_code(HD, 0, h);
+    const uint8_t* scale = raw + q8_v_scale(HD, 0, w);
+    uint32_t cw[4];
+    uint4 d8[2];
+    auto fetch = [&](int g) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) cw[i] = *reinterpret_cast<const uint32_t*>(code + (g * 4 + i) * HD * 4);
+#pragma unroll
+      for (int i = 0; i < 2; i++) d8[i] = *reinterpret_cast<const uint4*>(scale + g * 32 + i * 16);
+    };
+    fetch(0);
 #pragma unroll 1
-    for (int g = 0; g < S::kSlotPos / 16; g++) {  // 16 positions: 8 columns a term
+    for (int g = 0; g < S::kSlotPos / 16; g++) {
       uint32_t x[2][8];
-      uint4 d8;
+      const uint32_t c[4] = {cw[0], cw[1], cw[2], cw[3]};
+      const uint32_t d[8] = {d8[0].x, d8[0].y, d8[0].z, d8[0].w, d8[1].x, d8[1].y, d8[1].z, d8[1].w};
+      if (g + 1 < S::kSlotPos / 16) fetch(g + 1);
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        const int r = g * 16 + i * 4;
-        if (i % 2 == 0) d8 = *reinterpret_cast<const uint4*>(raw + q8_v_scale(HD, r, w));
-        const uint32_t cw = *reinterpret_cast<const uint32_t*>(raw + q8_v_code(HD, r, h));
         uint32_t hi[2], lo[2];
-        ta_q8(cw, ta_u2(i % 2 ? d8.z : d8.x), ta_u2(i % 2 ? d8.w : d8.y), hi, lo);
+        ta_q8(c[i], ta_u2(d[2 * i]), ta_u2(d[2 * i + 1]), hi, lo);
         x[0][i * 2] = hi[0], x[0][i * 2 + 1] = hi[1];
         x[1][i * 2] = lo[0], x[1][i * 2 + 1] = lo[1];
       }
@@ -589,41 +610,45 @@ __device__ __forceinline__ void load_q(const TreeArgs& a, const TaUnit& it, uint
   const int groups = 2 * ((it.rows + 15) >> 4);
 #pragma unroll 1
   for (int g8 = w; g8 < groups; g8 += 4) {
-    const int gr = g8 * 8 + (lane & 7), row = it.row0 + gr;
-    const float* src = a.q + (size_t)(it.s + row / a.group) * a.q_ld +
-                       (size_t)(it.kvh * a.group + row % a.group) * HD + (lane >> 3) * 8;
+    const int gr = g8 * 8 + (lane & 7), row = it.row0 + gr, node = row / a.group;
+    const float* src = a.q + (size_t)(it.s + node) * a.q_ld +
+                       (size_t)(it.kvh * a.group + row - node * a.group) * HD + (lane >> 3) * 8;
     float x[HD / 32][8];
+    if (gr >= it.rows) {
 #pragma unroll
-    for (int j = 0; j < HD / 32; j++) {
-      if (gr >= it.rows) {
+      for (int j = 0; j < HD / 32; j++)
 #pragma unroll
         for (int e = 0; e < 8; e++) x[j][e] = 0.0f;
-      } else if (vec) {
-        const float4 f0 = *reinterpret_cast<const float4*>(src + j * 32), f1 = *reinterpret_cast<const float4*>(src + j * 32 + 4);
-        x[j][0] = f0.x, x[j][1] = f0.y, x[j][2] = f0.z, x[j][3] = f0.w;
-        x[j][4] = f1.x, x[j][5] = f1.y, x[j][6] = f1.z, x[j][7] = f1.w;
-      } else {
+    } else if (vec) {
+#pragma unroll
+      for (int j = 0; j < HD / 32; j++)
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(src + j * 32 + e);
+          x[j][e] = f.x, x[j][e + 1] = f.y, x[j][e + 2] = f.z, x[j][e + 3] = f.w;
+        }
+    } else {
+#pragma unroll
+      for (int j = 0; j < HD / 32; j++)
 #pragma unroll
         for (int e = 0; e < 8; e++) x[j][e] = src[j * 32 + e];
-      }
     }
-    float mx = 0.0f;
-#pragma unroll
-    for (int j = 0; j < HD / 32; j++)
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        x[j][e] *= qs;
-        mx = fmaxf(mx, fabsf(x[j][e]));
-      }
-    float up0 = 1.0f, up1 = 1.0f, down = 1.0f;
+    // f16: times 2^k, k of the row's largest magnitude; the power may pass f32's
+    // range, so up to 2^60 of it goes with the scale and the rest on its own
+    float f0 = qs, f1 = 1.0f, down = 1.0f;
     if constexpr (S::kF16) {
+      float mx = 0.0f;
+#pragma unroll
+      for (int j = 0; j < HD / 32; j++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[j][e]));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16)) * fabsf(qs);
       const int e = (int)(__float_as_uint(mx) >> 23);
-      if (mx > 0.0f && e < 255) {  // 2^(137 - e), as two factors: it may pass f32's range
-        const int k = 137 - e, k0 = k >> 1;
-        up0 = __uint_as_float((uint32_t)(127 + k0) << 23);
-        up1 = __uint_as_float((uint32_t)(127 + k - k0) << 23);
+      if (mx > 0.0f && e < 255) {
+        const int k = 137 - e, k0 = max(-60, min(60, k));
+        f0 = qs * __uint_as_float((uint32_t)(127 + k0) << 23);
+        f1 = ldexpf(1.0f, k - k0);
         down = ldexpf(1.0f, -k);
       }
     }
@@ -633,8 +658,8 @@ __device__ __forceinline__ void load_q(const TreeArgs& a, const TaUnit& it, uint
       uint32_t y[S::kB][4];
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        float2 v = make_float2(x[j][2 * e], x[j][2 * e + 1]);
-        if constexpr (S::kF16) v = make_float2(v.x * up0 * up1, v.y * up0 * up1);
+        float2 v = ta_mul2(make_float2(x[j][2 * e], x[j][2 * e + 1]), make_float2(f0, f0));
+        if constexpr (S::kF16) v = ta_mul2(v, make_float2(f1, f1));
         uint32_t z[S::kB];
         ta_split<S::kF16, S::kB>(v, z);
 #pragma unroll
