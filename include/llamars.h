@@ -183,7 +183,8 @@ enum { LRS_KV_F32 = 0, LRS_KV_BF16 = 1, LRS_KV_Q8_0 = 2 };
 typedef struct lrs_model_options {
   uint32_t max_seq_len;   /* context per sequence (KVCache::new max_seq_len, src/cache.rs:12-36) */
   uint32_t max_sequences; /* concurrent sequences (slots) */
-  uint32_t kv_dtype;      /* LRS_KV_F32 (default, parity) or LRS_KV_BF16 */
+  uint32_t kv_dtype;      /* LRS_KV_F32 (default, parity), LRS_KV_BF16 or LRS_KV_Q8_0 (quantised as
+                             it is written; steps run one kernel each, persistent_decode is ignored) */
   uint32_t use_graph;     /* capture decode steps in a CUDA graph (1 = yes) */
   uint32_t device_recipe; /* LRS_RECIPE_* (llamars_synth.h): F32/F16/BF16 matrices are encoded
                              on the GPU at creation (maybe_quantize, src/loader.rs:406-447); 0 = as given */
@@ -364,6 +365,32 @@ lrs_status lrs_tree_attention(lrs_backend* backend, const lrs_kv_cache* cache,
                               const lrs_tree_batch* trees, const float* d_q, size_t q_ld,
                               float* d_out, size_t out_ld, uint32_t n_heads, float scale,
                               void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* Token trees of the models: parents[i] < i is the node that node i follows, -1 =
+ * the last committed position.  Checks a tree of n nodes (no CUDA call). */
+lrs_status lrs_tree_check(const int32_t* parents, size_t n);
+
+/* A forward pass over a drafted tree: node i is token tokens[i], held at position
+ * start_pos + i of slot `seq` (whose positions below start_pos are committed) and
+ * rotated as position start_pos + its depth; argmax_out[i] is the greedy token
+ * after it.  Any cache type; under tensor parallelism every rank makes the call. */
+lrs_status lrs_model_verify_tree(lrs_model* model, uint32_t seq, const uint32_t* tokens,
+                                 const int32_t* parents, size_t n, uint32_t start_pos,
+                                 uint32_t* argmax_out);
+
+/* The path that greedy decoding takes through a verified tree, from node 0 (a
+ * token already chosen): a child is taken when it is its parent's argmax.
+ * nodes_out (room for n) gets the path's *n_out nodes, *next_out the token after
+ * the last one.  No CUDA call. */
+lrs_status lrs_tree_greedy_path(const uint32_t* tokens, const int32_t* parents,
+                                const uint32_t* argmax, size_t n, uint32_t* nodes_out,
+                                size_t* n_out, uint32_t* next_out);
+
+/* Keeps a path of the tree last verified at start_pos: its nodes' K and V move to
+ * positions start_pos, start_pos + 1, ... in every layer, and the slot continues
+ * at start_pos + n.  `nodes` ascends. */
+lrs_status lrs_model_accept_tree(lrs_model* model, uint32_t seq, uint32_t start_pos,
+                                 const uint32_t* nodes, size_t n);
 
 /* Keeps one path of each tree: node d_nodes[d_start[t] + j] of tree t, held at
  * position d_ctx[t] + d_nodes[..], moves to position d_ctx[t] + j, in each of the

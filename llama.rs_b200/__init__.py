@@ -284,6 +284,13 @@ _sig("lrs_tree_attention_workspace", C.c_int32, _P, _KV, C.POINTER(TreeBatch), C
 _sig("lrs_tree_attention", C.c_int32, _P, _KV, C.POINTER(TreeBatch), _P, C.c_size_t, _P,
      C.c_size_t, C.c_uint32, C.c_float, _P, C.c_size_t, _P)
 
+_I32 = C.POINTER(C.c_int32)
+_sig("lrs_tree_check", C.c_int32, _I32, C.c_size_t)
+_sig("lrs_tree_greedy_path", C.c_int32, _U32, _I32, _U32, C.c_size_t, _U32,
+     C.POINTER(C.c_size_t), _U32)
+_sig("lrs_model_verify_tree", C.c_int32, _P, C.c_uint32, _U32, _I32, C.c_size_t, C.c_uint32, _U32)
+_sig("lrs_model_accept_tree", C.c_int32, _P, C.c_uint32, C.c_uint32, _U32, C.c_size_t)
+
 #: every symbol include/*.h declares (checked by the CPU tests)
 EXPORTED_SYMBOLS = (
     "lrs_last_error", "lrs_type_geometry", "lrs_backend_create", "lrs_backend_destroy",
@@ -303,7 +310,8 @@ EXPORTED_SYMBOLS = (
     "lrs_st_open", "lrs_st_close", "lrs_st_tensor_count", "lrs_st_tensor", "lrs_st_qwen2_desc",
     "lrs_model_load", "lrs_loaded_close",
     "lrs_kv_check", "lrs_kv_store", "lrs_kv_load", "lrs_kv_accept",
-    "lrs_tree_attention_workspace", "lrs_tree_attention",
+    "lrs_tree_attention_workspace", "lrs_tree_attention", "lrs_tree_check", "lrs_tree_greedy_path",
+    "lrs_model_verify_tree", "lrs_model_accept_tree",
 )
 
 
@@ -781,12 +789,16 @@ class CudaQwen2Model:
                  max_sequences: int = 1, kv_bf16: bool = False, use_graph: bool = True,
                  keepalive=None, tp_rank: int = 0, tp_world: int = 1, tp_id: bytes = b"",
                  device_recipe: LoadQuantization = LoadQuantization.NONE,
-                 tp_p2p: bool = False, persistent_decode: bool = False):
+                 tp_p2p: bool = False, persistent_decode: bool = False,
+                 kv_dtype: Optional[KvType] = None):
         """tp_world > 1 makes this process shard tp_rank of a tensor-parallel
         model (every rank passes the full desc and the same tp_id, made once by
         tp_unique_id() and shared out of band).  device_recipe encodes the
-        desc's F32/F16/BF16 matrices on the GPU (the load-time recipe)."""
-        opts = _ModelOptions(max_seq_len, max_sequences, 1 if kv_bf16 else 0,
+        desc's F32/F16/BF16 matrices on the GPU (the load-time recipe).
+        kv_dtype is the KV cache's type (kv_bf16=True is KvType.BF16)."""
+        if kv_dtype is None:
+            kv_dtype = KvType.BF16 if kv_bf16 else KvType.F32
+        opts = _ModelOptions(max_seq_len, max_sequences, int(KvType(kv_dtype)),
                              1 if use_graph else 0, int(device_recipe), 1 if tp_p2p else 0,
                              1 if persistent_decode else 0)
         h = _P()
@@ -851,6 +863,23 @@ class CudaQwen2Model:
         _check(_lib.lrs_model_forward_sample(self._h, seq, token_id, pos, C.byref(params),
                                              _uptr(r), r.size, u, _uptr(out)))
         return int(out[0])
+
+    def verify_tree(self, tokens: Sequence[int], parents: Sequence[int], start_pos: int,
+                    seq: int = 0) -> np.ndarray:
+        """One forward pass over a drafted token tree (lrs_model_verify_tree):
+        the greedy token after each node.  parents[i] < i, -1 = the last
+        committed position."""
+        t, p = _tree(tokens, parents)
+        out = np.zeros(t.size, dtype=np.uint32)
+        _check(_lib.lrs_model_verify_tree(self._h, seq, _uptr(t), p.ctypes.data_as(_I32), t.size,
+                                          start_pos, _uptr(out)))
+        return out
+
+    def accept_tree(self, nodes: Sequence[int], start_pos: int, seq: int = 0) -> None:
+        """Keeps a path of the tree verified at start_pos (lrs_model_accept_tree):
+        the slot continues at start_pos + len(nodes)."""
+        n = np.ascontiguousarray(nodes, dtype=np.uint32)
+        _check(_lib.lrs_model_accept_tree(self._h, seq, start_pos, _uptr(n), n.size))
 
     def prefill(self, tokens: Sequence[int], start_pos: int = 0, seq: int = 0,
                 want_logits: bool = True):
@@ -1246,6 +1275,28 @@ def write_qwen2_safetensors(model_dir: str, desc, dtype: str = "F32", shards: in
     with open(os.path.join(model_dir, "model.safetensors.index.json"), "w") as f:
         json.dump({"metadata": {"total_size": sum(len(t[3]) for t in tensors)},
                    "weight_map": weight_map}, f)
+
+
+def _tree(tokens, parents):
+    t = np.ascontiguousarray(tokens, dtype=np.uint32)
+    p = np.ascontiguousarray(parents, dtype=np.int32)
+    if t.ndim != 1 or t.shape != p.shape:
+        raise LrsError(1, "a tree has one parent per token")
+    return t, p
+
+
+def greedy_path(tokens: Sequence[int], parents: Sequence[int], argmax: Sequence[int]):
+    """The nodes that greedy decoding takes through a verified tree, from node 0,
+    and the token after them (lrs_tree_greedy_path)."""
+    t, p = _tree(tokens, parents)
+    a = np.ascontiguousarray(argmax, dtype=np.uint32)
+    if a.shape != t.shape:
+        raise LrsError(1, "a tree has one argmax per token")
+    nodes = np.zeros(max(1, t.size), dtype=np.uint32)
+    n, nxt = C.c_size_t(), C.c_uint32()
+    _check(_lib.lrs_tree_greedy_path(_uptr(t), p.ctypes.data_as(_I32), _uptr(a), t.size, _uptr(nodes),
+                                     C.byref(n), C.byref(nxt)))
+    return nodes[:n.value].tolist(), int(nxt.value)
 
 
 def sampler_check(params: Sampler, vocab: int) -> None:

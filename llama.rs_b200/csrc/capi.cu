@@ -401,7 +401,6 @@ struct lrs_model {
   std::vector<int> free_pages;
   std::vector<std::vector<int>> seq_pages;
   int* d_pages = nullptr;
-  size_t kv_elem = 4;
   // activations, for up to max_items items per step
   int max_items = 0, max_split = 64;
   float *residual = nullptr, *xn = nullptr, *q = nullptr, *k = nullptr, *v = nullptr,
@@ -435,6 +434,12 @@ struct lrs_model {
   unsigned long long* keys = nullptr;
   int *d_tok = nullptr, *d_pos = nullptr, *d_seq = nullptr, *d_step = nullptr;
   unsigned* d_attn_cnt = nullptr;  // [max_items][kv heads] split counters of the fused attention
+  // the tree attention (q8_0 caches, verification): node starts of a batch of one-node trees
+  // (0, 1, 2, ...) and of one tree (0, n), a verified tree's cells, committed positions and
+  // masks, and the kernel's workspace
+  int *d_iota = nullptr, *d_span = nullptr, *d_cell = nullptr, *d_ctx = nullptr, *d_nodes = nullptr;
+  unsigned long long* d_mask = nullptr;
+  void* tree_ws = nullptr;
   // batch-1 steps run the projections of a second GGML type among q/k/v (v
   // in Q8_0 under q4km) on a side stream, beside the first type's launch
   cudaStream_t side = nullptr;
@@ -588,12 +593,42 @@ int32_t ensure_pages(lrs_model* m, int seq, uint32_t last_pos) {
   return LRS_OK;
 }
 
+KvView kv_view(const lrs_model* m, const Layer& L) {
+  return KvView{static_cast<uint8_t*>(L.kpool), static_cast<uint8_t*>(L.vpool), m->d_pages, m->total_pages,
+                (int)m->opt.max_sequences, m->pages_per_seq, (int)m->c.num_key_value_heads, m->be->d_err};
+}
+
+// Attention arguments of `nodes` items, B one-node trees (a decode step) or one
+// tree (a prompt chunk: a chain; a verified tree: d_mask).
+TreeArgs tree_step(const lrs_model* m, const Layer& L, int B, bool one_tree, bool verify) {
+  const lrs_config& c = m->c;
+  TreeArgs t{};
+  t.c = kv_view(m, L);
+  t.seq = m->d_seq;
+  t.ctx = verify ? m->d_ctx : m->d_pos;
+  t.start = one_tree ? m->d_span : m->d_iota;
+  t.mask = verify ? m->d_mask : nullptr;
+  t.n_trees = one_tree ? 1 : B;
+  t.n_nodes = B;
+  t.max_nodes = one_tree ? B : 1;
+  t.max_len = (int)m->opt.max_seq_len;
+  t.q = m->q;
+  t.out = m->att;
+  t.q_ld = t.out_ld = (long long)c.num_attention_heads * c.head_dim;
+  t.group = (int)(c.num_attention_heads / c.num_key_value_heads);
+  t.scale = 1.0f / sqrtf((float)c.head_dim);
+  t.workspace = m->tree_ws;
+  return t;
+}
+
 // Queues one forward step for items 0..B-1 (d_tok / d_pos / d_seq already set):
 // Qwen2Model::forward_impl, src/model.rs:135-270, for B tokens at once.  When
 // `lm_item` >= 0 only that item runs the final norm + LM head (prefill);
 // lm_item == -1 runs it for every item; -2 skips it.
+// `verify`: the items are the nodes of one tree (d_cell / d_ctx / d_mask set, d_pos the
+// positions of their rotation).
 int32_t enqueue_step(lrs_model* m, int B, int lm_item, bool want_logits, bool greedy_advance,
-                     int n_steps_cap) {
+                     int n_steps_cap, bool verify = false) {
   const lrs_config& c = m->c;
   cudaStream_t st = m->be->stream;
   const int h = c.hidden_size, I = c.intermediate_size, nh = c.num_attention_heads,
@@ -698,18 +733,27 @@ int32_t enqueue_step(lrs_model* m, int B, int lm_item, bool want_logits, bool gr
     // every item its own sequence (a decode step): RoPE, the KV store and the
     // split merge run inside the attention kernel; prefill chunks (items of
     // one sequence read each other's rows) store every row first
-    const bool fused_attn = lm_item == -1 || B == 1;
-    if (!fused_attn)
-      LRS_CUDA(launch_rope_store(m->q, m->k, m->v, m->rope_cos, m->rope_sin, io, B, nh, nkv, hd,
-                                 L.kpool, L.vpool, kv_bf16, st));
-    AttnLaunch al{};
-    al.q = m->q, al.k = m->k, al.v = m->v, al.cos_t = m->rope_cos, al.sin_t = m->rope_sin;
-    al.io = io;
-    al.batch = B, al.nh = nh, al.nkv = nkv, al.hd = hd, al.kv_bf16 = kv_bf16, al.nsplit = nsplit;
-    al.kpool = L.kpool, al.vpool = L.vpool;
-    al.part = m->part, al.att = m->att, al.cnt = m->d_attn_cnt, al.err = m->be->d_err;
-    al.fused = fused_attn;
-    LRS_CUDA(launch_attention(al, st));
+    const bool fused_attn = (lm_item == -1 && !verify) || B == 1;
+    if (verify || m->opt.kv_dtype == LRS_KV_Q8_0) {
+      // rows rotated, written in the cache's type, attended to as trees
+      LRS_CUDA(launch_rope(m->q, m->k, m->rope_cos, m->rope_sin, m->d_pos, B, nh, nkv, hd, st));
+      const KvStoreArgs sa{kv_view(m, L), m->d_seq, verify ? m->d_cell : m->d_pos, B, m->k, m->v, kvw};
+      LRS_CUDA(launch_kv_store(sa, m->opt.kv_dtype, hd, sms, st));
+      LRS_CUDA(launch_tree_attention(tree_step(m, L, B, !fused_attn || verify, verify), m->opt.kv_dtype, hd,
+                                     sms, st));
+    } else {
+      if (!fused_attn)
+        LRS_CUDA(launch_rope_store(m->q, m->k, m->v, m->rope_cos, m->rope_sin, io, B, nh, nkv, hd,
+                                   L.kpool, L.vpool, kv_bf16, st));
+      AttnLaunch al{};
+      al.q = m->q, al.k = m->k, al.v = m->v, al.cos_t = m->rope_cos, al.sin_t = m->rope_sin;
+      al.io = io;
+      al.batch = B, al.nh = nh, al.nkv = nkv, al.hd = hd, al.kv_bf16 = kv_bf16, al.nsplit = nsplit;
+      al.kpool = L.kpool, al.vpool = L.vpool;
+      al.part = m->part, al.att = m->att, al.cnt = m->d_attn_cnt, al.err = m->be->d_err;
+      al.fused = fused_attn;
+      LRS_CUDA(launch_attention(al, st));
+    }
     if (a1) cudaEventRecord(a1, st);
     // o_proj + residual (src/model.rs:233-238)
     GemvMat om = mat_of(L.o, res_out(), h);
@@ -808,7 +852,7 @@ int32_t enqueue_step(lrs_model* m, int B, int lm_item, bool want_logits, bool gr
 // or x rows wider than shared memory) keep the per-kernel step.
 int32_t setup_step1(lrs_model* m) {
   const lrs_config& c = m->c;
-  if (m->tp_world != 1 || !m->opt.persistent_decode) return LRS_OK;
+  if (m->tp_world != 1 || !m->opt.persistent_decode || m->opt.kv_dtype == LRS_KV_Q8_0) return LRS_OK;
   if ((c.head_dim != 64 && c.head_dim != 128) || c.num_attention_heads / c.num_key_value_heads > 8)
     return LRS_OK;
   int coop = 0;
@@ -923,11 +967,15 @@ int32_t enqueue_step1(lrs_model* m) {
   return LRS_OK;
 }
 
-int32_t set_items(lrs_model* m, int n, const int* tok, const int* pos, const int* seq) {
+// one_tree: the items' attention runs as one tree (tree_step).
+int32_t set_items(lrs_model* m, int n, const int* tok, const int* pos, const int* seq,
+                  bool one_tree = false) {
   cudaStream_t st = m->be->stream;
   LRS_CUDA(cudaMemcpyAsync(m->d_tok, tok, n * sizeof(int), cudaMemcpyHostToDevice, st));
   LRS_CUDA(cudaMemcpyAsync(m->d_pos, pos, n * sizeof(int), cudaMemcpyHostToDevice, st));
   LRS_CUDA(cudaMemcpyAsync(m->d_seq, seq, n * sizeof(int), cudaMemcpyHostToDevice, st));
+  const int span[2] = {0, n};
+  if (one_tree) LRS_CUDA(cudaMemcpyAsync(m->d_span, span, sizeof span, cudaMemcpyHostToDevice, st));
   // the host arrays may go out of scope: make the copies complete
   LRS_CUDA(cudaStreamSynchronize(st));
   return LRS_OK;
@@ -1102,6 +1150,7 @@ int32_t create_model(lrs_backend* be, const lrs_model_desc* d, const lrs_model_o
   opt.kv_dtype = LRS_KV_F32;
   opt.use_graph = 1;
   if (options) opt = *options;
+  if (opt.kv_dtype > LRS_KV_Q8_0) opt.kv_dtype = LRS_KV_F32;
   if (opt.max_seq_len == 0 || opt.max_seq_len > c.max_position_embeddings)
     return fail(LRS_ERR_INVALID, "requested context " + std::to_string(opt.max_seq_len) +
                                      " exceeds model limit " +
@@ -1222,13 +1271,13 @@ int32_t create_model(lrs_backend* be, const lrs_model_desc* d, const lrs_model_o
       return cleanup(rc);
   }
   // Paged KV pools.
-  m->kv_elem = opt.kv_dtype == LRS_KV_BF16 ? 2 : 4;
+  const size_t page_bytes = (size_t)cl.num_key_value_heads *
+                            kv_tile_bytes(opt.kv_dtype, c.head_dim);
   m->pages_per_seq = (int)((opt.max_seq_len + kPageSize - 1) / kPageSize);
   m->total_pages = m->pages_per_seq * (int)opt.max_sequences;
-  const size_t page_elems = (size_t)cl.num_key_value_heads * kPageSize * c.head_dim;
   for (auto& L : m->layers) {
-    if ((rc = model_alloc(m.get(), &L.kpool, (size_t)m->total_pages * page_elems * m->kv_elem)) ||
-        (rc = model_alloc(m.get(), &L.vpool, (size_t)m->total_pages * page_elems * m->kv_elem)))
+    if ((rc = model_alloc(m.get(), &L.kpool, (size_t)m->total_pages * page_bytes)) ||
+        (rc = model_alloc(m.get(), &L.vpool, (size_t)m->total_pages * page_bytes)))
       return cleanup(rc);
   }
   for (int pg = m->total_pages - 1; pg >= 0; pg--) m->free_pages.push_back(pg);
@@ -1259,6 +1308,25 @@ int32_t create_model(lrs_backend* be, const lrs_model_desc* d, const lrs_model_o
       (rc = model_alloc(m.get(), (void**)&m->d_attn_cnt, B * c.num_key_value_heads * 4)))
     return cleanup(rc);
   LRS_CUDA(cudaMemset(m->d_attn_cnt, 0, B * c.num_key_value_heads * 4));
+  {
+    // the workspace of the largest step: one tree of 64 nodes, or max_items of one node
+    size_t ws = 0;
+    for (int one : {1, 0})
+      ws = std::max(ws, tree_attention_workspace_bytes(
+                            tree_step(m.get(), m->layers[0], one ? LRS_TREE_MAX_NODES : (int)B, one != 0, false),
+                            (int)c.head_dim, be->sms));
+    if ((rc = model_alloc(m.get(), (void**)&m->d_iota, (B + 1) * 4)) ||
+        (rc = model_alloc(m.get(), (void**)&m->d_span, 2 * 4)) ||
+        (rc = model_alloc(m.get(), (void**)&m->d_cell, LRS_TREE_MAX_NODES * 4)) ||
+        (rc = model_alloc(m.get(), (void**)&m->d_ctx, 4)) ||
+        (rc = model_alloc(m.get(), (void**)&m->d_nodes, LRS_TREE_MAX_NODES * 4)) ||
+        (rc = model_alloc(m.get(), (void**)&m->d_mask, LRS_TREE_MAX_NODES * 8)) ||
+        (rc = model_alloc(m.get(), &m->tree_ws, ws)))
+      return cleanup(rc);
+    std::vector<int> iota(B + 1);
+    for (size_t i = 0; i <= B; i++) iota[i] = (int)i;
+    LRS_CUDA(cudaMemcpy(m->d_iota, iota.data(), (B + 1) * 4, cudaMemcpyHostToDevice));
+  }
   LRS_CUDA(cudaStreamCreateWithFlags(&m->side, cudaStreamNonBlocking));
   LRS_CUDA(cudaEventCreateWithFlags(&m->ev_fork, cudaEventDisableTiming));
   LRS_CUDA(cudaEventCreateWithFlags(&m->ev_join, cudaEventDisableTiming));
@@ -1456,7 +1524,7 @@ lrs_status lrs_model_prefill(lrs_model* m, uint32_t seq, const uint32_t* tokens,
       tok[i] = (int)tokens[c0 + i];
       pos[i] = (int)(start_pos + c0 + i);
     }
-    if ((rc = set_items(m, nb, tok.data(), pos.data(), sq.data()))) return rc;
+    if ((rc = set_items(m, nb, tok.data(), pos.data(), sq.data(), m->opt.kv_dtype == LRS_KV_Q8_0))) return rc;
     const bool last = c0 + nb == n;
     rc = enqueue_step(m, nb, last && want ? nb - 1 : -2, logits_out != nullptr, false, 0);
     if (rc) return rc;
@@ -1502,6 +1570,117 @@ lrs_status lrs_model_forward_sample(lrs_model* m, uint32_t seq, uint32_t token, 
                          d_recent, (int)n_recent, *params, u, d_out, m->be->stream));
   LRS_CUDA(cudaMemcpyAsync(next_out, d_out, 4, cudaMemcpyDeviceToHost, m->be->stream));
   LRS_CUDA(cudaStreamSynchronize(m->be->stream));
+  return check_device_error(m->be);
+} catch (...) {
+  return lrs::status_of_current_exception();
+}
+
+lrs_status lrs_tree_check(const int32_t* parents, size_t n) try {
+  if (!parents) return fail(LRS_ERR_INVALID, "null argument");
+  if (n < 1 || n > LRS_TREE_MAX_NODES)
+    return fail(LRS_ERR_INVALID, "a tree has 1 to " + std::to_string(LRS_TREE_MAX_NODES) + " nodes");
+  for (size_t i = 0; i < n; i++)
+    if (parents[i] < -1 || parents[i] >= (int32_t)i)
+      return fail(LRS_ERR_INVALID, "node " + std::to_string(i) + " of the tree does not follow its parent " +
+                                       std::to_string(parents[i]));
+  return LRS_OK;
+} catch (...) {
+  return lrs::status_of_current_exception();
+}
+
+lrs_status lrs_tree_greedy_path(const uint32_t* tokens, const int32_t* parents, const uint32_t* argmax,
+                                size_t n, uint32_t* nodes_out, size_t* n_out, uint32_t* next_out) try {
+  if (!tokens || !argmax || !nodes_out || !n_out || !next_out) return fail(LRS_ERR_INVALID, "null argument");
+  int32_t rc = lrs_tree_check(parents, n);
+  if (rc) return rc;
+  size_t len = 0;
+  for (size_t at = 0;;) {
+    nodes_out[len++] = (uint32_t)at;
+    size_t i = at + 1;
+    while (i < n && (parents[i] != (int32_t)at || tokens[i] != argmax[at])) i++;
+    *next_out = argmax[at];
+    if (i == n) break;
+    at = i;
+  }
+  *n_out = len;
+  return LRS_OK;
+} catch (...) {
+  return lrs::status_of_current_exception();
+}
+
+lrs_status lrs_model_verify_tree(lrs_model* m, uint32_t seq, const uint32_t* tokens, const int32_t* parents,
+                                 size_t n, uint32_t start_pos, uint32_t* argmax_out) try {
+  if (!m || !tokens || !argmax_out) return fail(LRS_ERR_INVALID, "null argument");
+  int32_t rc = lrs_tree_check(parents, n);
+  if (rc) return rc;
+  if (seq >= m->opt.max_sequences) return fail(LRS_ERR_INVALID, "sequence slot out of range");
+  if ((size_t)start_pos + n > m->opt.max_seq_len)
+    return fail(LRS_ERR_INVALID, "position " + std::to_string((size_t)start_pos + n - 1) +
+                                     " exceeds configured context " + std::to_string(m->opt.max_seq_len));
+  int tok[LRS_TREE_MAX_NODES], pos[LRS_TREE_MAX_NODES], sq[LRS_TREE_MAX_NODES], cell[LRS_TREE_MAX_NODES];
+  unsigned long long mask[LRS_TREE_MAX_NODES];
+  for (size_t i = 0; i < n; i++) {
+    if (tokens[i] >= m->vocab_full)
+      return fail(LRS_ERR_INVALID, "token id " + std::to_string(tokens[i]) + " is outside vocabulary");
+    tok[i] = (int)tokens[i];
+    sq[i] = (int)seq;
+    cell[i] = (int)(start_pos + i);
+    pos[i] = parents[i] < 0 ? (int)start_pos : pos[parents[i]] + 1;
+    mask[i] = (parents[i] < 0 ? 0ull : mask[parents[i]]) | 1ull << i;
+  }
+  LRS_CUDA(cudaSetDevice(m->be->device));
+  if ((rc = ensure_pages(m, (int)seq, start_pos + (uint32_t)n - 1))) return rc;
+  cudaStream_t st = m->be->stream;
+  const int ctx = (int)start_pos;
+  LRS_CUDA(cudaMemcpyAsync(m->d_cell, cell, n * sizeof(int), cudaMemcpyHostToDevice, st));
+  LRS_CUDA(cudaMemcpyAsync(m->d_ctx, &ctx, sizeof(int), cudaMemcpyHostToDevice, st));
+  LRS_CUDA(cudaMemcpyAsync(m->d_mask, mask, n * sizeof(mask[0]), cudaMemcpyHostToDevice, st));
+  if ((rc = set_items(m, (int)n, tok, pos, sq, true))) return rc;
+  if ((rc = enqueue_step(m, (int)n, -1, false, false, 0, true))) return rc;
+  std::vector<unsigned long long> keys(n);
+  LRS_CUDA(cudaMemcpyAsync(keys.data(), m->keys, n * sizeof(keys[0]), cudaMemcpyDeviceToHost, st));
+  LRS_CUDA(cudaStreamSynchronize(st));
+  if ((rc = check_device_error(m->be))) return rc;
+  for (size_t i = 0; i < n; i++) argmax_out[i] = (uint32_t)(keys[i] & 0xffffffffull);
+  return LRS_OK;
+} catch (...) {
+  return lrs::status_of_current_exception();
+}
+
+lrs_status lrs_model_accept_tree(lrs_model* m, uint32_t seq, uint32_t start_pos, const uint32_t* nodes,
+                                 size_t n) try {
+  if (!m || (n && !nodes)) return fail(LRS_ERR_INVALID, "null argument");
+  if (seq >= m->opt.max_sequences) return fail(LRS_ERR_INVALID, "sequence slot out of range");
+  if (n == 0) return LRS_OK;
+  for (size_t i = 0; i < n; i++)
+    if (nodes[i] >= LRS_TREE_MAX_NODES || (i && nodes[i] <= nodes[i - 1]))
+      return fail(LRS_ERR_INVALID, "a path's nodes ascend, below " + std::to_string(LRS_TREE_MAX_NODES));
+  if (((size_t)start_pos + nodes[n - 1]) / kPageSize >= m->seq_pages[seq].size())
+    return fail(LRS_ERR_INVALID, "the path leaves the positions that slot " + std::to_string(seq) + " holds");
+  LRS_CUDA(cudaSetDevice(m->be->device));
+  cudaStream_t st = m->be->stream;
+  const int head[4] = {(int)seq, (int)start_pos, 0, (int)n};
+  LRS_CUDA(cudaMemcpyAsync(m->d_seq, &head[0], sizeof(int), cudaMemcpyHostToDevice, st));
+  LRS_CUDA(cudaMemcpyAsync(m->d_ctx, &head[1], sizeof(int), cudaMemcpyHostToDevice, st));
+  LRS_CUDA(cudaMemcpyAsync(m->d_span, &head[2], 2 * sizeof(int), cudaMemcpyHostToDevice, st));
+  LRS_CUDA(cudaMemcpyAsync(m->d_nodes, nodes, n * sizeof(int), cudaMemcpyHostToDevice, st));
+  std::vector<lrs_kv_cache> caches(m->layers.size());
+  for (size_t i = 0; i < caches.size(); i++) {
+    lrs_kv_cache& c = caches[i];
+    c.k_pool = m->layers[i].kpool;
+    c.v_pool = m->layers[i].vpool;
+    c.pages = m->d_pages;
+    c.n_pages = (uint32_t)m->total_pages;
+    c.n_seqs = m->opt.max_sequences;
+    c.max_pages = (uint32_t)m->pages_per_seq;
+    c.kv_heads = m->c.num_key_value_heads;
+    c.head_dim = m->c.head_dim;
+    c.kv_dtype = m->opt.kv_dtype;
+  }
+  int32_t rc = lrs_kv_accept(m->be, caches.data(), caches.size(), m->d_seq, m->d_ctx, m->d_span, m->d_nodes, 1,
+                             n, nullptr);
+  if (rc) return rc;
+  LRS_CUDA(cudaStreamSynchronize(st));
   return check_device_error(m->be);
 } catch (...) {
   return lrs::status_of_current_exception();

@@ -133,6 +133,21 @@ __global__ void __launch_bounds__(64)
   }
 }
 
+// RoPE of q and k in place, the rotation of rope_store_kernel (src/model.rs:86-95).
+__global__ void __launch_bounds__(64)
+    rope_kernel(float* q, float* k, const float* cos_t, const float* sin_t, const int* pos, int nh,
+                int nkv, int hd) {
+  const int b = blockIdx.x, h = blockIdx.y, half = hd / 2;
+  const float* c = cos_t + (size_t)pos[b] * half;
+  const float* s = sin_t + (size_t)pos[b] * half;
+  float* x = h < nh ? q + ((size_t)b * nh + h) * hd : k + ((size_t)b * nkv + h - nh) * hd;
+  for (int i = threadIdx.x; i < half; i += blockDim.x) {
+    const float re = x[i], im = x[i + half];
+    x[i] = __fsub_rn(__fmul_rn(re, c[i]), __fmul_rn(im, s[i]));
+    x[i + half] = __fadd_rn(__fmul_rn(re, s[i]), __fmul_rn(im, c[i]));
+  }
+}
+
 // ---- split-K GQA decode attention ------------------------------------------
 constexpr int kMaxGroup = 8;    // query heads per KV head handled by one CTA
 constexpr int kAttnWarps = 8;   // consumer warps; one more warp issues the copies
@@ -609,6 +624,12 @@ cudaError_t launch_dequant_rows(const uint8_t* w, uint32_t type, int cols, int r
 cudaError_t launch_rmsnorm(const float* x, const float* w, float eps, int n, int batch, float* out,
                            cudaStream_t st) {
   rmsnorm_kernel<<<batch, 256, 0, st>>>(x, w, eps, n, out);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_rope(float* q, float* k, const float* cos_t, const float* sin_t, const int* pos,
+                        int batch, int nh, int nkv, int hd, cudaStream_t st) {
+  rope_kernel<<<dim3(batch, nh + nkv), 64, 0, st>>>(q, k, cos_t, sin_t, pos, nh, nkv, hd);
   return cudaGetLastError();
 }
 

@@ -33,6 +33,9 @@ cudaError_t launch_rmsnorm(const float* x, const float* w, float eps, int n, int
 cudaError_t launch_rope_store(float* q, const float* k, const float* v, const float* cos_t,
                               const float* sin_t, StepIO io, int batch, int nh, int nkv, int hd,
                               void* kpool, void* vpool, int kv_bf16, cudaStream_t st);
+// RoPE of the q and k rows in place (launch_kv_store writes them then).
+cudaError_t launch_rope(float* q, float* k, const float* cos_t, const float* sin_t, const int* pos,
+                        int batch, int nh, int nkv, int hd, cudaStream_t st);
 // Split-K GQA decode attention over the paged cache (src/model.rs:206-231 with
 // softmax_inplace :298-313) into att[b][nh*hd].  Unfused: q already rotated
 // and the position's K/V already stored (launch_rope_store), a combine kernel

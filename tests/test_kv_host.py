@@ -155,3 +155,30 @@ def test_plain_attention_is_softmax(lrs):
     assert (err > 0).all() and err.max() < 1e-2
     empty, _ = kv_plain.attention(q, k, v, 0, [0] * n, 0.125)
     assert (empty == 0).all()
+
+
+# ----------------------------------------------------------- token trees -----
+@pytest.mark.parametrize("parents", [[0], [-2], [-1, 1], [-1, 0, 3], [], [-1] * 65], ids=str)
+def test_bad_parents_are_refused(lrs, parents):
+    n = len(parents)
+    with pytest.raises(lrs.LrsError) as e:
+        lrs.greedy_path([1] * n, parents, [1] * n)
+    assert e.value.code == INVALID
+
+
+def test_tree_arguments_of_different_lengths_are_refused(lrs):
+    for args in (([1, 2], [-1], [3, 3]), ([1], [-1], [3, 3])):
+        with pytest.raises(lrs.LrsError):
+            lrs.greedy_path(*args)
+
+
+@pytest.mark.parametrize("tokens,parents,argmax,path,nxt", [
+    ([5], [-1], [9], [0], 9),
+    ([5, 9], [-1, 0], [9, 4], [0, 1], 4),
+    ([5, 8, 9, 4], [-1, 0, 0, 2], [9, 1, 4, 7], [0, 2, 3], 7),      # the second child
+    ([5, 9, 9], [-1, -1, 0], [9, 3, 2], [0, 2], 2),                 # node 1 does not follow node 0
+    ([5, 9, 3, 9], [-1, 0, 1, 0], [9, 3, 6, 1], [0, 1, 2], 6),      # of two equal children the first
+    ([5, 6], [-1, 0], [9, 3], [0], 9),
+    (list(range(64)), list(range(-1, 63)), list(range(1, 65)), list(range(64)), 64)])
+def test_greedy_path(lrs, tokens, parents, argmax, path, nxt):
+    assert lrs.greedy_path(tokens, parents, argmax) == (path, nxt)
