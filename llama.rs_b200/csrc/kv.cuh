@@ -53,8 +53,7 @@ __device__ __forceinline__ int kv_page(const KvView& c, int seq, int pos) {
   return page;
 }
 
-// Rows (store: after RoPE of q and k when cos_t is given; rope_pos: positions
-// of the rotation, NULL = pos) and their slots and positions.
+// n rows of K and V, `ld` floats apart, and their slots and positions.
 struct KvStoreArgs {
   KvView c;
   const int* seq;
@@ -75,7 +74,7 @@ struct KvLoadArgs {
   float* v;
   long long ld;
 };
-cudaError_t launch_kv_load(const KvLoadArgs& a, uint32_t dtype, int hd, cudaStream_t st);
+cudaError_t launch_kv_load(const KvLoadArgs& a, uint32_t dtype, int hd, int sms, cudaStream_t st);
 
 struct TreeArgs {
   KvView c;

@@ -34,90 +34,145 @@ __device__ __forceinline__ uint32_t q8_code(float x, float inv) {
   const int i = r != r ? 0 : (int)fminf(fmaxf(r, -127.0f), 127.0f);
   return (uint32_t)i & 0xffu;
 }
+// Eight codes of a block whose products are finite and below 127.5: the sum with
+// 1.5 * 2^23 rounds a product to the nearest integer, ties to even.  False if one
+// is an exact tie, which goes away from zero (q8_code).
+__device__ __forceinline__ bool q8_codes(const float (&x)[8], float inv, uint32_t (&w)[2]) {
+  constexpr float kMagic = 12582912.0f;
+  float off = 0.0f;
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    uint32_t t[4];
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      // (scalar products: a packed one may be fused into the sums below)
+      const float2 y = make_float2(__fmul_rn(x[4 * h + i], inv), __fmul_rn(x[4 * h + i + 1], inv));
+      const float2 s = add2(y, make_float2(kMagic, kMagic));
+      const float2 r = add2(s, make_float2(-kMagic, -kMagic));
+      const float2 d = add2(y, make_float2(-r.x, -r.y));
+      off = fmaxf(off, fmaxf(fabsf(d.x), fabsf(d.y)));
+      t[i] = __float_as_uint(s.x), t[i + 1] = __float_as_uint(s.y);
+    }
+    w[h] = __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
+  }
+  return off < 0.5f;
+}
 
 // Rows [blockIdx.x * rows, + rows) of K (blockIdx.z = 0) or V (1) of head
-// blockIdx.y.  A lane owns four consecutive columns.  Q8_0: eight lanes share a
-// block's maximum by shuffles; K codes go out as words.  V interleaves four
-// positions per word, so the codes of the CTA's rows meet in shared memory and
-// leave as 16-byte stores wherever four consecutive rows are four aligned
-// positions of one slot, and as single bytes elsewhere (a decode step's rows,
-// the ends of a run): byte stores never touch a neighbouring position.
+// blockIdx.y.  The rows' cells are looked up once, one row a thread; then a lane
+// owns eight consecutive columns, and a warp has kBatch rows' loads under way
+// before it encodes the first (the lookups and loads, not the arithmetic, are what
+// a row waits for).  Q8_0: four lanes share a block's maximum by shuffles (as
+// integers: a NaN or a value past the limit shows there and takes the block to the
+// slow form).  V interleaves four positions per word, so the codes of the
+// CTA's rows meet in shared memory and leave as 16-byte stores wherever four
+// consecutive rows are four aligned positions of one slot, and as single bytes
+// elsewhere (a decode step's rows, the ends of a run): byte stores never touch a
+// neighbouring position.
+constexpr int kBatch = 2;
+
 template <int HD, int DT>
 __global__ void __launch_bounds__(32 * kStoreWarps)
     kv_store_kernel(const __grid_constant__ KvStoreArgs a, int rows, bool vec) {
-  constexpr int LPR = HD / 4, RPW = 32 / LPR;  // lanes a row, rows a warp
-  __shared__ uint32_t codes[kStoreRows][LPR];
+  constexpr int LPR = HD / 8, RPW = 32 / LPR;  // lanes a row, rows a warp
+  __shared__ uint2 codes[kStoreRows][LPR];
   __shared__ int row_page[kStoreRows], row_seq[kStoreRows], row_pos[kStoreRows];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int head = blockIdx.y;
   const bool is_v = blockIdx.z != 0;
   const long long i0 = (long long)blockIdx.x * rows;
   const int cnt = (int)min((long long)rows, a.n - i0);
-  const float* src = is_v ? a.v : a.k;
+  const float* src = (is_v ? a.v : a.k) + (size_t)i0 * a.ld + (size_t)head * HD;
   uint8_t* pool = is_v ? a.c.v : a.c.k;
   constexpr size_t TILE = kv_tile_bytes(DT, HD);
-  const int col = (lane % LPR) * 4;
-  for (int r0 = warp * RPW; r0 < cnt; r0 += kStoreWarps * RPW) {
-    const int r = r0 + lane / LPR;
-    const bool live = r < cnt;
-    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    int page = -1, pos = 0, seq = 0;
-    if (live) {
-      pos = a.pos[i0 + r];
-      seq = a.seq[i0 + r];
-      const float4 f = load4(src + (size_t)(i0 + r) * a.ld + (size_t)head * HD + col, vec);
-      x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
-      page = kv_page(a.c, seq, pos);
+  const int ln = lane % LPR, col = ln * 8;
+  constexpr int kStep = kStoreWarps * RPW;  // rows that the warps take at once
+  float4 f[kBatch][2];
+  auto load = [&](int r0) {
+#pragma unroll
+    for (int b = 0; b < kBatch; b++) {
+      const int r = r0 + b * kStep;
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+        f[b][h] = r < cnt ? load4(src + (size_t)r * a.ld + col + h * 4, vec) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
-    const int pr = pos & (kPageSize - 1);
-    uint8_t* tile = pool + ((size_t)max(page, 0) * a.c.heads + head) * TILE;
-    if constexpr (DT == LRS_KV_F32) {
-      if (page >= 0)
-        *reinterpret_cast<float4*>(tile + ((size_t)pr * HD + col) * 4) =
-            make_float4(x[0], x[1], x[2], x[3]);
-    } else if constexpr (DT == LRS_KV_BF16) {
-      if (page >= 0) {
-        const __nv_bfloat162 lo = __floats2bfloat162_rn(x[0], x[1]), hi = __floats2bfloat162_rn(x[2], x[3]);
-        *reinterpret_cast<uint2*>(tile + ((size_t)pr * HD + col) * 2) =
-            make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-      }
-    } else {
-      float m = 0.0f;
+  };
+  const int mine = warp * RPW + lane / LPR;
+  load(mine);
+  if (threadIdx.x < cnt) {
+    const int seq = a.seq[i0 + threadIdx.x], pos = a.pos[i0 + threadIdx.x];
+    row_seq[threadIdx.x] = seq;
+    row_pos[threadIdx.x] = pos;
+    row_page[threadIdx.x] = kv_page(a.c, seq, pos);
+  }
+  __syncthreads();
+  for (int r0 = mine; r0 - mine < cnt; r0 += kBatch * kStep) {
+    if (r0 != mine) load(r0);
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        x[i] = x[i] != x[i] ? 0.0f : fminf(fmaxf(x[i], -kQ8Limit), kQ8Limit);
-        m = fmaxf(m, fabsf(x[i]));
-      }
-#pragma unroll
-      for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const float d = __fdiv_rn(m, 127.0f);
-      const float inv = d == 0.0f ? 0.0f : __fdiv_rn(1.0f, d);
-      uint32_t w = 0;
-#pragma unroll
-      for (int i = 0; i < 4; i++) w |= q8_code(x[i], inv) << (8 * i);
-      const int b = col / 32;
-      if (page >= 0) {
-        if ((lane & 7) == 0)
-          *reinterpret_cast<__half*>(tile + (is_v ? q8_v_scale(HD, pr, b) : q8_k_scale(HD, pr, b))) =
-              __float2half_rn(d);
-        if (!is_v) *reinterpret_cast<uint32_t*>(tile + q8_k_code(pr, col)) = w;
-      }
-      if (is_v && live) {
-        codes[r][lane % LPR] = w;
-        if (lane % LPR == 0) {
-          row_page[r] = page;
-          row_seq[r] = seq;
-          row_pos[r] = pos;
+    for (int bt = 0; bt < kBatch; bt++) {
+      const int r = r0 + bt * kStep;
+      const bool live = r < cnt;
+      const int page = live ? row_page[r] : -1, pr = live ? row_pos[r] & (kPageSize - 1) : 0;
+      float x[8] = {f[bt][0].x, f[bt][0].y, f[bt][0].z, f[bt][0].w, f[bt][1].x, f[bt][1].y, f[bt][1].z, f[bt][1].w};
+      uint8_t* tile = pool + ((size_t)max(page, 0) * a.c.heads + head) * TILE;
+      if constexpr (DT == LRS_KV_F32) {
+        if (page >= 0) {
+          float4* o = reinterpret_cast<float4*>(tile + ((size_t)pr * HD + col) * 4);
+          o[0] = f[bt][0];
+          o[1] = f[bt][1];
         }
+      } else if constexpr (DT == LRS_KV_BF16) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const __nv_bfloat162 p = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+          w[i] = *reinterpret_cast<const uint32_t*>(&p);
+        }
+        if (page >= 0)
+          *reinterpret_cast<uint4*>(tile + ((size_t)pr * HD + col) * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+      } else {
+        int mb = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) mb = max(mb, __float_as_int(x[i]) & 0x7fffffff);
+        mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, 1));
+        mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, 2));
+        float m = __int_as_float(mb);
+        // the block of ordinary values: none past the limit, 1 / d finite
+        const bool plain = mb <= __float_as_int(kQ8Limit) && (mb == 0 || m > 1e-30f);
+        if (!plain) {
+          float mx = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            x[i] = x[i] != x[i] ? 0.0f : fminf(fmaxf(x[i], -kQ8Limit), kQ8Limit);
+            mx = fmaxf(mx, fabsf(x[i]));
+          }
+          const uint32_t four = 0xfu << (lane & 28);  // the block's lanes are here together
+          mx = fmaxf(mx, __shfl_xor_sync(four, mx, 1));
+          m = fmaxf(mx, __shfl_xor_sync(four, mx, 2));
+        }
+        const float d = __fdiv_rn(m, 127.0f);
+        const float inv = d == 0.0f ? 0.0f : __fdiv_rn(1.0f, d);
+        uint32_t w[2];
+        if (!q8_codes(x, inv, w) || !plain) {
+          w[0] = w[1] = 0;
+#pragma unroll
+          for (int i = 0; i < 8; i++) w[i / 4] |= q8_code(x[i], inv) << (8 * (i % 4));
+        }
+        if (page >= 0) {
+          if ((lane & 3) == 0)
+            *reinterpret_cast<__half*>(tile + (is_v ? q8_v_scale(HD, pr, col / 32) : q8_k_scale(HD, pr, col / 32))) =
+                __float2half_rn(d);
+          if (!is_v) *reinterpret_cast<uint2*>(tile + q8_k_code(pr, col)) = make_uint2(w[0], w[1]);
+        }
+        if (is_v && live) codes[r][ln] = make_uint2(w[0], w[1]);
       }
     }
   }
   if constexpr (DT == LRS_KV_Q8_0) {
     if (!is_v) return;
     __syncthreads();
-    for (int r0 = warp * RPW; r0 < cnt; r0 += kStoreWarps * RPW) {
-      const int r = r0 + lane / LPR;
-      if (r >= cnt || row_page[r] < 0) continue;
+    for (int r = mine; r < cnt; r += kStep) {
+      if (row_page[r] < 0) continue;
       const int pos = row_pos[r], g = r - (pos & 3);  // first row of the aligned group
       bool full = g >= 0 && g + 3 < cnt;
       for (int i = 0; i < 4 && full; i++)
@@ -125,67 +180,108 @@ __global__ void __launch_bounds__(32 * kStoreWarps)
       if (full && g != r) continue;  // row g writes the group
       const int pr = pos & (kPageSize - 1);
       uint8_t* tile = pool + ((size_t)row_page[r] * a.c.heads + head) * TILE;
-      if (full) {
-        uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) w[i] = codes[g + i][lane % LPR];
-        const uint32_t a0 = __byte_perm(w[0], w[1], 0x5140), a1 = __byte_perm(w[2], w[3], 0x5140);
-        const uint32_t b0 = __byte_perm(w[0], w[1], 0x7362), b1 = __byte_perm(w[2], w[3], 0x7362);
-        *reinterpret_cast<uint4*>(tile + q8_v_code(HD, pr, col)) =
-            make_uint4(__byte_perm(a0, a1, 0x5410), __byte_perm(a0, a1, 0x7632),
-                       __byte_perm(b0, b1, 0x5410), __byte_perm(b0, b1, 0x7632));
-      } else {
-        const uint32_t w = codes[r][lane % LPR];
+      for (int h = 0; h < 2; h++) {  // four columns each
+        const int c4 = col + 4 * h;
+        if (full) {
+          uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) tile[q8_v_code(HD, pr, col + i)] = (uint8_t)(w >> (8 * i));
+          for (int i = 0; i < 4; i++) w[i] = h ? codes[g + i][ln].y : codes[g + i][ln].x;
+          const uint32_t a0 = __byte_perm(w[0], w[1], 0x5140), a1 = __byte_perm(w[2], w[3], 0x5140);
+          const uint32_t b0 = __byte_perm(w[0], w[1], 0x7362), b1 = __byte_perm(w[2], w[3], 0x7362);
+          *reinterpret_cast<uint4*>(tile + q8_v_code(HD, pr, c4)) =
+              make_uint4(__byte_perm(a0, a1, 0x5410), __byte_perm(a0, a1, 0x7632),
+                         __byte_perm(b0, b1, 0x5410), __byte_perm(b0, b1, 0x7632));
+        } else {
+          const uint32_t w = h ? codes[r][ln].y : codes[r][ln].x;
+#pragma unroll
+          for (int i = 0; i < 4; i++) tile[q8_v_code(HD, pr, c4 + i)] = (uint8_t)(w >> (8 * i));
+        }
       }
     }
   }
 }
 
-// The inverse: a lane owns four columns of a row; rows of a CTA are
-// consecutive, so the lines that four positions share (V codes, K's 16-byte
-// chunks) are read from L2 once.
+// The inverse.  A CTA has kLoadRows consecutive rows of K or V, all heads: the
+// rows' cells are looked up once; then a thread takes four columns of a (row, head)
+// at a time, kLoadBatch of them under way together, neighbouring threads writing
+// neighbouring heads of a row.  The lines that four positions share (V codes, K's
+// 16-byte chunks) come from L2 once.
+constexpr int kLoadRows = 32, kLoadThreads = 256, kLoadBatch = 4;
+
 template <int HD, int DT>
-__global__ void __launch_bounds__(128)
-    kv_load_kernel(const __grid_constant__ KvLoadArgs a, bool vec) {
-  constexpr int LPR = HD / 4, RPC = 128 / LPR;
-  const int head = blockIdx.y;
-  const bool is_v = blockIdx.z != 0;
+__global__ void __launch_bounds__(kLoadThreads)
+    kv_load_kernel(const __grid_constant__ KvLoadArgs a, int rows, bool vec) {
+  constexpr int LPR = HD / 4, kStep = kLoadThreads / LPR;  // (row, head) pairs at once
+  __shared__ int row_page[kLoadRows], row_in[kLoadRows];
+  const bool is_v = blockIdx.y != 0;
   float* dst = is_v ? a.v : a.k;
-  const long long i = (long long)blockIdx.x * RPC + threadIdx.x / LPR;
-  if (!dst || i >= a.n) return;
-  const int col = (threadIdx.x % LPR) * 4;
-  const int pos = a.pos[i], page = kv_page(a.c, a.seq[i], pos);
-  if (page < 0) return;
-  const int pr = pos & (kPageSize - 1);
-  const uint8_t* tile =
-      (is_v ? a.c.v : a.c.k) + ((size_t)page * a.c.heads + head) * kv_tile_bytes(DT, HD);
-  float x[4];
-  if constexpr (DT == LRS_KV_F32) {
-    const float4 f = *reinterpret_cast<const float4*>(tile + ((size_t)pr * HD + col) * 4);
-    x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
-  } else if constexpr (DT == LRS_KV_BF16) {
-    const uint2 u = *reinterpret_cast<const uint2*>(tile + ((size_t)pr * HD + col) * 2);
-    x[0] = __uint_as_float(u.x << 16), x[1] = __uint_as_float(u.x & 0xffff0000u);
-    x[2] = __uint_as_float(u.y << 16), x[3] = __uint_as_float(u.y & 0xffff0000u);
-  } else if (is_v) {
-    const uint4 u = *reinterpret_cast<const uint4*>(tile + q8_v_code(HD, pr & ~3, col));
-    const float d = __half2float(*reinterpret_cast<const __half*>(tile + q8_v_scale(HD, pr, col / 32)));
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int j = 0; j < 4; j++) x[j] = __fmul_rn(d, (float)(int8_t)(w[j] >> (8 * (pr & 3))));
-  } else {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(tile + q8_k_code(pr, col));
-    const float d = __half2float(*reinterpret_cast<const __half*>(tile + q8_k_scale(HD, pr, col / 32)));
-#pragma unroll
-    for (int j = 0; j < 4; j++) x[j] = __fmul_rn(d, (float)(int8_t)(w >> (8 * j)));
+  const long long i0 = (long long)blockIdx.x * rows;
+  const int cnt = (int)min((long long)rows, a.n - i0);
+  if (!dst) return;
+  if (threadIdx.x < cnt) {
+    const int pos = a.pos[i0 + threadIdx.x];
+    row_page[threadIdx.x] = kv_page(a.c, a.seq[i0 + threadIdx.x], pos);
+    row_in[threadIdx.x] = pos & (kPageSize - 1);
   }
-  float* o = dst + (size_t)i * a.ld + (size_t)head * HD + col;
-  if (vec)
-    *reinterpret_cast<float4*>(o) = make_float4(x[0], x[1], x[2], x[3]);
-  else
-    for (int j = 0; j < 4; j++) o[j] = x[j];
+  __syncthreads();
+  constexpr size_t TILE = kv_tile_bytes(DT, HD);
+  const uint8_t* pool = is_v ? a.c.v : a.c.k;
+  const int heads = a.c.heads, col = (threadIdx.x % LPR) * 4;
+  int row = threadIdx.x / LPR / heads, head = threadIdx.x / LPR % heads;
+  while (row < cnt) {
+    uint4 raw[kLoadBatch];
+    __half d[kLoadBatch];
+    int in[kLoadBatch];
+    float* out[kLoadBatch];  // null: no such row
+#pragma unroll
+    for (int b = 0; b < kLoadBatch; b++) {
+      out[b] = nullptr;
+      if (row < cnt && row_page[row] >= 0) {
+        const int pr = row_in[row];
+        const uint8_t* t = pool + ((size_t)row_page[row] * heads + head) * TILE;
+        in[b] = pr;
+        out[b] = dst + (size_t)(i0 + row) * a.ld + (size_t)head * HD + col;
+        if constexpr (DT == LRS_KV_F32) {
+          raw[b] = *reinterpret_cast<const uint4*>(t + ((size_t)pr * HD + col) * 4);
+        } else if constexpr (DT == LRS_KV_BF16) {
+          const uint2 u = *reinterpret_cast<const uint2*>(t + ((size_t)pr * HD + col) * 2);
+          raw[b] = make_uint4(u.x << 16, u.x & 0xffff0000u, u.y << 16, u.y & 0xffff0000u);
+        } else if (is_v) {
+          raw[b] = *reinterpret_cast<const uint4*>(t + q8_v_code(HD, pr & ~3, col));
+          d[b] = *reinterpret_cast<const __half*>(t + q8_v_scale(HD, pr, col / 32));
+        } else {
+          raw[b].x = *reinterpret_cast<const uint32_t*>(t + q8_k_code(pr, col));
+          d[b] = *reinterpret_cast<const __half*>(t + q8_k_scale(HD, pr, col / 32));
+        }
+      }
+      for (head += kStep; head >= heads; head -= heads) row++;
+    }
+#pragma unroll
+    for (int b = 0; b < kLoadBatch; b++) {
+      if (!out[b]) continue;
+      uint4 v = raw[b];
+      if constexpr (DT == LRS_KV_Q8_0) {
+        const float f = __half2float(d[b]);
+        // K: the four bytes of a word; V: byte (position % 4) of four words
+        uint32_t w = v.x;
+        if (is_v) {
+          const uint32_t at = in[b] & 3, sel = at | (at + 4) << 4;
+          w = __byte_perm(__byte_perm(v.x, v.y, sel), __byte_perm(v.z, v.w, sel), 0x5410);
+        }
+        v = make_uint4(__float_as_uint(__fmul_rn(f, (float)(int8_t)w)),
+                       __float_as_uint(__fmul_rn(f, (float)(int8_t)(w >> 8))),
+                       __float_as_uint(__fmul_rn(f, (float)(int8_t)(w >> 16))),
+                       __float_as_uint(__fmul_rn(f, (float)(int8_t)(w >> 24))));
+      }
+      if (vec) {
+        __stcs(reinterpret_cast<uint4*>(out[b]), v);
+      } else {
+        out[b][0] = __uint_as_float(v.x), out[b][1] = __uint_as_float(v.y);
+        out[b][2] = __uint_as_float(v.z), out[b][3] = __uint_as_float(v.w);
+      }
+    }
+  }
 }
 
 // ---- accept ---------------------------------------------------------------
@@ -363,12 +459,14 @@ cudaError_t launch_kv_store(const KvStoreArgs& a, uint32_t dtype, int hd, int sm
   return cudaGetLastError();
 }
 
-cudaError_t launch_kv_load(const KvLoadArgs& a, uint32_t dtype, int hd, cudaStream_t st) {
-  const int rpc = 512 / hd;
+cudaError_t launch_kv_load(const KvLoadArgs& a, uint32_t dtype, int hd, int sms, cudaStream_t st) {
+  // few rows: fewer a CTA, so that they spread over the SMs
+  const long long big = (a.n + kLoadRows - 1) / kLoadRows * 2;
+  const int rows = big >= 4ll * sms ? kLoadRows : 4;
   const bool vec = a.ld % 4 == 0 && reinterpret_cast<uintptr_t>(a.k) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(a.v) % 16 == 0;
-  const dim3 grid((unsigned)((a.n + rpc - 1) / rpc), a.c.heads, 2);
-#define LRS_CALL(HD, DT) kv_load_kernel<HD, DT><<<grid, 128, 0, st>>>(a, vec)
+  const dim3 grid((unsigned)((a.n + rows - 1) / rows), 2);
+#define LRS_CALL(HD, DT) kv_load_kernel<HD, DT><<<grid, kLoadThreads, 0, st>>>(a, rows, vec)
   LRS_KV_DISPATCH(hd, dtype, LRS_CALL);
 #undef LRS_CALL
   return cudaGetLastError();
@@ -513,7 +611,7 @@ lrs_status lrs_kv_load(lrs_backend* be, const lrs_kv_cache* c, const int32_t* d_
   OnDevice on(be->device);
   if (on.err != cudaSuccess) return cuda_status(on.err, "cudaSetDevice");
   KvLoadArgs a{view_of(*c, be->d_err), d_seq, d_pos, (long long)n, d_k, d_v, (long long)ld};
-  return cuda_status(launch_kv_load(a, c->kv_dtype, (int)c->head_dim,
+  return cuda_status(launch_kv_load(a, c->kv_dtype, (int)c->head_dim, be->sms,
                                     stream ? (cudaStream_t)stream : be->stream),
                      "lrs_kv_load");
 } catch (...) {

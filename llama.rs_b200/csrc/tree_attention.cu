@@ -213,31 +213,6 @@ __device__ __forceinline__ void ta_ld16(uint32_t taddr, float* v) {
 #pragma unroll
   for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
 }
-// Two f32 operations in one instruction.
-__device__ __forceinline__ float2 ta_fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
-      " fma.rn.f32x2 w, x, y, z;\n mov.b64 {%0, %1}, w;\n}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
-__device__ __forceinline__ float2 ta_mul2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n .reg .b64 x, y, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n"
-      " mul.rn.f32x2 w, x, y;\n mov.b64 {%0, %1}, w;\n}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-__device__ __forceinline__ float2 ta_add2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n .reg .b64 x, y, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n"
-      " add.rn.f32x2 w, x, y;\n mov.b64 {%0, %1}, w;\n}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
 // The loaded registers may be used after this: it names them, so that no use moves above it.
 template <int N>
 __device__ __forceinline__ void ta_wait_ld(float (&v)[N]) {
@@ -341,12 +316,12 @@ __device__ __forceinline__ void ta_split(float2 v, uint32_t (&t)[TERMS]) {
     if constexpr (F16) {
       const __half2 h = __floats2half2_rn(v.x, v.y);
       t[i] = *reinterpret_cast<const uint32_t*>(&h);
-      if (i + 1 < TERMS) v = ta_add2(v, make_float2(-__low2float(h), -__high2float(h)));
+      if (i + 1 < TERMS) v = add2(v, make_float2(-__low2float(h), -__high2float(h)));
     } else {
       const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
       t[i] = *reinterpret_cast<const uint32_t*>(&h);
       if (i + 1 < TERMS)
-        v = ta_add2(v, make_float2(-__uint_as_float(t[i] << 16), -__uint_as_float(t[i] & 0xffff0000u)));
+        v = add2(v, make_float2(-__uint_as_float(t[i] << 16), -__uint_as_float(t[i] & 0xffff0000u)));
     }
   }
 }
@@ -583,11 +558,11 @@ __device__ __forceinline__ void ta_exponents(float (&s)[16], const float* c, con
     float2 x = make_float2(s[r], s[r + 1]), y = make_float2(s[r + 2], s[r + 3]);
     if constexpr (SCALED) {
       const float4 cc = *reinterpret_cast<const float4*>(c + r);
-      x = ta_fma2(x, make_float2(cc.x, cc.y), make_float2(mm.x, mm.y));
-      y = ta_fma2(y, make_float2(cc.z, cc.w), make_float2(mm.z, mm.w));
+      x = fma2(x, make_float2(cc.x, cc.y), make_float2(mm.x, mm.y));
+      y = fma2(y, make_float2(cc.z, cc.w), make_float2(mm.z, mm.w));
     } else {
-      x = ta_add2(x, make_float2(mm.x, mm.y));
-      y = ta_add2(y, make_float2(mm.z, mm.w));
+      x = add2(x, make_float2(mm.x, mm.y));
+      y = add2(y, make_float2(mm.z, mm.w));
     }
     s[r] = x.x, s[r + 1] = x.y, s[r + 2] = y.x, s[r + 3] = y.y;
   }
@@ -658,8 +633,8 @@ __device__ __forceinline__ void load_q(const TreeArgs& a, const TaUnit& it, uint
       uint32_t y[S::kB][4];
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        float2 v = ta_mul2(make_float2(x[j][2 * e], x[j][2 * e + 1]), make_float2(f0, f0));
-        if constexpr (S::kF16) v = ta_mul2(v, make_float2(f1, f1));
+        float2 v = mul2(make_float2(x[j][2 * e], x[j][2 * e + 1]), make_float2(f0, f0));
+        if constexpr (S::kF16) v = mul2(v, make_float2(f1, f1));
         uint32_t z[S::kB];
         ta_split<S::kF16, S::kB>(v, z);
 #pragma unroll
@@ -989,7 +964,7 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
 #pragma unroll
           for (int r = 0; r < 16; r += 2) {
             const float2 g = *reinterpret_cast<const float2*>(f + r);
-            const float2 d = ta_add2(make_float2(s[r], s[r + 1]), *reinterpret_cast<const float2*>(&sh.red[grp][0][r]));
+            const float2 d = add2(make_float2(s[r], s[r + 1]), *reinterpret_cast<const float2*>(&sh.red[grp][0][r]));
             s[r] = d.x, s[r + 1] = d.y;
             l[r / 2].x *= g.x, l[r / 2].y *= g.y;
           }
@@ -1012,7 +987,7 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
             for (int e = 0; e < 4; e++) {
               const int r = k * 8 + e * 2;
               const float2 x = make_float2(ta_exp2(s[r]), ta_exp2(s[r + 1]));
-              l[r / 2] = ta_add2(l[r / 2], x);
+              l[r / 2] = add2(l[r / 2], x);
               uint32_t z[S::kB];
               ta_split<kF16, S::kB>(x, z);
 #pragma unroll
@@ -1090,7 +1065,7 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
           ta_wait_ld(x);
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
-            const float2 y = ta_add2(make_float2(o[c * 16 + i], o[c * 16 + i + 1]), make_float2(x[i], x[i + 1]));
+            const float2 y = add2(make_float2(o[c * 16 + i], o[c * 16 + i + 1]), make_float2(x[i], x[i + 1]));
             o[c * 16 + i] = y.x, o[c * 16 + i + 1] = y.y;
           }
         }

@@ -123,6 +123,29 @@ def test_store_then_load(lrs, backend, dtype, hd, heads, n, slots, width, kind):
         assert np.array_equal(out[i].cpu().numpy(), kv_plain.held(lrs, cache.dtype, x).astype(np.float32))
 
 
+def test_store_rounds_ties_as_the_host_encoder(lrs, backend):
+    """Products that are exact ties, of either sign, and their neighbours."""
+    rng = np.random.default_rng(2)
+    n, heads, hd = 40, 2, 64
+    x = (rng.integers(-126, 127, (2, n, heads, hd)) + rng.choice([0.5, -0.5, 0.0, 0.49999997], (2, n, heads, hd)))
+    x = np.clip(x, -127, 127)
+    x[..., ::32] = 127.0                                 # d = 1
+    x *= 2.0 ** rng.integers(-90, 8, (2, n, 1, 1))       # exact powers of two keep the ties
+    x = x.astype(np.float32)
+    cache = Cache(lrs, "Q8_0", heads, hd, [0])
+    d_seq, d_pos, dk, dv = dev(np.zeros(n, np.int32)), dev(np.arange(n) + 3, np.int32), dev(x[0]), dev(x[1])
+    backend.kv_store(cache.c, d_seq.data_ptr(), d_pos.data_ptr(), n, dk.data_ptr(), dv.data_ptr(), stream=LEGACY)
+    sync_ok(backend)
+    pos = np.arange(n) + 3
+    for i in range(2):
+        full = np.zeros(cache.rows[0].shape, np.float32)
+        full[cache.pages[0, 0], :, pos] = x[i]
+        written = np.zeros(full.shape[:3], bool)
+        written[cache.pages[0, 0], :, pos] = True
+        want = np.where(cache.marks(written, bool(i)), kv_plain.pack(lrs, cache.dtype, full, bool(i)), cache.tiles[i])
+        assert np.array_equal(cache.bytes_now()[i], want)
+
+
 def test_store_clamps_what_q8_0_cannot_hold(lrs, backend):
     import torch
     cache = Cache(lrs, "Q8_0", 1, 64, [0])
