@@ -318,8 +318,8 @@ lrs_status lrs_kv_check(const lrs_kv_cache* cache, size_t* tile_bytes);
 /* KVCache::update (src/cache.rs:38-53) for n rows, in the cache's type: row i of
  * d_k and d_v (kv_heads * head_dim floats each, rows `ld` floats apart, 0 =
  * packed; K already rotated) becomes position d_pos[i] of slot d_seq[i].  The
- * positions of one call are distinct: which of two rows for one position
- * stays is not defined. */
+ * positions of one call are distinct: what a position that two rows name (in
+ * one slot, or through a page that two slots share) holds then is not defined. */
 lrs_status lrs_kv_store(lrs_backend* backend, const lrs_kv_cache* cache, const int32_t* d_seq,
                         const int32_t* d_pos, size_t n, const float* d_k, const float* d_v,
                         size_t ld, void* stream);
@@ -357,7 +357,10 @@ typedef struct lrs_tree_batch {
  * non-finite (all of the row's, if the value belongs to another node).
  * `d_workspace` (16-byte aligned, lrs_tree_attention_workspace bytes, contents
  * free) is in use until the work has finished: calls that may overlap, and
- * graphs that may run at once, need one each. */
+ * graphs that may run at once, need one each.  out may be q (then q_ld =
+ * out_ld).  A tree whose slot, node range or length is out of range is skipped,
+ * its rows left as they were; the rows of one that reaches a page out of range
+ * hold no defined values. */
 lrs_status lrs_tree_attention_workspace(const lrs_backend* backend, const lrs_kv_cache* cache,
                                         const lrs_tree_batch* trees, uint32_t n_heads,
                                         size_t* bytes);
@@ -397,7 +400,8 @@ lrs_status lrs_model_accept_tree(lrs_model* model, uint32_t seq, uint32_t start_
  * n_caches caches (the layers of a model: equal but for their pools).  A path's
  * nodes ascend, all below LRS_TREE_MAX_NODES; a tree whose path does not, or
  * leaves the slot's pages, is left as it was.  d_start is [n_trees + 1],
- * ascending from 0 to at most n_nodes; the slots of one call are distinct. */
+ * ascending from 0 to at most n_nodes; the slots of one call are distinct and
+ * share no page that they write, and no pool is named twice. */
 lrs_status lrs_kv_accept(lrs_backend* backend, const lrs_kv_cache* caches, size_t n_caches,
                          const int32_t* d_seq, const int32_t* d_ctx, const int32_t* d_start,
                          const int32_t* d_nodes, size_t n_trees, size_t n_nodes, void* stream);

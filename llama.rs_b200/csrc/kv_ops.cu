@@ -313,11 +313,13 @@ __global__ void __launch_bounds__(128) kv_accept_kernel(const __grid_constant__ 
   item /= a.c.heads;
   const int cache = (int)(item % a.n_caches), t = (int)(item / a.n_caches);
   if (t >= a.n_trees) return;
-  const int s = a.start[t], n = a.start[t + 1] - s, ctx = a.ctx[t], seq = a.seq[t];
-  if (n == 0) return;
-  bool ok = s >= 0 && n > 0 && n <= LRS_TREE_MAX_NODES && s + n <= a.n_nodes && seq >= 0 &&
+  const int s = a.start[t], end = a.start[t + 1], ctx = a.ctx[t], seq = a.seq[t];
+  if (s == end) return;
+  // (compared, not subtracted: the difference of two arbitrary values may overflow)
+  bool ok = s >= 0 && end > s && end <= a.n_nodes && end - s <= LRS_TREE_MAX_NODES && seq >= 0 &&
             seq < a.c.n_seqs && ctx >= 0 &&
             ctx <= (int)min((long long)a.c.max_pages * kPageSize, (long long)INT_MAX) - 1;
+  const int n = ok ? end - s : 0;
   int node0 = -1, node1 = -1;  // of rows `lane` and `lane + 32`
   if (ok) {
     if (lane < n) node0 = a.nodes[s + lane];
@@ -508,6 +510,15 @@ KvView view_of(const lrs_kv_cache& c, int* err) {
                 (int)c.n_pages, (int)c.n_seqs, (int)c.max_pages, (int)c.kv_heads, err};
 }
 
+// A device array of T, or null.
+template <typename T>
+bool aligned(const T* p) {
+  return reinterpret_cast<uintptr_t>(p) % sizeof(T) == 0;
+}
+int32_t unaligned(const char* what) {
+  return fail(LRS_ERR_INVALID, std::string(what) + ": an array is not aligned to its values");
+}
+
 int32_t check_rows(const lrs_kv_cache* c, size_t n, size_t* ld, const char* what) {
   int32_t rc = lrs_kv_check(c, nullptr);
   if (rc) return rc;
@@ -532,13 +543,15 @@ int32_t check_trees(const lrs_kv_cache* c, const lrs_tree_batch* t, uint32_t n_h
   if (!t->seq || !t->ctx || !t->start) return fail(LRS_ERR_INVALID, "null tree array");
   if (t->max_nodes == 0 || t->max_nodes > LRS_TREE_MAX_NODES)
     return fail(LRS_ERR_INVALID, "max_nodes must be in 1..=" + std::to_string(LRS_TREE_MAX_NODES));
+  if (!aligned(t->seq) || !aligned(t->ctx) || !aligned(t->start) || !aligned(t->mask)) return unaligned("tree batch");
   if (t->max_len == 0 || t->max_len > (uint64_t)c->max_pages * LRS_KV_PAGE)
     return fail(LRS_ERR_INVALID, "max_len " + std::to_string(t->max_len) +
                                      " is outside the slots' " + std::to_string(c->max_pages) + " pages");
-  // the kernels number the batch's tiles (128 positions by 16 rows at least) in int32
+  // the kernels number the batch's tiles (128 positions by 16 rows at least) and
+  // the positions of whole tiles in int32
   const uint64_t rows = ((uint64_t)t->max_nodes * (n_heads / c->kv_heads) + 15) / 16,
                  tiles = ((uint64_t)t->max_len + 127) / 128;
-  if (t->n_trees > 65535u || t->n_nodes > (1u << 24) ||
+  if (t->n_trees > 65535u || t->n_nodes > (1u << 24) || t->max_len > (uint32_t)INT_MAX - 128u ||
       rows * tiles > (uint64_t)INT_MAX / ((uint64_t)t->n_trees * c->kv_heads))
     return fail(LRS_ERR_UNSUPPORTED, "too many trees, nodes or positions");
   return LRS_OK;
@@ -578,6 +591,7 @@ lrs_status lrs_kv_check(const lrs_kv_cache* c, size_t* tile_bytes) try {
   if (!c->k_pool || !c->v_pool || !c->pages) return fail(LRS_ERR_INVALID, "KV cache: null pool or page table");
   if (reinterpret_cast<uintptr_t>(c->k_pool) % 16 || reinterpret_cast<uintptr_t>(c->v_pool) % 16)
     return fail(LRS_ERR_INVALID, "KV cache: pools must be 16-byte aligned");
+  if (!aligned(c->pages)) return unaligned("KV cache");
   if (tile_bytes) *tile_bytes = kv_tile_bytes(c->kv_dtype, (int)c->head_dim);
   return LRS_OK;
 } catch (...) {
@@ -591,6 +605,7 @@ lrs_status lrs_kv_store(lrs_backend* be, const lrs_kv_cache* c, const int32_t* d
   if (rc) return rc;
   if (n == 0) return LRS_OK;
   if (!be || !d_seq || !d_pos || !d_k || !d_v) return fail(LRS_ERR_INVALID, "null argument");
+  if (!aligned(d_seq) || !aligned(d_pos) || !aligned(d_k) || !aligned(d_v)) return unaligned("lrs_kv_store");
   OnDevice on(be->device);
   if (on.err != cudaSuccess) return cuda_status(on.err, "cudaSetDevice");
   KvStoreArgs a{view_of(*c, be->d_err), d_seq, d_pos, (long long)n, d_k, d_v, (long long)ld};
@@ -608,6 +623,7 @@ lrs_status lrs_kv_load(lrs_backend* be, const lrs_kv_cache* c, const int32_t* d_
   if (rc) return rc;
   if (n == 0 || (!d_k && !d_v)) return LRS_OK;
   if (!be || !d_seq || !d_pos) return fail(LRS_ERR_INVALID, "null argument");
+  if (!aligned(d_seq) || !aligned(d_pos) || !aligned(d_k) || !aligned(d_v)) return unaligned("lrs_kv_load");
   OnDevice on(be->device);
   if (on.err != cudaSuccess) return cuda_status(on.err, "cudaSetDevice");
   KvLoadArgs a{view_of(*c, be->d_err), d_seq, d_pos, (long long)n, d_k, d_v, (long long)ld};
@@ -634,7 +650,14 @@ lrs_status lrs_kv_accept(lrs_backend* be, const lrs_kv_cache* caches, size_t n_c
   if (n_trees > (size_t)INT_MAX || n_nodes > (size_t)INT_MAX)
     return fail(LRS_ERR_INVALID, "lrs_kv_accept: too many trees or nodes");
   if (n_caches == 0 || n_trees == 0 || n_nodes == 0) return LRS_OK;
+  // a pool named twice would be compacted by two warps at once
+  for (size_t i = 0; i < n_caches; i++)
+    for (size_t j = 0; j <= i; j++)
+      if ((j < i && (caches[i].k_pool == caches[j].k_pool || caches[i].v_pool == caches[j].v_pool)) ||
+          caches[i].k_pool == caches[j].v_pool || caches[i].v_pool == caches[j].k_pool)
+        return fail(LRS_ERR_INVALID, "lrs_kv_accept: a pool is named twice");
   if (!be || !d_seq || !d_ctx || !d_start || !d_nodes) return fail(LRS_ERR_INVALID, "null argument");
+  if (!aligned(d_seq) || !aligned(d_ctx) || !aligned(d_start) || !aligned(d_nodes)) return unaligned("lrs_kv_accept");
   const size_t per_cache = n_trees * caches[0].kv_heads * 2;
   if (per_cache > (size_t)INT_MAX) return fail(LRS_ERR_INVALID, "lrs_kv_accept: too many trees or nodes");
   OnDevice on(be->device);
@@ -693,6 +716,7 @@ lrs_status lrs_tree_attention(lrs_backend* be, const lrs_kv_cache* c, const lrs_
   if (!std::isfinite(scale)) return fail(LRS_ERR_INVALID, "lrs_tree_attention: scale must be finite");
   if (t->n_trees == 0 || t->n_nodes == 0) return LRS_OK;
   if (!be || !d_q || !d_out) return fail(LRS_ERR_INVALID, "null argument");
+  if (!aligned(d_q) || !aligned(d_out)) return unaligned("lrs_tree_attention");
   TreeArgs a = tree_args(*c, *t, n_heads, be->d_err);
   const size_t need = tree_attention_workspace_bytes(a, (int)c->head_dim, be->sms);
   if (workspace_bytes < need || (need && !d_workspace))

@@ -287,13 +287,14 @@ __device__ __forceinline__ bool ta_try_many(uint32_t bar, uint32_t parity) {
   return done != 0;
 }
 constexpr uint32_t kPolls = 1u << 20;
-// A wait that gives up after a bounded number of polls, or when another role did.
+// A whole warp's wait, which gives up after a bounded number of polls, or when
+// another role did: its lanes go on together either way.
 __device__ __forceinline__ bool ta_wait(TaShared& sh, uint64_t* bar, uint32_t parity) {
   const uint32_t at = smem_u32(bar);
 #pragma unroll 1
   for (uint32_t i = 0; i < kPolls / 2048; i++) {
-    if (ta_try_many(at, parity)) return true;
-    if (*reinterpret_cast<volatile int*>(&sh.abort)) return false;
+    if (__all_sync(0xffffffffu, ta_try_many(at, parity))) return true;
+    if (__any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&sh.abort))) return false;
   }
   *reinterpret_cast<volatile int*>(&sh.abort) = 1;
   return false;
@@ -347,15 +348,16 @@ struct TaTree {
   int s, n, ctx, len, seq, chunks, tiles;  // chunks of rows, tiles of a chunk
   __device__ __forceinline__ bool load(const TreeArgs& a, int t, int nr) {
     s = a.start[t];
-    n = a.start[t + 1] - s;
+    const int end = a.start[t + 1];  // (compared with s first: the difference may overflow)
     ctx = a.ctx[t];
     seq = a.seq[t];
-    chunks = tiles = 0;
-    if (s < 0 || n < 0 || (long long)s + n > a.n_nodes || n > a.max_nodes || ctx < 0 ||
-        (long long)ctx + n > a.max_len || seq < 0 || seq >= a.c.n_seqs) {
+    chunks = tiles = n = 0;
+    if (s < 0 || end < s || end > a.n_nodes || end - s > a.max_nodes || ctx < 0 || ctx > a.max_len ||
+        end - s > a.max_len - ctx || seq < 0 || seq >= a.c.n_seqs) {
       atomicExch(a.c.err, kErrCacheIndex);
       return false;
     }
+    n = end - s;
     len = ctx + n;
     if (n == 0) return true;
     chunks = (n * a.group + nr - 1) / nr;
@@ -1217,7 +1219,7 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
       for (int half = 0; half < 2; half++) {
         bool good = ta_wait(sh, &sh.ak_full[half], qk & 1);
         if (half == 0 && good && qk > 0) good = ta_wait(sh, &sh.s_empty, (qk - 1) & 1);
-        if (!__all_sync(0xffffffffu, good)) return false;
+        if (!good) return false;
         ta_fence_after();
 #pragma unroll
         for (int i = 0; i < S::kProducts; i++) {
@@ -1247,7 +1249,6 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
         vbuf.step();
         pbuf.step();
         if (ok && tile > 0) ok = ta_wait(sh, &sh.o_empty, (tile - 1) & 1);
-        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         ta_fence_after();
         const uint32_t d = tmem + S::kTmO, idesc = ta_idesc(kF16, true, steps * 16), av = tmem + S::kTmV + vb * S::kVCols;

@@ -709,6 +709,43 @@ def test_bad_paths_are_skipped(lrs, backend, dtype):
         assert np.array_equal(got, want)
 
 
+def test_starts_at_the_ends_of_int32_are_skipped(lrs, backend):
+    """Node ranges whose ends' difference passes 32 bits: no tree, nothing read."""
+    import torch
+    cache = Cache(lrs, "BF16", 2, 64, [100, 100])
+    top, low = 2 ** 31 - 1, -2 ** 31
+    for start in ([top - 10, low + 20], [0, top], [low, low + 8], [top, top - 3], [-5, 3], [3, 99]):
+        d = [dev([0], np.int32), dev([20], np.int32), dev(start, np.int32), dev([0, 1, 2, 3, 4, 5, 6, 8], np.int32)]
+        backend.kv_accept(cache.c, *(x.data_ptr() for x in d), 1, 8, stream=LEGACY)
+        torch.cuda.synchronize()
+        with pytest.raises(lrs.LrsError, match="out of range"):
+            backend.synchronize()
+        for got, want in zip(cache.bytes_now(), cache.tiles):
+            assert np.array_equal(got, want)
+        trees = Trees(lrs, backend, cache, [(20, 5), (30, 3)], 3, max_nodes=64, max_len=100)
+        trees.d["start"].copy_(dev(start + [start[1]], np.int32))
+        trees.run(backend)
+        torch.cuda.synchronize()
+        with pytest.raises(lrs.LrsError, match="out of range"):
+            backend.synchronize()
+        assert bool((trees.out == -5.0).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_out_may_be_q(lrs, backend, dtype):
+    s = [(700, 9), (5, 2), (0, 1), (1500, 20)]
+    cache = Cache(lrs, dtype, 2, 128, [c + n for c, n in reversed(s)])
+    trees = Trees(lrs, backend, cache, s, 7)
+    trees.run(backend)
+    sync_ok(backend)
+    want = trees.out.clone()
+    trees.out = trees.d["q"]
+    trees.run(backend)
+    sync_ok(backend)
+    rows = trees.n * trees.out_ld
+    assert bool((trees.out[:rows] == want[:rows]).all())
+
+
 def test_accept_in_more_caches_than_a_launch(lrs, backend):
     base = Cache(lrs, "BF16", 1, 64, [30])
     pools = [[p.clone() for p in base.pool] for _ in range(150)]

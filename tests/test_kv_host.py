@@ -118,6 +118,49 @@ def test_accept_wants_equal_caches(lrs):
             be.kv_accept([_cache(lrs), _cache(lrs, **other)], A, A, A, A, 1, 1)
 
 
+def test_accept_wants_distinct_pools(lrs):
+    be = _Host(lrs)
+    apart = [_cache(lrs, k_pool=A * (2 * i + 2), v_pool=A * (2 * i + 3)) for i in range(3)]
+    for bad in (dict(k_pool=apart[0].k_pool), dict(v_pool=apart[1].v_pool),
+                             dict(k_pool=apart[0].v_pool), dict(v_pool=apart[1].k_pool)):
+        last = _cache(lrs, **{**dict(k_pool=50 * A, v_pool=51 * A), **bad})
+        with pytest.raises(lrs.LrsError, match="named twice") as e:
+            be.kv_accept(apart + [last], A, A, A, A, 1, 1)
+        assert e.value.code == INVALID
+    with pytest.raises(lrs.LrsError, match="named twice"):  # one cache's two pools
+        be.kv_accept([_cache(lrs)], A, A, A, A, 1, 1)
+
+
+def test_unaligned_arrays_are_refused(lrs):
+    be, B = _Host(lrs), A + 2
+    c = _cache(lrs, v_pool=2 * A)
+    calls = [lambda i=i: be.kv_store(c, *(B if j == i else A for j in range(2)), 1,
+                                     *(B if j == i else A for j in (2, 3))) for i in range(4)]
+    calls += [lambda i=i: be.kv_load(c, *(B if j == i else A for j in range(2)), 1,
+                                     *(B if j == i else A for j in (2, 3))) for i in range(4)]
+    calls += [lambda i=i: be.kv_accept([c], *(B if j == i else A for j in range(4)), 1, 1) for i in range(4)]
+    calls += [lambda n=n: be.tree_attention_workspace(c, _trees(lrs, **{n: B}), 4) for n in ("seq", "ctx", "start", "mask")]
+    calls += [lambda: be.tree_attention_workspace(c, _trees(lrs, mask=A + 4), 4)]
+    calls += [lambda q=q: be.tree_attention(c, _trees(lrs), *q, 4, d_workspace=A, workspace_bytes=1 << 30)
+              for q in ((B, A), (A, B))]
+    calls += [_cache(lrs, pages=B).tile_bytes]
+    be._h = C.c_void_p(A)  # a handle that the refused calls do not read
+    try:
+        for call in calls:
+            with pytest.raises(lrs.LrsError, match="aligned") as e:
+                call()
+            assert e.value.code == INVALID
+    finally:
+        be._h = None
+
+
+def test_lengths_near_int32_are_refused(lrs):
+    c = _cache(lrs, max_pages=(2 ** 31 - 1) // 64)
+    with pytest.raises(lrs.LrsError) as e:
+        _Host(lrs).tree_attention_workspace(c, _trees(lrs, max_len=2 ** 31 - 64), 2)
+    assert e.value.code == UNSUPPORTED
+
+
 def test_default_stream_is_not_the_backends(lrs):
     assert [lrs._cuda_stream(s) for s in (None, 0, 1, 12345)] == [None, 1, 1, 12345]
 
