@@ -68,7 +68,7 @@ struct TaShape {
   // Registers a thread: at launch, K and V, the softmax, O (increases beyond what
   // the others gave would wait for good).
   static constexpr int kRegs = NR == 64 ? 64 : NR == 32 ? 72 : 80;
-  static constexpr int kRegsKV = 64, kRegsS = NR == 64 ? 56 : NR == 32 ? 64 : 80;
+  static constexpr int kRegsKV = NR == 64 ? 48 : 64, kRegsS = NR == 16 ? 80 : 64;
   static constexpr int kRegsO = 96;
   static_assert((1 + kVG) * kRegsKV + kSG * kRegsS + kRegsO <= (2 + kVG + kSG) * kRegs, "registers");
   static_assert(kRegsS <= kRegs && kRegsKV <= kRegs && kRegsO > kRegs, "the roles' changes of registers");
@@ -125,7 +125,7 @@ struct TaShared {
   float fin[2][kMaxRows];                // per unit parity: the factor of a row's output
   unsigned long long mask[2][kMaxRows];  // the row's node mask
   uint32_t vis[4][LRS_TREE_MAX_NODES];   // rows of a softmax group that see a node
-  float* out[2][kMaxRows];               // the row's output
+  alignas(16) float* out[2][kMaxRows];   // the row's output
   unsigned vbad[2][8][2];                // nodes whose V is not finite, per warp that reads V
   int moved[4][4];  // per tile and softmax group
   int fail[2][4];  // a softmax warp's wait gave up, per tile parity and group
@@ -450,14 +450,16 @@ __device__ __forceinline__ void decode_k(const uint8_t* raw, uint32_t at, int r,
       uint32_t hi[8], lo[8];
       const __half2 d2 = __half2half2(d1);
       const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-      d1 = *reinterpret_cast<const __half*>(scale + ((b + 1 < kSteps ? b + 1 : b) >> 1) * 2);
-      if (b + 1 < kSteps) w4 = *reinterpret_cast<const uint4*>(code + (b + 1) * kPageSize * 16);
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         uint32_t x[2], y[2];
         ta_q8(w[i], d2, d2, x, y);
         hi[i * 2] = x[0], hi[i * 2 + 1] = x[1];
         lo[i * 2] = y[0], lo[i * 2 + 1] = y[1];
+      }
+      if (b + 1 < kSteps) {
+        w4 = *reinterpret_cast<const uint4*>(code + (b + 1) * kPageSize * 16);
+        d1 = *reinterpret_cast<const __half*>(scale + ((b + 1) >> 1) * 2);
       }
       ta_st8(at + b * 8, hi);
       ta_st8(at + HD / 2 + b * 8, lo);
@@ -513,16 +515,15 @@ __device__ __forceinline__ void decode_v(const uint8_t* raw, uint32_t col, int w
 #pragma unroll 1
     for (int g = 0; g < S::kSlotPos / 16; g++) {
       uint32_t x[2][8];
-      const uint32_t c[4] = {cw[0], cw[1], cw[2], cw[3]};
       const uint32_t d[8] = {d8[0].x, d8[0].y, d8[0].z, d8[0].w, d8[1].x, d8[1].y, d8[1].z, d8[1].w};
-      if (g + 1 < S::kSlotPos / 16) fetch(g + 1);
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         uint32_t hi[2], lo[2];
-        ta_q8(c[i], ta_u2(d[2 * i]), ta_u2(d[2 * i + 1]), hi, lo);
+        ta_q8(cw[i], ta_u2(d[2 * i]), ta_u2(d[2 * i + 1]), hi, lo);
         x[0][i * 2] = hi[0], x[0][i * 2 + 1] = hi[1];
         x[1][i * 2] = lo[0], x[1][i * 2 + 1] = lo[1];
       }
+      if (g + 1 < S::kSlotPos / 16) fetch(g + 1);
 #pragma unroll
       for (int q = 0; q < 2; q++) ta_st8(col + q * (kTilePos / 2) + g * 8, x[q]);
     }
@@ -1084,15 +1085,19 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
 #pragma unroll
         for (int g = 0; g < S::kVG; g++)
           vbad |= sh.vbad[u][g * 4 + i][0] | (unsigned long long)sh.vbad[u][g * 4 + i][1] << 32;
-      if (__builtin_expect(vbad != 0, 0)) {
-#pragma unroll
-        for (int r = 0; r < NR; r++)
-          if (sh.mask[u][r] & vbad) o[r] = __int_as_float(0x7fc00000);
+      if (__builtin_expect(vbad != 0, 0)) {  // (the four warps write the same)
+#pragma unroll 1
+        for (int r = lane; r < NR; r += 32)
+          if (sh.mask[u][r] & vbad) sh.fin[u][r] = __int_as_float(0x7fc00000);
+        __syncwarp();
       }
 #pragma unroll
-      for (int r = 0; r < NR; r++) {
+      for (int r = 0; r < NR; r += 2) {
         if (r % 16 == 0 && r >= it.rows) break;
-        if (r < it.rows) sh.out[u][r][h] = o[r] * sh.fin[u][r];
+        const float2 f = *reinterpret_cast<const float2*>(&sh.fin[u][r]);
+        const ulonglong2 at = *reinterpret_cast<const ulonglong2*>(&sh.out[u][r]);
+        if (r < it.rows) reinterpret_cast<float*>(at.x)[h] = o[r] * f.x;
+        if (r + 1 < it.rows) reinterpret_cast<float*>(at.y)[h] = o[r + 1] * f.y;
       }
       __syncwarp();
       if (lane == 0) ta_arrive(&sh.u_empty[u]);
@@ -1210,60 +1215,60 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
                                           : 0x000000001020ull;
     const uint64_t qdesc = ta_desc(sbase + S::kOffQ, 128, HD / 8 * 128);
     const uint64_t pdesc = ta_desc(sbase + S::kOffP, NR * 16, 128);
-    uint32_t tile = 0, qk = 0;
+    uint32_t tile = 0, qk = 0;  // products issued
     TaRing<S::kNV> vbuf;
     TaRing<S::kNP> pbuf;
-    auto qk_tile = [&](int steps) {  // scores of tile `qk`
-      const uint32_t d = tmem + S::kTmS, idesc = ta_idesc(kF16, false, steps * 16);
-#pragma unroll
-      for (int half = 0; half < 2; half++) {
-        bool good = ta_wait(sh, &sh.ak_full[half], qk & 1);
-        if (half == 0 && good && qk > 0) good = ta_wait(sh, &sh.s_empty, (qk - 1) & 1);
-        if (!good) return false;
-        ta_fence_after();
-#pragma unroll
-        for (int i = 0; i < S::kProducts; i++) {
-          const uint32_t ta = (uint32_t)(kTerms >> (8 * i)) & 15, tb = (uint32_t)(kTerms >> (8 * i + 4)) & 15;
-          const uint32_t at = tmem + S::kTmK + ta * (HD / 2);
-          const uint64_t qd = qdesc + tb * (S::kQTerm >> 4);
-          const uint32_t ah = at + half * (HD / 4);
-          const uint64_t qh = qd + half * (HD / 2);
-          if constexpr (HD == 128) ta_mma4(d, ah, qh, 16, idesc, (half | i) != 0, el);
-          else ta_mma2(d, ah, qh, 16, idesc, (half | i) != 0, el);
-        }
-        ta_commit(bar_at(&sh.ak_empty[half]), el);
-      }
-      ta_commit(bar_at(&sh.s_full), el);
-      qk++;
-      return true;
-    };
     while (feed.next(sh, lane, ok)) {
       const int steps = NR == 16 ? 1 : (__shfl_sync(0xffffffffu, it.rows, 0) + 15) >> 4;
       const int tiles = __shfl_sync(0xffffffffu, it.t1 - it.t0, 0);
-      ok = qk_tile(steps);
 #pragma unroll 1
-      for (int t = 0; t < tiles && ok; t++, tile++) {
-        if (t + 1 < tiles) ok = qk_tile(steps);
-        const uint32_t vb = vbuf.at, pb = pbuf.at;
-        ok = ok && ta_wait(sh, &sh.av_full[vb], vbuf.parity) && ta_wait(sh, &sh.p_full[pb], pbuf.parity);
-        vbuf.step();
-        pbuf.step();
-        if (ok && tile > 0) ok = ta_wait(sh, &sh.o_empty, (tile - 1) & 1);
-        if (!ok) break;
-        ta_fence_after();
-        const uint32_t d = tmem + S::kTmO, idesc = ta_idesc(kF16, true, steps * 16), av = tmem + S::kTmV + vb * S::kVCols;
-        const uint64_t pd = pdesc + (uint64_t)(pb * (S::kPBuf >> 4));
+      for (int t = 0; t <= tiles && ok; t++) {
+        if (t < tiles) {  // scores of tile t
+          const uint32_t d = tmem + S::kTmS, idesc = ta_idesc(kF16, false, steps * 16);
 #pragma unroll
-        for (int i = 0; i < S::kProducts; i++) {
-          const uint32_t ta = (uint32_t)(kTerms >> (8 * i)) & 15, tb = (uint32_t)(kTerms >> (8 * i + 4)) & 15;
-          const uint32_t at = av + ta * (kTilePos / 2);
-          const uint64_t pt = pd + tb * (S::kPTerm >> 4);
-          ta_mma4(d, at, pt, 2 * NR, idesc, i != 0, el);
-          ta_mma4(d, at + 32, pt + 8 * NR, 2 * NR, idesc, true, el);
+          for (int half = 0; half < 2; half++) {
+            ok = ok && ta_wait(sh, &sh.ak_full[half], qk & 1);
+            if (half == 0 && qk > 0) ok = ok && ta_wait(sh, &sh.s_empty, (qk - 1) & 1);
+            if (!ok) break;
+            ta_fence_after();
+#pragma unroll
+            for (int i = 0; i < S::kProducts; i++) {
+              const uint32_t ta = (uint32_t)(kTerms >> (8 * i)) & 15, tb = (uint32_t)(kTerms >> (8 * i + 4)) & 15;
+              const uint32_t ah = tmem + S::kTmK + ta * (HD / 2) + half * (HD / 4);
+              const uint64_t qh = qdesc + tb * (S::kQTerm >> 4) + half * (HD / 2);
+              if constexpr (HD == 128) ta_mma4(d, ah, qh, 16, idesc, (half | i) != 0, el);
+              else ta_mma2(d, ah, qh, 16, idesc, (half | i) != 0, el);
+            }
+            ta_commit(bar_at(&sh.ak_empty[half]), el);
+          }
+          if (!ok) break;
+          ta_commit(bar_at(&sh.s_full), el);
+          qk++;
         }
-        ta_commit(bar_at(&sh.o_full), el);
-        ta_commit(bar_at(&sh.av_empty[vb]), el);
-        ta_commit(bar_at(&sh.p_empty[pb]), el);
+        if (t > 0) {  // values of the tile before it
+          const uint32_t vb = vbuf.at, pb = pbuf.at;
+          ok = ok && ta_wait(sh, &sh.av_full[vb], vbuf.parity) && ta_wait(sh, &sh.p_full[pb], pbuf.parity);
+          vbuf.step();
+          pbuf.step();
+          if (ok && tile > 0) ok = ta_wait(sh, &sh.o_empty, (tile - 1) & 1);
+          if (!ok) break;
+          ta_fence_after();
+          const uint32_t d = tmem + S::kTmO, idesc = ta_idesc(kF16, true, steps * 16);
+          const uint32_t av = tmem + S::kTmV + vb * S::kVCols;
+          const uint64_t pd = pdesc + (uint64_t)(pb * (S::kPBuf >> 4));
+#pragma unroll
+          for (int i = 0; i < S::kProducts; i++) {
+            const uint32_t ta = (uint32_t)(kTerms >> (8 * i)) & 15, tb = (uint32_t)(kTerms >> (8 * i + 4)) & 15;
+            const uint32_t at = av + ta * (kTilePos / 2);
+            const uint64_t pt = pd + tb * (S::kPTerm >> 4);
+            ta_mma4(d, at, pt, 2 * NR, idesc, i != 0, el);
+            ta_mma4(d, at + 32, pt + 8 * NR, 2 * NR, idesc, true, el);
+          }
+          ta_commit(bar_at(&sh.o_full), el);
+          ta_commit(bar_at(&sh.av_empty[vb]), el);
+          ta_commit(bar_at(&sh.p_empty[pb]), el);
+          tile++;
+        }
       }
     }
     if (!ok) {  // MMAs in flight end before their memory goes away
