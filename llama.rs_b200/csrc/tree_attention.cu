@@ -122,13 +122,13 @@ struct TaShared {
   float nm[kMaxRows];                    // kShift - maximum (0 before the row has one)
   float f[4][kMaxRows];                  // rescaling of the earlier tiles, per tile
   float red[4][4][16];                  // a softmax group's warps meet here
+  float top[kMaxRows];                  // a row's maximum - kShift, kUnset before it has one
   float fin[2][kMaxRows];                // per unit parity: the factor of a row's output
   unsigned long long mask[2][kMaxRows];  // the row's node mask
   uint32_t vis[4][LRS_TREE_MAX_NODES];   // rows of a softmax group that see a node
   alignas(16) float* out[2][kMaxRows];   // the row's output
   unsigned vbad[2][8][2];                // nodes whose V is not finite, per warp that reads V
-  int moved[4][4];  // per tile and softmax group
-  int fail[2][4];  // a softmax warp's wait gave up, per tile parity and group
+  alignas(16) int moved[4][4];  // per tile and softmax group
   TaUnit unit[kUnits];
   uint64_t k_full[8], k_empty[8], v_full[8], v_empty[8];
   uint64_t ak_full[2], ak_empty[2];  // K's halves of the columns
@@ -385,16 +385,15 @@ __host__ __device__ constexpr size_t ta_seg_floats() {
 struct TaFeed {
   TaUnit u;
   int index = -1;  // number of the unit in this CTA
-  TaRing<kUnits> ring;
   // False at the end of the list, or (ok = false) when the wait gave up.
   __device__ __forceinline__ bool next(TaShared& sh, int lane, bool& ok) {
-    ok = ok && ta_wait(sh, &sh.unit_full[ring.at], ring.parity);
-    if (!ok) return false;
-    u = sh.unit[ring.at];
-    __syncwarp();
-    if (lane == 0) ta_arrive(&sh.unit_empty[ring.at]);
-    ring.step();
     index++;
+    const int at = index % kUnits;
+    ok = ok && ta_wait(sh, &sh.unit_full[at], index / kUnits & 1);
+    if (!ok) return false;
+    u = sh.unit[at];
+    __syncwarp();
+    if (lane == 0) ta_arrive(&sh.unit_empty[at]);
     return u.t1 > 0;
   }
 };
@@ -688,7 +687,6 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
       mbar_init(&sh.p_empty[i], 1);
       mbar_init(&sh.u_full[i], 4 * S::kSG);
       mbar_init(&sh.u_empty[i], kWarpsD);
-      sh.fail[i][0] = sh.fail[i][1] = sh.fail[i][2] = sh.fail[i][3] = 0;
     }
 #pragma unroll 1
     for (int i = 0; i < kUnits; i++) {
@@ -878,53 +876,52 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
     float* nm = sh.nm + base;
     float2 l[8];
     uint32_t tile = 0;
-    TaRing<S::kNP> buf;
-    // the four warps meet at barriers: one whose wait gave up goes on (on stale
-    // data, in bounds) to the next vote, where they leave together
+    // the four warps meet at barriers: one whose wait gave up goes on (without
+    // waits, on stale data, in bounds) to the next unit's, where they leave together
     for (;;) {
       const bool more = feed.next(sh, lane, ok);
       const int u = feed.index & 1;
       const float* c = sh.c[feed.index % kUnits] + base;
       const bool whole = it.t0 == 0 && it.t1 == it.tiles, idle = base >= it.rows;  // idle: no rows here
       float* seg = segs + (size_t)(2 * blockIdx.x + (it.t0 == 0)) * ta_seg_floats<HD, NR>();
-      unsigned long long row_mask = 0;  // of row base + lane
-      float* my_out = nullptr;
-      if (more && lane < 16 && base + lane < it.rows) {
-        const int row = it.row0 + base + lane, node = row / a.group, g = row % a.group;
-        my_out = whole ? a.out + (size_t)(it.s + node) * a.out_ld + (size_t)(it.kvh * a.group + g) * HD
-                       : seg + 2 * NR + (base + lane) * HD;
-        row_mask = a.mask ? a.mask[it.s + node] : (node == 63 ? ~0ull : (2ull << node) - 1);
-        if (it.n < 64) row_mask &= (1ull << it.n) - 1;
-      }
       if (more && feed.index >= 2) ok = ok && ta_wait(sh, &sh.u_empty[u], ((feed.index >> 1) - 1) & 1);
       if (more && gt < 16) {
+        unsigned long long row_mask = 0;
+        float* my_out = nullptr;
+        if (my < it.rows) {
+          const int row = it.row0 + my, node = row / a.group, g = row - node * a.group;
+          my_out = whole ? a.out + (size_t)(it.s + node) * a.out_ld + (size_t)(it.kvh * a.group + g) * HD
+                         : seg + 2 * NR + my * HD;
+          row_mask = a.mask ? a.mask[it.s + node] : (node == 63 ? ~0ull : (2ull << node) - 1);
+          if (it.n < 64) row_mask &= (1ull << it.n) - 1;
+        }
+        sh.mask[u][my] = row_mask;
         sh.out[u][my] = my_out;
+        sh.top[my] = kUnset;
         nm[gt] = 0.0f;
       }
       if (ta_group_or(bar, !more || !ok)) break;
 #pragma unroll
       for (int r = 0; r < 8; r++) l[r] = make_float2(0.0f, 0.0f);
-      bool masks = false, left = false, unset = true;  // unset: a row may have no maximum yet
-      float max_of = kUnset;                           // this thread's row's, - kShift
+      bool masks = false, unset = true;  // unset: a row may have no maximum yet
 #pragma unroll 1
       for (int t = it.t0; t < it.t1; t++, tile++) {
-        const int p = t * kTilePos + w * 32 + lane;
         uint32_t vis = 0xffffu;  // rows that see this lane's position
         if (__builtin_expect((t + 1) * kTilePos > it.ctx, 0)) {
           if (!masks) {  // the rows that see each node, from the nodes that each row sees
             masks = true;
-            if (gt < 16) sh.mask[u][my] = row_mask;
+            const unsigned long long row_mask = sh.mask[u][base + (lane & 15)];
 #pragma unroll 1
             for (int j = w; j < it.n; j += 4) {
-              const uint32_t v = __ballot_sync(0xffffffffu, row_mask >> j & 1);
+              const uint32_t v = __ballot_sync(0xffffffffu, lane < 16 && (row_mask >> j & 1));
               if (lane == 0) sh.vis[grp][j] = v;
             }
             ta_group_sync(bar);
           }
+          const int p = t * kTilePos + w * 32 + lane;
           if (p >= it.ctx) vis = p < it.len ? sh.vis[grp][p - it.ctx] : 0;
         }
         ok = ok && ta_wait(sh, &sh.s_full, tile & 1);
-        if (__builtin_expect(!ok, 0)) sh.fail[tile & 1][grp] = 1;
         ta_fence_after();
         float s[16];
         float* f = sh.f[tile & 3] + base;
@@ -939,8 +936,6 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
 #pragma unroll
         for (int r = 1; r < 16; r++) top = fmaxf(top, s[r]);
         const bool move = ta_group_or(bar, !idle && (unset || top > kLimit));
-        left = *reinterpret_cast<volatile int*>(&sh.fail[tile & 1][grp]) != 0;
-        if (__builtin_expect(left, 0)) break;
         if (__builtin_expect(move, 0)) {
           // the rows' largest exponents over the tile, to kShift
           float mx = -INFINITY;
@@ -953,15 +948,17 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
           ta_group_sync(bar);
           bool none = false;
           if (gt < 16) {
+            const float old = sh.top[my];
             mx = fmaxf(fmaxf(sh.red[grp][0][gt], sh.red[grp][1][gt]), fmaxf(sh.red[grp][2][gt], sh.red[grp][3][gt]));
             // a row without a maximum takes the tile's, the others a larger one
-            float by = max_of == kUnset ? mx - kShift : fmaxf(mx - kShift, 0.0f);
+            float by = old == kUnset ? mx - kShift : fmaxf(mx - kShift, 0.0f);
             if (!(mx > -INFINITY)) by = 0.0f;
-            f[gt] = max_of == kUnset ? 0.0f : ta_exp2(-by);
+            f[gt] = old == kUnset ? 0.0f : ta_exp2(-by);
             sh.red[grp][0][gt] = -by;
-            if (mx > -INFINITY) max_of = (max_of == kUnset ? 0.0f : max_of) + by;
-            none = max_of == kUnset;
-            nm[gt] = none ? 0.0f : -max_of;
+            const float now = mx > -INFINITY ? (old == kUnset ? 0.0f : old) + by : old;
+            none = now == kUnset;
+            sh.top[my] = now;
+            nm[gt] = none ? 0.0f : -now;
           }
           unset = ta_group_or(bar, none);
 #pragma unroll
@@ -971,15 +968,12 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
             s[r] = d.x, s[r + 1] = d.y;
             l[r / 2].x *= g.x, l[r / 2].y *= g.y;
           }
-        } else if (gt < 16) {
-          f[gt] = 1.0f;
         }
         if (gt == 0) sh.moved[tile & 3][grp] = move;
         // P in terms, N-major (a lane writes 8 rows at once), and the row sums
-        const uint32_t pb = buf.at;
+        const uint32_t pb = tile % S::kNP;
         // (of two buffers the older product had ended before these scores came)
-        if (S::kNP == 1 && tile >= 1) ok = ok && ta_wait(sh, &sh.p_empty[pb], buf.parity ^ 1);
-        buf.step();
+        if (S::kNP == 1 && tile >= 1) ok = ok && ta_wait(sh, &sh.p_empty[pb], (tile - 1) & 1);
         const int pp = w * 32 + lane;
         uint8_t* dst = smem + S::kOffP + pb * S::kPBuf + (pp >> 3) * (NR * 16) + (pp & 7) * 16 + base * 16;
         if (!idle) {
@@ -1006,7 +1000,6 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
         __syncwarp();
         if (lane == 0) ta_arrive(&sh.p_full[pb]);
       }
-      if (left) break;
       // the rows' sums over the lanes: 16 rows by 32 lanes to a row a lane pair
       float* lf = reinterpret_cast<float*>(l);
       int row = 0;
@@ -1028,7 +1021,7 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
       if (gt < 16) {
         const float sum = (sh.red[grp][0][gt] + sh.red[grp][1][gt]) + (sh.red[grp][2][gt] + sh.red[grp][3][gt]);
         sh.fin[u][my] = !whole ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
-        if (!whole && my < it.rows) seg[2 * my] = max_of, seg[2 * my + 1] = sum;
+        if (!whole && my < it.rows) seg[2 * my] = sh.top[my], seg[2 * my + 1] = sum;
       }
       __syncwarp();
       if (lane == 0) ta_arrive(&sh.u_full[u]);
@@ -1049,20 +1042,15 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
         ok = ta_wait(sh, &sh.o_full, tile & 1);
         if (!ok) break;
         ta_fence_after();
-        int moved = 0;
-#pragma unroll
-        for (int g = 0; g < S::kSG; g++) moved |= sh.moved[tile & 3][g];
-        if (__builtin_expect(moved, 0)) {
-          const float* f = sh.f[tile & 3];
-#pragma unroll
-          for (int r = 0; r < NR; r++) {
-            if (r % 16 == 0 && r / 16 >= steps) break;
-            o[r] *= f[r];
-          }
-        }
+        const int4 moved = *reinterpret_cast<const int4*>(sh.moved[tile & 3]);
+        const float* f = sh.f[tile & 3];
 #pragma unroll
         for (int c = 0; c < NR / 16; c++) {
           if (c >= steps) break;
+          if (__builtin_expect(c == 0 ? moved.x : c == 1 ? moved.y : c == 2 ? moved.z : moved.w, 0)) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[c * 16 + i] *= f[c * 16 + i];
+          }
           float x[16];
           ta_ld16(tmem + lanes + S::kTmO + c * 16, x);
           ta_wait_ld(x);
