@@ -131,9 +131,13 @@ struct TaShared {
   alignas(16) int moved[4][4];  // per tile and softmax group
   TaUnit unit[kUnits];
   uint64_t k_full[8], k_empty[8], v_full[8], v_empty[8];
-  uint64_t ak_full[2], ak_empty[2];  // K's halves of the columns
-  uint64_t s_full, s_empty, o_full, o_empty, drain;
-  uint64_t av_full[2], av_empty[2], p_full[2], p_empty[2], u_full[2], u_empty[2];
+  // Phases count tiles (of pv_*: every second one).  Before the MMA warp issues a
+  // product it makes one wait for all that the product needs, as each costs it some
+  // 200 clocks: qk_go, K's first half of the columns here and the last scores read
+  // (k_rest: the other half); pv_go, V and P here and the last sums read.
+  uint64_t qk_go, k_rest, k_half, s_full;  // k_half: the first half's scores are done
+  uint64_t pv_go[2], pv_done[2], drain;
+  uint64_t u_full[2], u_empty[2];
   uint64_t unit_full[kUnits], unit_empty[kUnits];
   int abort;
   uint32_t tmem;
@@ -273,12 +277,14 @@ __device__ __forceinline__ bool ta_try_wait(uint32_t bar, uint32_t parity) {
       : "memory");
   return done != 0;
 }
-// A run of tests, as few instructions as waiting warps may take from the others.
+// A run of tests by a whole warp, as few instructions as waiting warps may take from
+// the others; the lanes agree on the result.
 __device__ __forceinline__ bool ta_try_many(uint32_t bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
       "{\n .reg .pred p, q;\n .reg .u32 n;\n mov.u32 n, 2048;\n"
-      "AGAIN:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra DONE;\n"
+      "AGAIN:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      " vote.sync.all.pred p, p, 0xffffffff;\n @p bra DONE;\n"
       " sub.u32 n, n, 1;\n setp.ne.u32 q, n, 0;\n @q bra AGAIN;\n"
       "DONE:\n selp.u32 %0, 1, 0, p;\n}"
       : "=r"(done)
@@ -293,11 +299,15 @@ __device__ __forceinline__ bool ta_wait(TaShared& sh, uint64_t* bar, uint32_t pa
   const uint32_t at = smem_u32(bar);
 #pragma unroll 1
   for (uint32_t i = 0; i < kPolls / 2048; i++) {
-    if (__all_sync(0xffffffffu, ta_try_many(at, parity))) return true;
+    if (ta_try_many(at, parity)) return true;
     if (__any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&sh.abort))) return false;
   }
   *reinterpret_cast<volatile int*>(&sh.abort) = 1;
   return false;
+}
+// Waits for the product of P and V of this CTA's tile `tile`.
+__device__ __forceinline__ bool wait_pv(TaShared& sh, uint32_t tile) {
+  return ta_wait(sh, &sh.pv_done[tile & 1], tile >> 1 & 1);
 }
 // A position in a ring of N barriers and the parity of its current pass.
 template <int N>
@@ -444,7 +454,8 @@ __device__ __forceinline__ void decode_k(const uint8_t* raw, uint32_t at, int r,
     const uint8_t* scale = raw + q8_k_scale(HD, r, half * kSteps / 2);
     uint4 w4 = *reinterpret_cast<const uint4*>(code);
     __half d1 = *reinterpret_cast<const __half*>(scale);
-#pragma unroll 1
+    // (two steps a turn: one took 5 % longer over the whole kernel, four no less)
+#pragma unroll 2
     for (int b = 0; b < kSteps; b++) {  // the next step's words are under way
       uint32_t hi[8], lo[8];
       const __half2 d2 = __half2half2(d1);
@@ -671,20 +682,14 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
       mbar_init(&sh.v_full[i], 1);
       mbar_init(&sh.v_empty[i], kWarpsD);
     }
-    for (int i = 0; i < 2; i++) {
-      mbar_init(&sh.ak_full[i], 4);
-      mbar_init(&sh.ak_empty[i], 1);
-    }
+    mbar_init(&sh.qk_go, 4 + 4 * S::kSG);
+    mbar_init(&sh.k_rest, 4);
+    mbar_init(&sh.k_half, 1);
     mbar_init(&sh.s_full, 1);
-    mbar_init(&sh.s_empty, 4 * S::kSG);
-    mbar_init(&sh.o_full, 1);
-    mbar_init(&sh.o_empty, kWarpsD);
     mbar_init(&sh.drain, 1);
     for (int i = 0; i < 2; i++) {
-      mbar_init(&sh.av_full[i], S::kVG * kWarpsD);
-      mbar_init(&sh.av_empty[i], 1);
-      mbar_init(&sh.p_full[i], 4 * S::kSG);
-      mbar_init(&sh.p_empty[i], 1);
+      mbar_init(&sh.pv_go[i], 4 * S::kSG + (S::kVG + 1) * kWarpsD);
+      mbar_init(&sh.pv_done[i], 1);
       mbar_init(&sh.u_full[i], 4 * S::kSG);
       mbar_init(&sh.u_empty[i], kWarpsD);
     }
@@ -800,7 +805,7 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
     ring.at = warp * 32 / S::kSlotPos;
     while (feed.next(sh, lane, ok)) {
       // the last unit's scores are done with q and its factors
-      if (tile > 0) ok = ta_wait(sh, &sh.ak_empty[1], (tile - 1) & 1);
+      if (tile > 0) ok = ta_wait(sh, &sh.s_full, (tile - 1) & 1);
       if (!ok) break;
       load_q<HD, DT, NR>(a, it, smem, sh.c[feed.index % kUnits], warp, lane);
       fence_proxy_async();
@@ -812,7 +817,7 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
         const int r = (warp * 32 + lane) % S::kSlotPos;
 #pragma unroll 1
         for (int half = 0; half < 2; half++) {
-          if (ok && tile > 0) ok = ta_wait(sh, &sh.ak_empty[half], (tile - 1) & 1);
+          if (ok && tile > 0) ok = ta_wait(sh, half ? &sh.s_full : &sh.k_half, (tile - 1) & 1);
           if (!ok) break;
           ta_fence_after();
           decode_k<HD, DT, NR>(raw, tmem + lanes + S::kTmK, r, half);
@@ -821,7 +826,7 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
           ta_wait_st();
           ta_fence_before();
           __syncwarp();
-          if (lane == 0) ta_arrive(&sh.ak_full[half]);
+          if (lane == 0) ta_arrive(half ? &sh.k_rest : &sh.qk_go);
         }
       }
     }
@@ -833,7 +838,6 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
     uint32_t tile = 0;
     TaRing<S::kRingV> ring;
     ring.at = vg * kMine;
-    TaRing<S::kNV> buf;
     while (w < kWarpsD && feed.next(sh, lane, ok)) {
       // the words of the unit before last have been read
       const int par = feed.index & 1;
@@ -843,9 +847,8 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
       __syncwarp();
 #pragma unroll 1
       for (int t = it.t0; t < it.t1 && ok; t++, tile++) {
-        const uint32_t vb = buf.at;
-        if (tile >= S::kNV) ok = ta_wait(sh, &sh.av_empty[vb], buf.parity ^ 1);
-        buf.step();
+        const uint32_t vb = tile % S::kNV;
+        if (tile >= S::kNV) ok = wait_pv(sh, tile - S::kNV);
         ta_fence_after();
 #pragma unroll 1
         for (int k = vg * kMine; k < (vg + 1) * kMine && ok; k++) {
@@ -865,7 +868,7 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
         ta_wait_st();
         ta_fence_before();
         __syncwarp();
-        if (lane == 0) ta_arrive(&sh.av_full[vb]);
+        if (lane == 0) ta_arrive(&sh.pv_go[tile & 1]);
       }
     }
   } else if (warp < S::kWarpO) {
@@ -876,6 +879,7 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
     float* nm = sh.nm + base;
     float2 l[8];
     uint32_t tile = 0;
+    if (lane == 0) ta_arrive(&sh.qk_go);  // no scores before the first tile's
     // the four warps meet at barriers: one whose wait gave up goes on (without
     // waits, on stale data, in bounds) to the next unit's, where they leave together
     for (;;) {
@@ -929,7 +933,7 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
         ta_wait_ld(s);
         ta_fence_before();
         __syncwarp();
-        if (lane == 0) ta_arrive(&sh.s_empty);  // the next tile's scores may come
+        if (lane == 0) ta_arrive(&sh.qk_go);  // the next tile's scores may come
         ta_exponents<kF16>(s, c, nm, vis);
         // does a score exceed its row's maximum by more than the margin?
         float top = s[0];
@@ -973,7 +977,7 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
         // P in terms, N-major (a lane writes 8 rows at once), and the row sums
         const uint32_t pb = tile % S::kNP;
         // (of two buffers the older product had ended before these scores came)
-        if (S::kNP == 1 && tile >= 1) ok = ok && ta_wait(sh, &sh.p_empty[pb], (tile - 1) & 1);
+        if (S::kNP == 1 && tile >= 1) ok = ok && wait_pv(sh, tile - 1);
         const int pp = w * 32 + lane;
         uint8_t* dst = smem + S::kOffP + pb * S::kPBuf + (pp >> 3) * (NR * 16) + (pp & 7) * 16 + base * 16;
         if (!idle) {
@@ -998,7 +1002,7 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
           fence_proxy_async();
         }
         __syncwarp();
-        if (lane == 0) ta_arrive(&sh.p_full[pb]);
+        if (lane == 0) ta_arrive(&sh.pv_go[tile & 1]);
       }
       // the rows' sums over the lanes: 16 rows by 32 lanes to a row a lane pair
       float* lf = reinterpret_cast<float*>(l);
@@ -1032,6 +1036,7 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
     ta_regs_inc<S::kRegsO>();
     const int w = warp - S::kWarpO, h = w * 32 + lane;
     uint32_t tile = 0;
+    if (w < kWarpsD && lane == 0) ta_arrive(&sh.pv_go[0]);  // no sums before the first tile's
     while (w < kWarpsD && feed.next(sh, lane, ok)) {
       const int u = feed.index & 1, steps = (it.rows + 15) >> 4;
       float o[NR];
@@ -1039,7 +1044,7 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
       for (int r = 0; r < NR; r++) o[r] = 0.0f;
 #pragma unroll 1
       for (int t = it.t0; t < it.t1 && ok; t++, tile++) {
-        ok = ta_wait(sh, &sh.o_full, tile & 1);
+        ok = wait_pv(sh, tile);
         if (!ok) break;
         ta_fence_after();
         const int4 moved = *reinterpret_cast<const int4*>(sh.moved[tile & 3]);
@@ -1062,7 +1067,7 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
         }
         ta_fence_before();
         __syncwarp();
-        if (lane == 0) ta_arrive(&sh.o_empty);
+        if (lane == 0) ta_arrive(&sh.pv_go[(tile + 1) & 1]);
       }
       if (!ok) break;
       ok = ta_wait(sh, &sh.u_full[u], (feed.index >> 1) & 1);
@@ -1204,8 +1209,6 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
     const uint64_t qdesc = ta_desc(sbase + S::kOffQ, 128, HD / 8 * 128);
     const uint64_t pdesc = ta_desc(sbase + S::kOffP, NR * 16, 128);
     uint32_t tile = 0, qk = 0;  // products issued
-    TaRing<S::kNV> vbuf;
-    TaRing<S::kNP> pbuf;
     while (feed.next(sh, lane, ok)) {
       const int steps = NR == 16 ? 1 : (__shfl_sync(0xffffffffu, it.rows, 0) + 15) >> 4;
       const int tiles = __shfl_sync(0xffffffffu, it.t1 - it.t0, 0);
@@ -1215,8 +1218,7 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
           const uint32_t d = tmem + S::kTmS, idesc = ta_idesc(kF16, false, steps * 16);
 #pragma unroll
           for (int half = 0; half < 2; half++) {
-            ok = ok && ta_wait(sh, &sh.ak_full[half], qk & 1);
-            if (half == 0 && qk > 0) ok = ok && ta_wait(sh, &sh.s_empty, (qk - 1) & 1);
+            ok = ok && ta_wait(sh, half ? &sh.k_rest : &sh.qk_go, qk & 1);
             if (!ok) break;
             ta_fence_after();
 #pragma unroll
@@ -1227,18 +1229,14 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
               if constexpr (HD == 128) ta_mma4(d, ah, qh, 16, idesc, (half | i) != 0, el);
               else ta_mma2(d, ah, qh, 16, idesc, (half | i) != 0, el);
             }
-            ta_commit(bar_at(&sh.ak_empty[half]), el);
+            ta_commit(bar_at(half ? &sh.s_full : &sh.k_half), el);
           }
           if (!ok) break;
-          ta_commit(bar_at(&sh.s_full), el);
           qk++;
         }
         if (t > 0) {  // values of the tile before it
-          const uint32_t vb = vbuf.at, pb = pbuf.at;
-          ok = ok && ta_wait(sh, &sh.av_full[vb], vbuf.parity) && ta_wait(sh, &sh.p_full[pb], pbuf.parity);
-          vbuf.step();
-          pbuf.step();
-          if (ok && tile > 0) ok = ta_wait(sh, &sh.o_empty, (tile - 1) & 1);
+          const uint32_t vb = tile % S::kNV, pb = tile % S::kNP;
+          ok = ta_wait(sh, &sh.pv_go[tile & 1], tile >> 1 & 1);
           if (!ok) break;
           ta_fence_after();
           const uint32_t d = tmem + S::kTmO, idesc = ta_idesc(kF16, true, steps * 16);
@@ -1252,9 +1250,7 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
             ta_mma4(d, at, pt, 2 * NR, idesc, i != 0, el);
             ta_mma4(d, at + 32, pt + 8 * NR, 2 * NR, idesc, true, el);
           }
-          ta_commit(bar_at(&sh.o_full), el);
-          ta_commit(bar_at(&sh.av_empty[vb]), el);
-          ta_commit(bar_at(&sh.p_empty[pb]), el);
+          ta_commit(bar_at(&sh.pv_done[tile & 1]), el);
           tile++;
         }
       }
