@@ -360,7 +360,8 @@ typedef struct lrs_tree_batch {
  * graphs that may run at once, need one each.  out may be q (then q_ld =
  * out_ld).  A tree whose slot, node range or length is out of range is skipped,
  * its rows left as they were; the rows of one that reaches a page out of range
- * hold no defined values. */
+ * hold no defined values.  Of a tree without nodes nothing
+ * else is looked at (padded batches). */
 lrs_status lrs_tree_attention_workspace(const lrs_backend* backend, const lrs_kv_cache* cache,
                                         const lrs_tree_batch* trees, uint32_t n_heads,
                                         size_t* bytes);

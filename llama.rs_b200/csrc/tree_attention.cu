@@ -14,6 +14,15 @@
 // the cache there (a lane is a position of K, a column of V), so a tile passes
 // shared memory once, as raw cache bytes.
 //
+// A CTA is a pipeline of roles (TaShape): a copy warp brings a tile's raw pages in by
+// bulk copies; four warps decode K, four (eight) V; the softmax has a group of four
+// warps per 16 rows, a lane being a position, so that a row's statistics need the
+// other lanes only when its maximum moves; four warps keep the sums of O, a lane being
+// a column; one warp issues the MMAs.  The tiles of all trees are one list that the
+// CTAs share evenly, whatever the trees' lengths; what a unit (the rows of one tree,
+// KV head and chunk) has in several CTAs leaves as (maximum, sum, O) segments, which
+// tree_combine_kernel merges.
+//
 // Arithmetic.  The products are exact and accumulate in f32: each operand is a
 // sum of 16-bit terms, of which the products that matter at 2^-22 are taken.
 //   Q8_0  d * code = hi + lo in f16, exactly (hi = rn(d code), lo its error:
@@ -30,6 +39,17 @@
 // sums hold 2^-25 of the largest weight.  A lane is a position, so the test is
 // one comparison per score and one vote; the cross-lane maximum and the
 // rescaling of O run only in the tiles that raise it (the first one, mostly).
+//
+// What bounds it.  64 trees of 8 nodes on 2,100 to 4,100 positions, q8_0, 4 KV heads
+// of 7 queries, 128 wide: 118 us, 1.97 TB/s of the cache's bytes and 0.51 PFLOP/s of the
+// three products; 4 trees of 64 nodes on 7,200 to 8,200: 118 us, 0.72 PFLOP/s.  A tile takes some
+// 3,000 clocks, of which the tensor pipe needs 1,536 and the copies, at DRAM's rate,
+// 1,476; the schedulers issue in 64 of 100 clocks.  So the bound is the
+// instructions of decoding (of the values K and V's terms take 2.3 each) and of the
+// softmax, and next to it the chain of one tile's softmax (some 2,500 clocks).  A CTA
+// spends some 15,000 clocks before its first product (the schedule, cold instruction
+// fetches, q) and after its last one: small calls are that and the launches (5 nodes on
+// 100 positions: 15.4 us, two launches' 5 us among them).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -59,8 +79,10 @@ struct TaShape {
   static constexpr int kA = DT == LRS_KV_F32 ? 3 : DT == LRS_KV_BF16 ? 1 : 2;  // terms of K, V
   static constexpr int kB = DT == LRS_KV_Q8_0 ? 2 : 3;                        // terms of q, P
   static constexpr bool kF16 = DT == LRS_KV_Q8_0;
-  // Groups of four warps: K, V (up to 32 rows two, half of the positions each),
-  // the softmax (16 rows each), O; then a warp for the copies and one for the MMAs.
+  // Groups of four warps: K, V (up to 32 rows two, half of the positions each: a decode
+  // step of 64 sequences 41 us, with one 45; at 64 rows the threads are spent), the
+  // softmax (16 rows each: groups of 32 took the same time at 64 rows, and would be half
+  // idle below), O; then a warp for the copies and one for the MMAs.
   static constexpr int kSG = NR / 16, kVG = NR == 64 ? 1 : 2;
   static constexpr int kWarpV = 4, kWarpS = kWarpV + 4 * kVG, kWarpO = kWarpS + 4 * kSG;
   static constexpr int kWarpCopy = kWarpO + 4, kWarpMma = kWarpCopy + 1;
@@ -362,6 +384,7 @@ struct TaTree {
     ctx = a.ctx[t];
     seq = a.seq[t];
     chunks = tiles = n = 0;
+    if (s == end) return true;  // no nodes: nothing else of it is looked at (padded batches)
     if (s < 0 || end < s || end > a.n_nodes || end - s > a.max_nodes || ctx < 0 || ctx > a.max_len ||
         end - s > a.max_len - ctx || seq < 0 || seq >= a.c.n_seqs) {
       atomicExch(a.c.err, kErrCacheIndex);
@@ -369,7 +392,6 @@ struct TaTree {
     }
     n = end - s;
     len = ctx + n;
-    if (n == 0) return true;
     chunks = (n * a.group + nr - 1) / nr;
     tiles = (len + kTilePos - 1) / kTilePos;
     return true;
@@ -1300,16 +1322,24 @@ __global__ void __launch_bounds__(HD * 4) tree_combine_kernel(const __grid_const
       l == 0.0f ? 0.0f : o / l;
 }
 
-// Rows a unit: the smallest of 16, 32, 64 that holds a tree's rows.
-int unit_rows(const TreeArgs& a) {
+long long tiles_of(const TreeArgs& a, int nr) {
+  return (long long)a.n_trees * a.c.heads * ((a.max_nodes * a.group + nr - 1) / nr) *
+         ((a.max_len + kTilePos - 1) / kTilePos);
+}
+
+// Rows a unit: 16 while that gives a CTA two tiles at most, as the 16-row kernel starts
+// and ends sooner; else the smallest of 16, 32, 64 that holds a tree's rows, as each unit
+// decodes K and V for itself.  Measured with 16 / 32 / 64 rows, q8_0, 4 KV heads x 7 x 128:
+// 8 nodes on 1,100 positions 16.5 / 16.6 / 20.3 us, 5 on 3,000 19.9 / 22.2 / 24.8 us, 64
+// trees of one node on 700 to 1,100 34 / 38 / 41 us, but 64 of 8 on 2,100 to 4,100 221 /
+// 158 / 107 us; 8 of 13, f32, 2 x 6 x 128, on 1,500 to 2,050 78 / 53 / 55 us.
+int unit_rows(const TreeArgs& a, int sms) {
   const int rows = a.max_nodes * a.group;
-  return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  return rows <= 16 || tiles_of(a, 16) <= 2ll * sms ? 16 : rows <= 32 ? 32 : 64;
 }
 
 int grid_ctas(const TreeArgs& a, int sms) {
-  const int nr = unit_rows(a);
-  const long long units = (long long)a.n_trees * a.c.heads * ((a.max_nodes * a.group + nr - 1) / nr);
-  return (int)std::min<long long>(sms, units * ((a.max_len + kTilePos - 1) / kTilePos));
+  return (int)std::min<long long>(sms, tiles_of(a, unit_rows(a, sms)));
 }
 
 template <int HD, int DT, int NR>
@@ -1337,7 +1367,7 @@ cudaError_t launch(const TreeArgs& a, int sms, cudaStream_t st) {
 
 template <int HD, int DT>
 cudaError_t launch_rows(const TreeArgs& a, int sms, cudaStream_t st) {
-  switch (unit_rows(a)) {
+  switch (unit_rows(a, sms)) {
     case 16: return launch<HD, DT, 16>(a, sms, st);
     case 32: return launch<HD, DT, 32>(a, sms, st);
     default: return launch<HD, DT, 64>(a, sms, st);
@@ -1348,7 +1378,7 @@ cudaError_t launch_rows(const TreeArgs& a, int sms, cudaStream_t st) {
 
 size_t tree_attention_workspace_bytes(const TreeArgs& a, int hd, int sms) {
   if (a.n_trees == 0 || a.n_nodes == 0) return 0;
-  const size_t nr = unit_rows(a);
+  const size_t nr = unit_rows(a, sms);
   return (size_t)grid_ctas(a, sms) * (sizeof(TaDesc) + 2 * 4 * (2 * nr + nr * hd)) + 16;
 }
 

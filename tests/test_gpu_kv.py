@@ -732,6 +732,46 @@ def test_starts_at_the_ends_of_int32_are_skipped(lrs, backend):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_padded_batch(lrs, backend, dtype):
+    """Trees without nodes may hold anything; the others are right and nothing is reported."""
+    s = [(0, 0), (70, 3), (9, 0), (130, 1), (0, 0)]
+    cache = Cache(lrs, dtype, 2, 64, [c + n for c, n in reversed(s)])
+    trees = Trees(lrs, backend, cache, s, 3, max_nodes=3, max_len=140)
+    for i, (slot, ctx) in zip((0, 2, 4), ((-1, -7), (99, 2 ** 31 - 1), (0, 141))):
+        trees.d["seq"][i], trees.d["ctx"][i] = slot, ctx
+    trees.run(backend)
+    sync_ok(backend)
+    trees.check()
+    d = [dev([-1, 3, 99], np.int32), dev([-5, 60, 2 ** 31 - 1], np.int32), dev([0, 0, 1, 1], np.int32), dev([2], np.int32)]
+    backend.kv_accept(cache.c, *(x.data_ptr() for x in d), 3, 1, stream=LEGACY)
+    sync_ok(backend)
+    for got, want in zip(cache.bytes_now(), accepted(cache, [60], [[2]], [3])):
+        assert np.array_equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("max_len", [200, 3000, 40000])
+def test_rows_by_the_batchs_bounds(lrs, backend, dtype, max_len):
+    """The same trees under bounds that choose units of 16 and of 64 rows."""
+    s = [(150, 9), (90, 30), (3, 5)]
+    cache = Cache(lrs, dtype, 2, 64, [c + n for c, n in reversed(s)], extra=640)
+    trees = Trees(lrs, backend, cache, s, 7, max_len=max_len)
+    trees.run(backend)
+    sync_ok(backend)
+    trees.check()
+
+
+@pytest.mark.parametrize("dtype", ["BF16", "Q8_0"])
+def test_more_trees_than_threads(lrs, backend, dtype):
+    s = [(i * 7 % 60, i % 3) for i in range(2500)]
+    cache = Cache(lrs, dtype, 1, 64, [c + n for c, n in reversed(s)])
+    trees = Trees(lrs, backend, cache, s, 4)
+    trees.run(backend)
+    sync_ok(backend)
+    trees.check()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_out_may_be_q(lrs, backend, dtype):
     s = [(700, 9), (5, 2), (0, 1), (1500, 20)]
     cache = Cache(lrs, dtype, 2, 128, [c + n for c, n in reversed(s)])
