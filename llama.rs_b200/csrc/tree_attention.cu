@@ -14,7 +14,7 @@
 // the cache there (a lane is a position of K, a column of V), so a tile passes
 // shared memory once, as raw cache bytes.
 //
-// A CTA is a pipeline of roles (TaShape): a copy warp brings a tile's raw pages in by
+// A CTA is a pipeline of roles (TaShape): two copy warps bring a tile's raw pages in by
 // bulk copies; four warps decode K, four (eight) V; the softmax has a group of four
 // warps per 16 rows, a lane being a position, so that a row's statistics need the
 // other lanes only when its maximum moves; four warps keep the sums of O, a lane being
@@ -82,10 +82,10 @@ struct TaShape {
   // Groups of four warps: K, V (up to 32 rows two, half of the positions each: a decode
   // step of 64 sequences 41 us, with one 45; at 64 rows the threads are spent), the
   // softmax (16 rows each: groups of 32 took the same time at 64 rows, and would be half
-  // idle below), O; then a warp for the copies and one for the MMAs.
+  // idle below), O; then a warp each for K's copies, V's and the MMAs.
   static constexpr int kSG = NR / 16, kVG = NR == 64 ? 1 : 2;
   static constexpr int kWarpV = 4, kWarpS = kWarpV + 4 * kVG, kWarpO = kWarpS + 4 * kSG;
-  static constexpr int kWarpCopy = kWarpO + 4, kWarpMma = kWarpCopy + 1;
+  static constexpr int kWarpCopyK = kWarpO + 4, kWarpCopyV = kWarpCopyK + 1, kWarpMma = kWarpCopyV + 1;
   static constexpr int kThreads = 32 * (kWarpMma + 1);
   // Registers a thread: at launch, K and V, the softmax, O (increases beyond what
   // the others gave would wait for good).
@@ -135,7 +135,7 @@ struct TaShape {
 // A unit: the rows of one (tree, KV head, chunk of rows) and its tiles here.
 struct TaUnit {
   int t0, t1, tiles;  // tiles t0..t1 of `tiles`; t1 = 0 ends the list
-  int ctx, len, s, n, kvh, row0, rows;
+  int ctx, len, s, n, kvh, row0, rows, seq;
 };
 constexpr int kUnits = 4;  // units announced ahead
 
@@ -683,6 +683,64 @@ __device__ __forceinline__ void load_q(const TreeArgs& a, const TaUnit& it, uint
   }
 }
 
+// The copies of K's or V's raw tiles into their ring, by one warp each: they take
+// turns of some 100 instructions a slot, at a pace of 10 clocks and more beside the other
+// warps (one warp for both was what f32 caches waited for: 8 trees of 13 nodes on 1,550 to 2,050
+// positions took 54 us, now 43).
+template <int HD, int DT, int NR, bool V>
+struct TaCopy {
+  using S = TaShape<HD, DT, NR>;
+  static constexpr int kRing = V ? S::kRingV : S::kRingK, kSlot = V ? S::kSlotV : S::kSlotK;
+  static constexpr int kPart = S::kTileB / (kPageSize / S::kSlotPos);  // bytes of a slot's rows
+  uint64_t pol = evict_first_policy();
+  uint32_t issued = 0;
+  TaRing<kRing> ring;
+  // The tiles of a unit; false if a wait gave up.
+  __device__ __forceinline__ bool unit(const TreeArgs& a, TaShared& sh, uint8_t* smem, const TaUnit& un, int lane) {
+    const uint8_t* pool = (V ? a.c.v : a.c.k) + (size_t)un.kvh * S::kTileB;
+    const size_t page_bytes = (size_t)a.c.heads * S::kTileB;
+    const int used = (un.len + kPageSize - 1) / kPageSize;  // the slot's pages that hold positions
+    int ids = -1;                                           // a lane holds one of 32 pages
+    const int first = un.t0 * S::kSlots, end = un.t1 * S::kSlots;
+#pragma unroll 1
+    for (int k = first; k < end; k++) {  // slots of kSlotPos positions
+      const int pg = k * S::kSlotPos / kPageSize, at32 = (pg - first * S::kSlotPos / kPageSize) & 31;
+      if (at32 == 0 && k * S::kSlotPos % kPageSize == 0)
+        ids = pg + lane < used ? kv_page(a.c, un.seq, (pg + lane) * kPageSize) : -1;
+      const int page = __shfl_sync(0xffffffffu, ids, at32);
+      const uint32_t at = ring.at;
+      uint64_t* full = V ? &sh.v_full[at] : &sh.k_full[at];
+      if (issued >= (uint32_t)kRing && !ta_wait(sh, V ? &sh.v_empty[at] : &sh.k_empty[at], ring.parity ^ 1)) return false;
+      ring.step();
+      issued++;
+      uint8_t* dst = smem + (V ? S::kOffV : S::kOffRing) + at * kSlot;
+      const uint8_t* src = pool + max(page, 0) * page_bytes + k * S::kSlotPos % kPageSize / S::kSlotPos * kPart;
+      if (page < 0) {
+        if (lane == 0) ta_arrive(full);
+      } else if (V || DT == LRS_KV_Q8_0) {
+        if (lane == 0) {
+          mbar_expect_tx(full, kPart);
+          tma_load_1d(dst, src, kPart, full, pol);
+        }
+      } else {
+        if (lane == 0) mbar_expect_tx(full, kPart);
+        __syncwarp();
+        constexpr int kRow = kPart / S::kSlotPos;
+        for (int r = lane; r < S::kSlotPos; r += 32) tma_load_1d(dst + r * S::kRowK, src + r * kRow, kRow, full, pol);
+      }
+    }
+    return true;
+  }
+  // Copies in flight land before shared memory goes away (they may outlive their
+  // readers only when a wait gave up).
+  __device__ __forceinline__ void land(TaShared& sh) {
+    for (uint32_t i = issued > kRing ? issued - kRing : 0; i < issued; i++)
+      for (uint32_t j = 0; j < kPolls && !ta_try_wait(smem_u32(V ? &sh.v_full[i % kRing] : &sh.k_full[i % kRing]),
+                                                       (i / kRing) & 1); j++) {
+      }
+  }
+};
+
 template <int HD, int DT, int NR>
 __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
     tree_attention_kernel(const __grid_constant__ TreeArgs a) {
@@ -718,7 +776,7 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
 #pragma unroll 1
     for (int i = 0; i < kUnits; i++) {
       mbar_init(&sh.unit_full[i], 1);
-      mbar_init(&sh.unit_empty[i], 4 + 4 * S::kSG + (S::kVG + 1) * kWarpsD + 1);  // the warps that take units
+      mbar_init(&sh.unit_empty[i], 4 + 4 * S::kSG + (S::kVG + 1) * kWarpsD + 2);  // the warps that take units
     }
     sh.abort = 0;
     fence_barrier_init();
@@ -1053,7 +1111,7 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
       if (lane == 0) ta_arrive(&sh.u_full[u]);
       ta_group_sync(bar);  // red is free again
     }
-  } else if (warp < S::kWarpCopy) {
+  } else if (warp < S::kWarpCopyK) {
     // ---- O: a lane is a column; sums of the tiles' products in registers ----
     ta_regs_inc<S::kRegsO>();
     const int w = warp - S::kWarpO, h = w * 32 + lane;
@@ -1117,12 +1175,9 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
       __syncwarp();
       if (lane == 0) ta_arrive(&sh.u_empty[u]);
     }
-  } else if (warp == S::kWarpCopy) {
-    // ---- copies: raw K and V tiles of the pages ----
-    const uint64_t pol = evict_first_policy();
-    uint32_t nk = 0, nv = 0;  // K and V slots issued
-    TaRing<S::kRingK> kr;
-    TaRing<S::kRingV> vr;
+  } else if (warp == S::kWarpCopyK) {
+    // ---- K's copies, and the list of units ----
+    TaCopy<HD, DT, NR, false> copy;
     TaRing<kUnits> list;
     TaTree tr;
     int tree = sh.tree, unit = sh.unit0, tile = sh.tile, left = sh.last - sh.first;
@@ -1140,7 +1195,7 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
       if (left > 0) {
         const int share = tr.share(a);
         un.t0 = tile, un.t1 = min(tr.tiles, tile + left), un.tiles = tr.tiles;
-        un.ctx = tr.ctx, un.len = tr.len, un.s = tr.s, un.n = tr.n;
+        un.ctx = tr.ctx, un.len = tr.len, un.s = tr.s, un.n = tr.n, un.seq = tr.seq;
         un.kvh = unit / tr.chunks;
         un.row0 = unit % tr.chunks * share;
         un.rows = min(share, tr.n * a.group - un.row0);
@@ -1156,67 +1211,14 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
       }
       list.step();
       if (un.t1 == 0) break;
-      const int used = (un.len + kPageSize - 1) / kPageSize;  // the slot's pages that hold positions
-      int from = -1, ids = -1;  // a lane holds page `from + lane`
-#pragma unroll 1
-      for (int t = un.t0; t < un.t1 && ok; t++) {
-#pragma unroll 1
-        for (int k = 0; k < S::kSlots && ok; k++) {
-          const uint32_t ks = kr.at, vs = vr.at;
-          const int p = t * kTilePos + k * S::kSlotPos;
-          if (from < 0 || p / kPageSize >= from + 32) {
-            from = p / kPageSize;
-            ids = from + lane < used ? kv_page(a.c, tr.seq, (from + lane) * kPageSize) : -1;
-          }
-          const int page = __shfl_sync(0xffffffffu, ids, p / kPageSize - from);
-          const size_t off = ((size_t)max(page, 0) * a.c.heads + un.kvh) * S::kTileB;
-          uint8_t* kd = smem + S::kOffRing + ks * S::kSlotK;
-          uint8_t* vd = smem + S::kOffV + vs * S::kSlotV;
-          constexpr int kPart = S::kTileB / (kPageSize / S::kSlotPos);  // bytes of the slot's rows
-          const size_t part = off + (size_t)(p % kPageSize / S::kSlotPos) * kPart;
-          if (nk >= S::kRingK) ok = ta_wait(sh, &sh.k_empty[ks], kr.parity ^ 1);
-          kr.step();
-          if (!ok) break;
-          if (page < 0) {
-            if (lane == 0) ta_arrive(&sh.k_full[ks]);
-          } else {
-            if (lane == 0) mbar_expect_tx(&sh.k_full[ks], kPart);
-            __syncwarp();
-            if constexpr (DT == LRS_KV_Q8_0) {
-              if (lane == 0) tma_load_1d(kd, a.c.k + part, kPart, &sh.k_full[ks], pol);
-            } else {
-              constexpr int kRow = kPart / S::kSlotPos;
-              for (int r = lane; r < S::kSlotPos; r += 32)
-                tma_load_1d(kd + r * S::kRowK, a.c.k + part + (size_t)r * kRow, kRow, &sh.k_full[ks], pol);
-            }
-          }
-          nk++;
-          if (nv >= S::kRingV) ok = ta_wait(sh, &sh.v_empty[vs], vr.parity ^ 1);
-          vr.step();
-          if (!ok) break;
-          if (lane == 0) {
-            if (page < 0) {
-              ta_arrive(&sh.v_full[vs]);
-            } else {
-              mbar_expect_tx(&sh.v_full[vs], kPart);
-              tma_load_1d(vd, a.c.v + part, kPart, &sh.v_full[vs], pol);
-            }
-          }
-          nv++;
-        }
-      }
+      ok = copy.unit(a, sh, smem, un, lane);
     }
-    // copies in flight land before shared memory goes away (they may outlive
-    // their readers only when a wait gave up)
-    if (!ok) {
-      auto land = [&](uint64_t* full, uint32_t ring, uint32_t issued) {
-        for (uint32_t i = issued > ring ? issued - ring : 0; i < issued; i++)
-          for (uint32_t j = 0; j < kPolls && !ta_try_wait(smem_u32(&full[i % ring]), (i / ring) & 1); j++) {
-          }
-      };
-      land(sh.k_full, S::kRingK, nk);
-      land(sh.v_full, S::kRingV, nv);
-    }
+    if (!ok) copy.land(sh);
+  } else if (warp == S::kWarpCopyV) {
+    // ---- V's copies ----
+    TaCopy<HD, DT, NR, true> copy;
+    while (ok && feed.next(sh, lane, ok)) ok = copy.unit(a, sh, smem, it, lane);
+    if (!ok) copy.land(sh);
   } else {
     // ---- MMAs ----
     const uint32_t el = ta_elect();
