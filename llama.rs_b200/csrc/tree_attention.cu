@@ -41,15 +41,15 @@
 // rescaling of O run only in the tiles that raise it (the first one, mostly).
 //
 // What bounds it.  64 trees of 8 nodes on 2,100 to 4,100 positions, q8_0, 4 KV heads
-// of 7 queries, 128 wide: 118 us, 1.97 TB/s of the cache's bytes and 0.51 PFLOP/s of the
-// three products; 4 trees of 64 nodes on 7,200 to 8,200: 118 us, 0.72 PFLOP/s.  A tile takes some
-// 3,000 clocks, of which the tensor pipe needs 1,536 and the copies, at DRAM's rate,
-// 1,476; the schedulers issue in 64 of 100 clocks.  So the bound is the
-// instructions of decoding (of the values K and V's terms take 2.3 each) and of the
-// softmax, and next to it the chain of one tile's softmax (some 2,500 clocks).  A CTA
-// spends some 15,000 clocks before its first product (the schedule, cold instruction
-// fetches, q) and after its last one: small calls are that and the launches (5 nodes on
-// 100 positions: 15.4 us, two launches' 5 us among them).
+// of 7 queries, 128 wide: 114 us, 2.0 TB/s of the cache's bytes and 0.53 PFLOP/s of the
+// three products; 4 trees of 64 nodes on 7,200 to 8,200: 113 us, 0.75 PFLOP/s.  A tile
+// takes some 3,000 clocks, of which the tensor pipe needs 1,536 and the copies, at DRAM's
+// rate, 1,476; the schedulers issue in 65 of 100 clocks.  So the bound is the instructions
+// of decoding (a lane's 128 values of K or V take some 450) and of the softmax, whose
+// warps make 8 to 12 clocks an instruction beside one another.  A CTA spends some 15,000
+// clocks before its first product (the schedule, cold instruction fetches, q) and after
+// its last one: small calls are that and the launch (5 nodes on 100 positions, bf16, 12.3
+// us; a decode step of 64 sequences at 700 to 1,100, q8_0, 35 us).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
