@@ -356,12 +356,12 @@ typedef struct lrs_tree_batch {
  * infinite; a non-finite value that it does attend to makes its outputs
  * non-finite (all of the row's, if the value belongs to another node).
  * `d_workspace` (16-byte aligned, lrs_tree_attention_workspace bytes, contents
- * free) is in use until the work has finished: calls that may overlap, and
- * graphs that may run at once, need one each.  out may be q (then q_ld =
- * out_ld).  A tree whose slot, node range or length is out of range is skipped,
- * its rows left as they were; the rows of one that reaches a page out of range
- * hold no defined values.  Of a tree without nodes nothing
- * else is looked at (padded batches). */
+ * free; a batch with no field above another's needs no more than that one) is in
+ * use until the work has finished: calls that may overlap, and graphs that may
+ * run at once, need one each.  out may be q (then q_ld = out_ld).  A tree whose
+ * slot, node range or length is out of range is skipped, its rows left as they
+ * were; the rows of one that reaches a page out of range hold no defined values.
+ * Of a tree without nodes nothing else is looked at (padded batches). */
 lrs_status lrs_tree_attention_workspace(const lrs_backend* backend, const lrs_kv_cache* cache,
                                         const lrs_tree_batch* trees, uint32_t n_heads,
                                         size_t* bytes);

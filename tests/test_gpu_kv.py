@@ -771,6 +771,20 @@ def test_more_trees_than_threads(lrs, backend, dtype):
     trees.check()
 
 
+def test_workspace_of_a_smaller_batch_is_no_larger(lrs, backend):
+    rng = np.random.default_rng(11)
+    cache = lrs.KvCache(4096, 8192, 4096, 64, 64, 4096, 2, 64, 2)
+
+    def size(trees, nodes, length, heads):
+        return backend.tree_attention_workspace(cache, lrs.TreeBatch(4096, 4096, 4096, None, trees, trees * nodes, nodes,
+                                                                     length), 2 * heads)
+    for _ in range(4000):
+        big = [int(np.exp(rng.uniform(0, np.log(m + 0.99)))) for m in (300, 64, 9000)]
+        small = [int(rng.integers(1, b + 1)) for b in big]
+        heads = int(rng.integers(1, 9))
+        assert size(*small, heads) <= size(*big, heads), (big, small, heads)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_out_may_be_q(lrs, backend, dtype):
     s = [(700, 9), (5, 2), (0, 1), (1500, 20)]
