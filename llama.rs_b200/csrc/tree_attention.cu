@@ -1084,6 +1084,9 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
         __syncwarp();
         if (lane == 0) ta_arrive(&sh.pv_go[tile & 1]);
       }
+      // (the sums take the place of the last tile's shifts, which the other warps may
+      // still be reading where it moved a maximum)
+      ta_group_sync(bar);
       // the rows' sums over the lanes: 16 rows by 32 lanes to a row a lane pair
       float* lf = reinterpret_cast<float*>(l);
       int row = 0;
