@@ -353,8 +353,10 @@ typedef struct lrs_tree_batch {
  * (q_ld, out_ld floats apart, 0 = packed), q already rotated.  A node that
  * attends to nothing gets zeros; rows from start[n_trees] on are left as they
  * were.  What a node's mask leaves out does not reach its output, be it NaN or
- * infinite; a non-finite value that it does attend to makes its outputs
- * non-finite (all of the row's, if the value belongs to another node).
+ * infinite; a non-finite value that it does attend to, or that q holds, makes its
+ * outputs non-finite (all of the row's, if the value belongs to another node),
+ * but that an infinity in K may count as the score of -inf that it makes, a weight
+ * of zero; scores that are all -inf give NaN.
  * `d_workspace` (16-byte aligned, lrs_tree_attention_workspace bytes, contents
  * free; a batch with no field above another's needs no more than that one) is in
  * use until the work has finished: calls that may overlap, and graphs that may

@@ -403,7 +403,7 @@ struct TaTree {
   __device__ __forceinline__ int total(const TreeArgs& a) const { return tiles * chunks * a.c.heads; }
 };
 
-// Partial results: [2 * CTAs] segments of [kMaxRows] (m, l) and [NR][HD] sums.
+// Partial results: [2 * CTAs] segments of [NR] (m, l) and [NR][HD] sums.
 struct TaDesc {
   int nseg;  // segments of the unit whose second one starts this CTA; 0 = none
   int kvh, row0, rows, s;
@@ -1107,7 +1107,9 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
       ta_group_sync(bar);
       if (gt < 16) {
         const float sum = (sh.red[grp][0][gt] + sh.red[grp][1][gt]) + (sh.red[grp][2][gt] + sh.red[grp][3][gt]);
-        sh.fin[u][my] = !whole ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+        // zeros for a row that sees nothing; one whose scores are all -inf or NaN gets NaN
+        const bool nothing = it.ctx == 0 && sh.mask[u][my] == 0;
+        sh.fin[u][my] = !whole ? 1.0f : nothing ? 0.0f : 1.0f / sum;
         if (!whole && my < it.rows) seg[2 * my] = sh.top[my], seg[2 * my + 1] = sum;
       }
       __syncwarp();
@@ -1300,7 +1302,10 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
 }
 
 // Merges the segments of the units that several CTAs share: block (c, y) rows
-// 4 y .. 4 y + 3 of the unit that CTA c is the second one of.
+// 4 y .. 4 y + 3 of the unit that CTA c is the second one of.  A segment in which a row
+// has no maximum (kUnset) saw nothing of the row's, or scores that are all -inf or NaN: its
+// sums are 0 or NaN, and are added like the others', so that NaN stays.  Units of several
+// tiles have committed positions, so that no row here sees nothing at all.
 template <int HD, int NR>
 __global__ void __launch_bounds__(HD * 4) tree_combine_kernel(const __grid_constant__ TreeArgs a, int ctas) {
   pdl_wait();
@@ -1312,19 +1317,18 @@ __global__ void __launch_bounds__(HD * 4) tree_combine_kernel(const __grid_const
   // the first segment ends CTA c - 1, the others start CTAs c, c + 1, ...
   const float* first = segs + (2 * (size_t)(c - 1) + 1) * kSeg;
   const float* next = segs + 2 * (size_t)c * kSeg;
-  float m = first[2 * r], l = m == kUnset ? 0.0f : first[2 * r + 1], o = m == kUnset ? 0.0f : first[2 * NR + r * HD + h];
+  float m = first[2 * r], l = first[2 * r + 1], o = first[2 * NR + r * HD + h];
 #pragma unroll 4
   for (int i = 1; i < d.nseg; i++, next += 2 * kSeg) {
     const float mi = next[2 * r], li = next[2 * r + 1], oi = next[2 * NR + r * HD + h];
-    if (mi == kUnset) continue;
-    const float top = fmaxf(m, mi), f = m == kUnset ? 0.0f : exp2f(m - top), g = exp2f(mi - top);
+    const float top = fmaxf(m, mi), f = exp2f(m - top), g = exp2f(mi - top);
     l = l * f + li * g;
     o = o * f + oi * g;
     m = top;
   }
   const int row = d.row0 + r;
   a.out[(size_t)(d.s + row / a.group) * a.out_ld + ((size_t)d.kvh * a.group + row % a.group) * HD + h] =
-      l == 0.0f ? 0.0f : o / l;
+      o / l;
 }
 
 long long tiles_of(const TreeArgs& a, int nr) {

@@ -3,7 +3,8 @@ are not finite, what is reported where."""
 import numpy as np
 import pytest
 
-from test_gpu_kv import DTYPES, Cache, Trees, sync_ok
+import kv_plain
+from test_gpu_kv import DTYPES, Cache, Trees, dev, sync_ok
 
 pytestmark = pytest.mark.gpu
 
@@ -26,3 +27,94 @@ def test_units_of_one_tile(lrs, backend, dtype, group, nodes):
         trees.run(backend)
         sync_ok(backend)
         assert torch.equal(first, trees.out)
+
+
+# ------------------------------------------------- values that are not finite --
+BITS = {"nan": {"F32": 0x7fc00000, "BF16": 0x7fc0, "Q8_0": 0x7e00}, "inf": {"F32": 0x7f800000, "BF16": 0x7f80, "Q8_0": 0x7c00},
+        "-inf": {"F32": 0xff800000, "BF16": 0xff80, "Q8_0": 0xfc00}}
+
+
+def poison(cache, dtype, which, slot, pos, head, col, what):
+    """One value of the cache (of q8_0: the scale of its block) becomes NaN or infinite."""
+    import torch
+    hd, bits = cache.hd, BITS[what][dtype]
+    tile = cache.pool[which][int(cache.pages[slot, pos // 64]), head]
+    r, signed = pos % 64, bits - (1 << 32 if dtype == "F32" else 1 << 16) if bits >> (31 if dtype == "F32" else 15) else bits
+    if dtype == "Q8_0":
+        at = 64 * hd + 2 * (col // 32 * 64 + r if which else r * (hd // 32) + col // 32)
+        tile[at:at + 2].view(torch.int16).fill_(signed)
+    else:
+        tile.view(torch.int16 if dtype == "BF16" else torch.int32)[r * hd + col] = signed
+
+
+def check_rows(trees, bad, part=()):
+    """Rows (tree, node, head) of `bad` hold no finite value, those of `part` some that are
+    not; all others are within their bounds."""
+    got = trees.out.cpu().numpy()[:trees.rows * trees.out_ld].reshape(trees.rows, trees.nh, -1)
+    for t, (ctx, n) in enumerate(trees.sizes):
+        k, v = (trees.cache.rows_of(trees.slots[t], ctx + n, i) for i in range(2))
+        q = np.nan_to_num(trees.q(t), nan=0.0, posinf=0.0, neginf=0.0)
+        want, err = kv_plain.attention(q, k, v, ctx, trees.masks[t], trees.scale)
+        for i in range(n):
+            for h in range(trees.nh):
+                row = got[trees.start[t] + i, h]
+                if (t, i, h) in bad:
+                    assert not np.isfinite(row).any(), (t, i, h)
+                elif (t, i, h) in part:
+                    assert not np.isfinite(row).all(), (t, i, h)
+                else:
+                    assert (np.abs(row - want[i, h]) <= err[i, h]).all(), (t, i, h)
+
+
+@pytest.mark.parametrize("what", ["nan", "inf", "-inf"])
+@pytest.mark.parametrize("ctx", [0, 70, 4000])  # a unit of one tile, a unit shared by CTAs
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_queries_that_are_not_finite(lrs, backend, dtype, ctx, what):
+    s = [(ctx, 3), (5, 2)]
+    cache = Cache(lrs, dtype, 2, 128, [c + n for c, n in reversed(s)])
+    trees = Trees(lrs, backend, cache, s, 3)
+    node, head, value = 1, 4, {"nan": np.nan, "inf": np.inf, "-inf": -np.inf}[what]
+    trees.qbuf[node * trees.q_ld + head * 128 + 17] = value
+    trees.d["q"].copy_(dev(trees.qbuf))
+    trees.run(backend)
+    sync_ok(backend)
+    check_rows(trees, {(0, node, head)})
+
+
+@pytest.mark.parametrize("pos", [0, 129, 3967, 3968])  # the last is the one position of the last tile, a node
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_cached_values_that_are_not_finite(lrs, backend, dtype, which, pos):
+    """A NaN that a row attends to shows, wherever the split of a long context puts it."""
+    s = [(3968, 1)]
+    cache = Cache(lrs, dtype, 2, 128, [3969])
+    trees = Trees(lrs, backend, cache, s, 3)
+    poison(cache, dtype, which, 0, pos, 1, 40, "nan")
+    trees.run(backend)
+    sync_ok(backend)
+    rows = {(0, 0, h) for h in (3, 4, 5)}
+    check_rows(trees, rows if which == 0 else (), rows)
+
+
+@pytest.mark.parametrize("ctx", [0, 100, 4000])
+def test_scores_of_minus_infinity(lrs, backend, ctx):
+    """bf16 K of -inf against a q whose three terms are positive: the weight is zero, and
+    NaN is the result where no other score is left."""
+    n = 3
+    cache = Cache(lrs, "BF16", 1, 64, [ctx + n])
+    trees = Trees(lrs, backend, cache, [(ctx, n)], 2, masks="chain")
+    trees.qbuf[:] = 0.0
+    trees.qbuf[0::64] = 1.0 + 2.0 ** -9 + 2.0 ** -18  # column 0 of every row, three terms of one sign
+    trees.scale = float(np.float32(np.log(2.0)))
+    assert np.float32(trees.scale) * np.float32(1.44269504088896) == 1.0
+    trees.d["q"].copy_(dev(trees.qbuf))
+    for p in range(ctx + n):
+        if p != ctx + 1:  # node 1 keeps its score
+            poison(cache, "BF16", 0, 0, p, 0, 0, "-inf")
+    trees.run(backend)
+    sync_ok(backend)
+    got = trees.out.cpu().numpy()[:n * 128].reshape(n, 2, 64)
+    assert np.isnan(got[0]).all()
+    v = cache.rows_of(0, ctx + n, 1)[0, ctx + 1]
+    # one weight over itself: three sums that may truncate (2^-23), an inverse and a product (2^-24)
+    assert (np.abs(got[1:] - v) <= 2.0 ** -21 * np.abs(v)).all()
