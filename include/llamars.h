@@ -297,7 +297,8 @@ uint32_t lrs_model_step_kernels(const lrs_model* model);
  * lengths) is checked on the device: an entry out of range is skipped, nothing
  * outside the pools and arrays is read or written, and the next
  * lrs_backend_synchronize (after the work has finished) returns
- * LRS_ERR_INVALID. */
+ * LRS_ERR_INVALID.  Matvecs and model calls do not: they report their own work's
+ * errors only. */
 #define LRS_KV_PAGE 64
 #define LRS_TREE_MAX_NODES 64
 

@@ -95,11 +95,15 @@ const NcclApi& nccl() {
       return fail(LRS_ERR_CUDA, std::string("NCCL: ") + nccl().GetErrorString(r_));        \
   } while (0)
 
-int32_t check_device_error(lrs_backend* be) {
+// What one of the backend's error words holds, which is clear then.
+int32_t check_device_error(lrs_backend* be, int word = kErrOwn) {
   int h = 0;
-  LRS_CUDA(cudaMemcpy(&h, be->d_err, sizeof(int), cudaMemcpyDeviceToHost));
+  LRS_CUDA(cudaMemcpy(&h, be->d_err + word, sizeof(int), cudaMemcpyDeviceToHost));
   if (h) {
-    cudaMemset(be->d_err, 0, sizeof(int));
+    LRS_CUDA(launch_take_error(be->d_err + word, be->d_err + kErrTaken, be->stream));
+    LRS_CUDA(cudaMemcpyAsync(&h, be->d_err + kErrTaken, sizeof(int), cudaMemcpyDeviceToHost, be->stream));
+    LRS_CUDA(cudaStreamSynchronize(be->stream));
+    if (h == 0) return LRS_OK;  // another thread's call has reported it
     if (h == kErrCacheIndex)
       return fail(LRS_ERR_INVALID,
                   "a KV cache operator skipped a slot, position, page, node or length out of range");
@@ -214,11 +218,12 @@ lrs_status lrs_backend_create(int device, lrs_backend** out) try {
   be->device = device;
   be->sms = prop.multiProcessorCount;
   if (cudaStreamCreateWithFlags(&be->stream, cudaStreamNonBlocking) != cudaSuccess ||
-      cudaMalloc(&be->d_err, sizeof(int)) != cudaSuccess) {
+      cudaMalloc(&be->d_err, kErrWords * sizeof(int)) != cudaSuccess) {
     delete be;
     return fail(LRS_ERR_CUDA, "stream / flag allocation failed");
   }
-  cudaMemset(be->d_err, 0, sizeof(int));
+  cudaMemsetAsync(be->d_err, 0, kErrWords * sizeof(int), be->stream);
+  cudaStreamSynchronize(be->stream);  // callers' streams do not wait for it
   *out = be;
   return LRS_OK;
 } catch (...) {
@@ -246,7 +251,8 @@ lrs_status lrs_backend_synchronize(lrs_backend* be) try {
   if (!be) return fail(LRS_ERR_INVALID, "null backend");
   LRS_CUDA(cudaSetDevice(be->device));
   LRS_CUDA(cudaStreamSynchronize(be->stream));
-  return check_device_error(be);
+  int32_t rc = check_device_error(be);
+  return rc ? rc : check_device_error(be, kErrQueued);
 } catch (...) {
   return lrs::status_of_current_exception();
 }
@@ -1677,8 +1683,8 @@ lrs_status lrs_model_accept_tree(lrs_model* m, uint32_t seq, uint32_t start_pos,
     c.head_dim = m->c.head_dim;
     c.kv_dtype = m->opt.kv_dtype;
   }
-  int32_t rc = lrs_kv_accept(m->be, caches.data(), caches.size(), m->d_seq, m->d_ctx, m->d_span, m->d_nodes, 1,
-                             n, nullptr);
+  int32_t rc = kv_accept(m->be, caches.data(), caches.size(), m->d_seq, m->d_ctx, m->d_span, m->d_nodes, 1, n,
+                         kErrOwn, st);
   if (rc) return rc;
   LRS_CUDA(cudaStreamSynchronize(st));
   return check_device_error(m->be);
@@ -1859,7 +1865,11 @@ lrs_status lrs_model_decode_greedy(lrs_model* m, size_t n_seqs, const uint32_t* 
                                    size_t n_steps, uint32_t* tokens_out) try {
   int32_t rc = lrs_model_decode_enqueue(m, n_seqs, seqs, first_tokens, start_pos, n_steps);
   if (rc) return rc;
-  if (!tokens_out || n_steps == 0) return lrs_backend_synchronize(m->be);
+  if (!tokens_out || n_steps == 0) {
+    LRS_CUDA(cudaSetDevice(m->be->device));
+    LRS_CUDA(cudaStreamSynchronize(m->be->stream));
+    return check_device_error(m->be);
+  }
   return lrs_model_read_tokens(m, n_seqs, n_steps, tokens_out);
 } catch (...) {
   return lrs::status_of_current_exception();

@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_split_kernel(const __grid_c
       for (int i = 0; i < ntiles; i++) {
         const int st = i % sp.stages;
         if (i >= sp.stages && !mbar_wait_bounded(&empty[st], ((i / sp.stages) - 1) & 1)) {
-          atomicExch(a.err, 1);
+          atomicExch(a.err, LRS_ERR_DEVICE_TIMEOUT);
           break;
         }
         const size_t off = kv_offset(a.io, b, s0 + kTile * i, nkv, kvh, HD) * ESZ;
@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_split_kernel(const __grid_c
       // stay until the last copies have landed (they may outlive the consumers
       // on an error exit)
       for (int i = max(0, ntiles - sp.stages); i < ntiles; i++)
-        if (!mbar_wait_bounded(&full[i % sp.stages], (i / sp.stages) & 1)) atomicExch(a.err, 1);
+        if (!mbar_wait_bounded(&full[i % sp.stages], (i / sp.stages) & 1)) atomicExch(a.err, LRS_ERR_DEVICE_TIMEOUT);
     }
     return;
   }
@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_split_kernel(const __grid_c
       }
     }
     if (attn_consumer_sync_or(!got)) {  // a copy never landed: every consumer leaves
-      if (tid == 0) atomicExch(a.err, 1);
+      if (tid == 0) atomicExch(a.err, LRS_ERR_DEVICE_TIMEOUT);
       ok = false;
       break;
     }
@@ -595,6 +595,10 @@ __global__ void __launch_bounds__(HD) attn_combine_kernel(const float* part, con
   att[((size_t)b * nh + h) * HD + d] = O / Lsum;
 }
 
+// An error word is read and cleared in one: what a kernel on another stream sets
+// meanwhile is either taken here or still there.
+__global__ void take_error_kernel(int* word, int* taken) { *taken = atomicExch(word, 0); }
+
 __global__ void advance_kernel(const unsigned long long* keys, int* tok, int* pos, int batch,
                                int* step, int n_steps, uint32_t* tokens_out, uint32_t* last) {
   const int s = *step;
@@ -619,6 +623,11 @@ cudaError_t launch_embed(const uint8_t* w, uint32_t type, int cols, const int* r
 cudaError_t launch_dequant_rows(const uint8_t* w, uint32_t type, int cols, int row0, int n,
                                 float* out, cudaStream_t st) {
   return embed_dispatch(w, type, cols, nullptr, row0, n, out, nullptr, st);
+}
+
+cudaError_t launch_take_error(int* word, int* taken, cudaStream_t st) {
+  take_error_kernel<<<1, 1, 0, st>>>(word, taken);
+  return cudaGetLastError();
 }
 
 cudaError_t launch_rmsnorm(const float* x, const float* w, float eps, int n, int batch, float* out,

@@ -26,6 +26,8 @@ cudaError_t launch_embed(const uint8_t* w, uint32_t type, int cols, const int* r
 cudaError_t launch_dequant_rows(const uint8_t* w, uint32_t type, int cols, int row0, int n,
                                 float* out, cudaStream_t st);
 // out[b][i] = x[b][i] * (inv_rms_b * w[i])  (RMSNorm::forward, src/model.rs:65-73)
+// *taken = *word, and *word = 0, in one step.
+cudaError_t launch_take_error(int* word, int* taken, cudaStream_t st);
 cudaError_t launch_rmsnorm(const float* x, const float* w, float eps, int n, int batch, float* out,
                            cudaStream_t st);
 // RoPE on q and k (src/model.rs:86-95, table rows indexed by position) and

@@ -5,11 +5,16 @@
 #include <cstddef>
 #include <cstdint>
 
+// The backend's error words: what its own work left (matvecs, the sampler, the
+// models' steps), what the operators that callers queue left, and the place that a
+// word is taken to.
+enum { kErrOwn = 0, kErrQueued = 1, kErrTaken = 2, kErrWords = 3 };
+
 struct lrs_backend {
   int device = 0;
   int sms = 148;
   cudaStream_t stream = nullptr;
-  int* d_err = nullptr;
+  int* d_err = nullptr;  // [kErrWords]
   float* d_x = nullptr;
   float* d_y = nullptr;
   size_t x_cap = 0, y_cap = 0;

@@ -11,9 +11,11 @@ namespace lrs {
 
 static_assert(kPageSize == LRS_KV_PAGE, "one page size");
 
-// What the error word (lrs_backend::d_err) holds after a kernel skipped an
-// entry that names a slot, position, page or node out of range.
+// What an error word (lrs_backend::d_err) holds after a kernel skipped an entry
+// that names a slot, position, page or node out of range.  Below
+// LRS_ERR_DEVICE_TIMEOUT, which it must not replace: kernels set it by maximum.
 constexpr int kErrCacheIndex = 2;
+static_assert(kErrCacheIndex < LRS_ERR_DEVICE_TIMEOUT, "the graver error stays");
 
 // Largest magnitude of a Q8_0 cache: 512 * 127, so that d * code is a finite f16.
 constexpr float kQ8Limit = 65024.0f;
@@ -47,7 +49,7 @@ __device__ __forceinline__ int kv_page(const KvView& c, int seq, int pos) {
   if (seq >= 0 && seq < c.n_seqs && pos >= 0 && pos / kPageSize < c.max_pages)
     page = c.pages[(size_t)seq * c.max_pages + pos / kPageSize];
   if (page < 0 || page >= c.n_pages) {
-    atomicExch(c.err, kErrCacheIndex);
+    atomicMax(c.err, kErrCacheIndex);
     return -1;
   }
   return page;
@@ -75,6 +77,11 @@ struct KvLoadArgs {
   long long ld;
 };
 cudaError_t launch_kv_load(const KvLoadArgs& a, uint32_t dtype, int hd, int sms, cudaStream_t st);
+
+// lrs_kv_accept, which leaves a skipped tree's error in one of the backend's words.
+int32_t kv_accept(lrs_backend* be, const lrs_kv_cache* caches, size_t n_caches, const int32_t* d_seq,
+                  const int32_t* d_ctx, const int32_t* d_start, const int32_t* d_nodes, size_t n_trees,
+                  size_t n_nodes, int err_word, void* stream);
 
 struct TreeArgs {
   KvView c;

@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(128) kv_accept_kernel(const __grid_constant__ 
     }
   }
   if (!ok) {
-    if (lane == 0) atomicExch(a.c.err, kErrCacheIndex);
+    if (lane == 0) atomicMax(a.c.err, kErrCacheIndex);
     return;
   }
   uint8_t* pool = is_v ? a.v[cache] : a.k[cache];
@@ -583,6 +583,60 @@ TreeArgs tree_args(const lrs_kv_cache& c, const lrs_tree_batch& t, uint32_t n_he
 
 }  // namespace
 
+int32_t lrs::kv_accept(lrs_backend* be, const lrs_kv_cache* caches, size_t n_caches, const int32_t* d_seq,
+                       const int32_t* d_ctx, const int32_t* d_start, const int32_t* d_nodes, size_t n_trees,
+                       size_t n_nodes, int err_word, void* stream) {
+  if (n_caches && !caches) return fail(LRS_ERR_INVALID, "null cache");
+  int32_t rc;
+  for (size_t i = 0; i < n_caches; i++) {
+    if ((rc = lrs_kv_check(&caches[i], nullptr))) return rc;
+    const lrs_kv_cache &x = caches[i], &y = caches[0];
+    if (x.pages != y.pages || x.n_pages != y.n_pages || x.n_seqs != y.n_seqs ||
+        x.max_pages != y.max_pages || x.kv_heads != y.kv_heads || x.head_dim != y.head_dim ||
+        x.kv_dtype != y.kv_dtype)
+      return fail(LRS_ERR_INVALID, "lrs_kv_accept: the caches may differ in their pools only");
+  }
+  if (n_trees > (size_t)INT_MAX || n_nodes > (size_t)INT_MAX)
+    return fail(LRS_ERR_INVALID, "lrs_kv_accept: too many trees or nodes");
+  if (n_caches == 0 || n_trees == 0 || n_nodes == 0) return LRS_OK;
+  // a pool named twice would be compacted by two warps at once
+  for (size_t i = 0; i < n_caches; i++)
+    for (size_t j = 0; j <= i; j++)
+      if ((j < i && (caches[i].k_pool == caches[j].k_pool || caches[i].v_pool == caches[j].v_pool)) ||
+          caches[i].k_pool == caches[j].v_pool || caches[i].v_pool == caches[j].k_pool)
+        return fail(LRS_ERR_INVALID, "lrs_kv_accept: a pool is named twice");
+  if (!be || !d_seq || !d_ctx || !d_start || !d_nodes) return fail(LRS_ERR_INVALID, "null argument");
+  if (!aligned(d_seq) || !aligned(d_ctx) || !aligned(d_start) || !aligned(d_nodes)) return unaligned("lrs_kv_accept");
+  const size_t per_cache = n_trees * caches[0].kv_heads * 2;
+  if (per_cache > (size_t)INT_MAX) return fail(LRS_ERR_INVALID, "lrs_kv_accept: too many trees or nodes");
+  OnDevice on(be->device);
+  if (on.err != cudaSuccess) return cuda_status(on.err, "cudaSetDevice");
+  cudaStream_t st = stream ? (cudaStream_t)stream : be->stream;
+  const size_t most = std::max<size_t>(1, std::min<size_t>(kAcceptCaches, (size_t)INT_MAX / per_cache));
+  for (size_t c0 = 0; c0 < n_caches; c0 += most) {
+    AcceptArgs a{};
+    a.c = view_of(caches[0], be->d_err + err_word);
+    a.n_caches = (int)std::min(most, n_caches - c0);
+    for (int i = 0; i < a.n_caches; i++) {
+      a.k[i] = static_cast<uint8_t*>(caches[c0 + i].k_pool);
+      a.v[i] = static_cast<uint8_t*>(caches[c0 + i].v_pool);
+    }
+    a.seq = d_seq;
+    a.ctx = d_ctx;
+    a.start = d_start;
+    a.nodes = d_nodes;
+    a.n_trees = (int)n_trees;
+    a.n_nodes = (int)n_nodes;
+    const unsigned grid = (unsigned)((per_cache * a.n_caches + 3) / 4);
+#define LRS_CALL(HD, DT) kv_accept_kernel<HD, DT><<<grid, 128, 0, st>>>(a)
+    LRS_KV_DISPATCH(caches[0].head_dim, caches[0].kv_dtype, LRS_CALL);
+#undef LRS_CALL
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_status(e, "lrs_kv_accept");
+  }
+  return LRS_OK;
+}
+
 extern "C" {
 
 lrs_status lrs_kv_check(const lrs_kv_cache* c, size_t* tile_bytes) try {
@@ -617,7 +671,7 @@ lrs_status lrs_kv_store(lrs_backend* be, const lrs_kv_cache* c, const int32_t* d
   if (!aligned(d_seq) || !aligned(d_pos) || !aligned(d_k) || !aligned(d_v)) return unaligned("lrs_kv_store");
   OnDevice on(be->device);
   if (on.err != cudaSuccess) return cuda_status(on.err, "cudaSetDevice");
-  KvStoreArgs a{view_of(*c, be->d_err), d_seq, d_pos, (long long)n, d_k, d_v, (long long)ld};
+  KvStoreArgs a{view_of(*c, be->d_err + kErrQueued), d_seq, d_pos, (long long)n, d_k, d_v, (long long)ld};
   return cuda_status(launch_kv_store(a, c->kv_dtype, (int)c->head_dim, be->sms,
                                      stream ? (cudaStream_t)stream : be->stream),
                      "lrs_kv_store");
@@ -635,7 +689,7 @@ lrs_status lrs_kv_load(lrs_backend* be, const lrs_kv_cache* c, const int32_t* d_
   if (!aligned(d_seq) || !aligned(d_pos) || !aligned(d_k) || !aligned(d_v)) return unaligned("lrs_kv_load");
   OnDevice on(be->device);
   if (on.err != cudaSuccess) return cuda_status(on.err, "cudaSetDevice");
-  KvLoadArgs a{view_of(*c, be->d_err), d_seq, d_pos, (long long)n, d_k, d_v, (long long)ld};
+  KvLoadArgs a{view_of(*c, be->d_err + kErrQueued), d_seq, d_pos, (long long)n, d_k, d_v, (long long)ld};
   return cuda_status(launch_kv_load(a, c->kv_dtype, (int)c->head_dim, be->sms,
                                     stream ? (cudaStream_t)stream : be->stream),
                      "lrs_kv_load");
@@ -646,55 +700,8 @@ lrs_status lrs_kv_load(lrs_backend* be, const lrs_kv_cache* c, const int32_t* d_
 lrs_status lrs_kv_accept(lrs_backend* be, const lrs_kv_cache* caches, size_t n_caches,
                          const int32_t* d_seq, const int32_t* d_ctx, const int32_t* d_start,
                          const int32_t* d_nodes, size_t n_trees, size_t n_nodes, void* stream) try {
-  if (n_caches && !caches) return fail(LRS_ERR_INVALID, "null cache");
-  int32_t rc;
-  for (size_t i = 0; i < n_caches; i++) {
-    if ((rc = lrs_kv_check(&caches[i], nullptr))) return rc;
-    const lrs_kv_cache &x = caches[i], &y = caches[0];
-    if (x.pages != y.pages || x.n_pages != y.n_pages || x.n_seqs != y.n_seqs ||
-        x.max_pages != y.max_pages || x.kv_heads != y.kv_heads || x.head_dim != y.head_dim ||
-        x.kv_dtype != y.kv_dtype)
-      return fail(LRS_ERR_INVALID, "lrs_kv_accept: the caches may differ in their pools only");
-  }
-  if (n_trees > (size_t)INT_MAX || n_nodes > (size_t)INT_MAX)
-    return fail(LRS_ERR_INVALID, "lrs_kv_accept: too many trees or nodes");
-  if (n_caches == 0 || n_trees == 0 || n_nodes == 0) return LRS_OK;
-  // a pool named twice would be compacted by two warps at once
-  for (size_t i = 0; i < n_caches; i++)
-    for (size_t j = 0; j <= i; j++)
-      if ((j < i && (caches[i].k_pool == caches[j].k_pool || caches[i].v_pool == caches[j].v_pool)) ||
-          caches[i].k_pool == caches[j].v_pool || caches[i].v_pool == caches[j].k_pool)
-        return fail(LRS_ERR_INVALID, "lrs_kv_accept: a pool is named twice");
-  if (!be || !d_seq || !d_ctx || !d_start || !d_nodes) return fail(LRS_ERR_INVALID, "null argument");
-  if (!aligned(d_seq) || !aligned(d_ctx) || !aligned(d_start) || !aligned(d_nodes)) return unaligned("lrs_kv_accept");
-  const size_t per_cache = n_trees * caches[0].kv_heads * 2;
-  if (per_cache > (size_t)INT_MAX) return fail(LRS_ERR_INVALID, "lrs_kv_accept: too many trees or nodes");
-  OnDevice on(be->device);
-  if (on.err != cudaSuccess) return cuda_status(on.err, "cudaSetDevice");
-  cudaStream_t st = stream ? (cudaStream_t)stream : be->stream;
-  const size_t most = std::max<size_t>(1, std::min<size_t>(kAcceptCaches, (size_t)INT_MAX / per_cache));
-  for (size_t c0 = 0; c0 < n_caches; c0 += most) {
-    AcceptArgs a{};
-    a.c = view_of(caches[0], be->d_err);
-    a.n_caches = (int)std::min(most, n_caches - c0);
-    for (int i = 0; i < a.n_caches; i++) {
-      a.k[i] = static_cast<uint8_t*>(caches[c0 + i].k_pool);
-      a.v[i] = static_cast<uint8_t*>(caches[c0 + i].v_pool);
-    }
-    a.seq = d_seq;
-    a.ctx = d_ctx;
-    a.start = d_start;
-    a.nodes = d_nodes;
-    a.n_trees = (int)n_trees;
-    a.n_nodes = (int)n_nodes;
-    const unsigned grid = (unsigned)((per_cache * a.n_caches + 3) / 4);
-#define LRS_CALL(HD, DT) kv_accept_kernel<HD, DT><<<grid, 128, 0, st>>>(a)
-    LRS_KV_DISPATCH(caches[0].head_dim, caches[0].kv_dtype, LRS_CALL);
-#undef LRS_CALL
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return cuda_status(e, "lrs_kv_accept");
-  }
-  return LRS_OK;
+  return kv_accept(be, caches, n_caches, d_seq, d_ctx, d_start, d_nodes, n_trees, n_nodes,
+                   kErrQueued, stream);
 } catch (...) {
   return lrs::status_of_current_exception();
 }
@@ -726,7 +733,7 @@ lrs_status lrs_tree_attention(lrs_backend* be, const lrs_kv_cache* c, const lrs_
   if (t->n_trees == 0 || t->n_nodes == 0) return LRS_OK;
   if (!be || !d_q || !d_out) return fail(LRS_ERR_INVALID, "null argument");
   if (!aligned(d_q) || !aligned(d_out)) return unaligned("lrs_tree_attention");
-  TreeArgs a = tree_args(*c, *t, n_heads, be->d_err);
+  TreeArgs a = tree_args(*c, *t, n_heads, be->d_err + kErrQueued);
   const size_t need = tree_attention_workspace_bytes(a, (int)c->head_dim, be->sms);
   if (workspace_bytes < need || (need && !d_workspace))
     return fail(LRS_ERR_INVALID, "lrs_tree_attention: workspace of " + std::to_string(workspace_bytes) +

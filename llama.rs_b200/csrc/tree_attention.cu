@@ -387,7 +387,7 @@ struct TaTree {
     if (s == end) return true;  // no nodes: nothing else of it is looked at (padded batches)
     if (s < 0 || end < s || end > a.n_nodes || end - s > a.max_nodes || ctx < 0 || ctx > a.max_len ||
         end - s > a.max_len - ctx || seq < 0 || seq >= a.c.n_seqs) {
-      atomicExch(a.c.err, kErrCacheIndex);
+      atomicMax(a.c.err, kErrCacheIndex);
       return false;
     }
     n = end - s;
@@ -1290,7 +1290,7 @@ __global__ void __launch_bounds__(TaShape<HD, DT, NR>::kThreads, 1)
       }
     }
   }
-  if (!ok) atomicExch(a.c.err, LRS_ERR_DEVICE_TIMEOUT);
+  if (!ok) atomicMax(a.c.err, LRS_ERR_DEVICE_TIMEOUT);
   ta_fence_before();
   __syncthreads();
   if (warp == S::kWarpMma) {

@@ -118,3 +118,38 @@ def test_scores_of_minus_infinity(lrs, backend, ctx):
     v = cache.rows_of(0, ctx + n, 1)[0, ctx + 1]
     # one weight over itself: three sums that may truncate (2^-23), an inverse and a product (2^-24)
     assert (np.abs(got[1:] - v) <= 2.0 ** -21 * np.abs(v)).all()
+
+
+# ------------------------------------------------------- what is reported where --
+@pytest.mark.parametrize("stream", ["legacy", "backend", "side"])
+def test_skipped_entries_are_not_the_models(lrs, backend, stream):
+    """A row that kv_store skips fails neither a matvec nor a model's call, which would
+    withhold its result, and is still there for the next synchronize."""
+    import torch
+    cfg = lrs.LlamaConfig(512, 1024, 8, 4, 2, 2000, 1e-6, 1e6, 32768, 64, True)
+    sm = lrs.SynthModel(cfg, 5, lrs.LoadQuantization.Q4KM)
+    m = lrs.CudaQwen2Model(backend, sm.desc(), max_seq_len=256, max_sequences=2)
+    prompt = lrs.prompt_tokens(5, 70, cfg.vocab_size)
+    w = lrs.QuantTensor.quantize(np.ones(64 * 32, np.float32), 64, 32, lrs.QuantType.Q8_0)
+    calls = [lambda: backend.matvec_batched(w, np.ones((1, 32), np.float32)).tolist(),
+             lambda: m.prefill(prompt)[1], lambda: m.forward_token(3, 70)[1],
+             lambda: m.decode_greedy([3], [70], 4).tolist(), lambda: m.verify_tree([3, 4], [-1, 0], 74).tolist(),
+             lambda: m.accept_tree([0, 1], 74), lambda: m.forward_sample(3, 76, lrs.Sampler(), [1], 0.5)]
+    want = [call() for call in calls]
+    cache = Cache(lrs, "Q8_0", 2, 64, [70])
+    d_seq, d_pos, dx = dev([9], np.int32), dev([3], np.int32), dev(np.ones((2, 64), np.float32))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def skip():
+        at = {"legacy": 0, "backend": None, "side": side.cuda_stream}[stream]
+        backend.kv_store(cache.c, d_seq.data_ptr(), d_pos.data_ptr(), 1, dx.data_ptr(), dx.data_ptr(), stream=at)
+        torch.cuda.synchronize()
+
+    for call, expect in zip(calls, want):
+        skip()
+        assert call() == expect
+        with pytest.raises(lrs.LrsError, match="out of range") as e:
+            backend.synchronize()
+        assert e.value.code == 1
+        backend.synchronize()  # once
