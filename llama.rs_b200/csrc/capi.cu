@@ -605,8 +605,9 @@ KvView kv_view(const lrs_model* m, const Layer& L) {
 }
 
 // Attention arguments of `nodes` items, B one-node trees (a decode step) or one
-// tree (a prompt chunk: a chain; a verified tree: d_mask).
-TreeArgs tree_step(const lrs_model* m, const Layer& L, int B, bool one_tree, bool verify) {
+// tree (a prompt chunk: a chain; a verified tree: d_mask).  `len`: no item's
+// positions reach past it; the kernel's form is chosen by it.
+TreeArgs tree_step(const lrs_model* m, const Layer& L, int B, bool one_tree, bool verify, uint32_t len) {
   const lrs_config& c = m->c;
   TreeArgs t{};
   t.c = kv_view(m, L);
@@ -617,7 +618,7 @@ TreeArgs tree_step(const lrs_model* m, const Layer& L, int B, bool one_tree, boo
   t.n_trees = one_tree ? 1 : B;
   t.n_nodes = B;
   t.max_nodes = one_tree ? B : 1;
-  t.max_len = (int)m->opt.max_seq_len;
+  t.max_len = (int)len;
   t.q = m->q;
   t.out = m->att;
   t.q_ld = t.out_ld = (long long)c.num_attention_heads * c.head_dim;
@@ -632,9 +633,10 @@ TreeArgs tree_step(const lrs_model* m, const Layer& L, int B, bool one_tree, boo
 // `lm_item` >= 0 only that item runs the final norm + LM head (prefill);
 // lm_item == -1 runs it for every item; -2 skips it.
 // `verify`: the items are the nodes of one tree (d_cell / d_ctx / d_mask set, d_pos the
-// positions of their rotation).
+// positions of their rotation).  `len`: positions that the items reach, where the caller
+// knows them; a decode step's graph is launched at any position of the context.
 int32_t enqueue_step(lrs_model* m, int B, int lm_item, bool want_logits, bool greedy_advance,
-                     int n_steps_cap, bool verify = false) {
+                     int n_steps_cap, uint32_t len, bool verify = false) {
   const lrs_config& c = m->c;
   cudaStream_t st = m->be->stream;
   const int h = c.hidden_size, I = c.intermediate_size, nh = c.num_attention_heads,
@@ -745,8 +747,8 @@ int32_t enqueue_step(lrs_model* m, int B, int lm_item, bool want_logits, bool gr
       LRS_CUDA(launch_rope(m->q, m->k, m->rope_cos, m->rope_sin, m->d_pos, B, nh, nkv, hd, st));
       const KvStoreArgs sa{kv_view(m, L), m->d_seq, verify ? m->d_cell : m->d_pos, B, m->k, m->v, kvw};
       LRS_CUDA(launch_kv_store(sa, m->opt.kv_dtype, hd, sms, st));
-      LRS_CUDA(launch_tree_attention(tree_step(m, L, B, !fused_attn || verify, verify), m->opt.kv_dtype, hd,
-                                     sms, st));
+      LRS_CUDA(launch_tree_attention(tree_step(m, L, B, !fused_attn || verify, verify, len), m->opt.kv_dtype,
+                                     hd, sms, st));
     } else {
       if (!fused_attn)
         LRS_CUDA(launch_rope_store(m->q, m->k, m->v, m->rope_cos, m->rope_sin, io, B, nh, nkv, hd,
@@ -1319,7 +1321,8 @@ int32_t create_model(lrs_backend* be, const lrs_model_desc* d, const lrs_model_o
     size_t ws = 0;
     for (int one : {1, 0})
       ws = std::max(ws, tree_attention_workspace_bytes(
-                            tree_step(m.get(), m->layers[0], one ? LRS_TREE_MAX_NODES : (int)B, one != 0, false),
+                            tree_step(m.get(), m->layers[0], one ? LRS_TREE_MAX_NODES : (int)B, one != 0, false,
+                                      opt.max_seq_len),
                             (int)c.head_dim, be->sms));
     if ((rc = model_alloc(m.get(), (void**)&m->d_iota, (B + 1) * 4)) ||
         (rc = model_alloc(m.get(), (void**)&m->d_span, 2 * 4)) ||
@@ -1532,7 +1535,8 @@ lrs_status lrs_model_prefill(lrs_model* m, uint32_t seq, const uint32_t* tokens,
     }
     if ((rc = set_items(m, nb, tok.data(), pos.data(), sq.data(), m->opt.kv_dtype == LRS_KV_Q8_0))) return rc;
     const bool last = c0 + nb == n;
-    rc = enqueue_step(m, nb, last && want ? nb - 1 : -2, logits_out != nullptr, false, 0);
+    rc = enqueue_step(m, nb, last && want ? nb - 1 : -2, logits_out != nullptr, false, 0,
+                      (uint32_t)(start_pos + c0 + nb));
     if (rc) return rc;
   }
   if (logits_out)
@@ -1569,7 +1573,7 @@ lrs_status lrs_model_forward_sample(lrs_model* m, uint32_t seq, uint32_t token, 
   if ((rc = ensure_pages(m, (int)seq, pos))) return rc;
   int t = (int)token, p = (int)pos, s = (int)seq;
   if ((rc = set_items(m, 1, &t, &p, &s))) return rc;
-  if ((rc = enqueue_step(m, 1, 0, true, false, 0))) return rc;
+  if ((rc = enqueue_step(m, 1, 0, true, false, 0, pos + 1))) return rc;
   uint32_t *d_recent, *d_out;
   if ((rc = sample_buffers(m->be, recent, n_recent, &d_recent, &d_out))) return rc;
   LRS_CUDA(launch_sample(m->tp_world > 1 ? m->logits_full : m->logits, (int)m->vocab_full,
@@ -1642,7 +1646,7 @@ lrs_status lrs_model_verify_tree(lrs_model* m, uint32_t seq, const uint32_t* tok
   LRS_CUDA(cudaMemcpyAsync(m->d_ctx, &ctx, sizeof(int), cudaMemcpyHostToDevice, st));
   LRS_CUDA(cudaMemcpyAsync(m->d_mask, mask, n * sizeof(mask[0]), cudaMemcpyHostToDevice, st));
   if ((rc = set_items(m, (int)n, tok, pos, sq, true))) return rc;
-  if ((rc = enqueue_step(m, (int)n, -1, false, false, 0, true))) return rc;
+  if ((rc = enqueue_step(m, (int)n, -1, false, false, 0, start_pos + (uint32_t)n, true))) return rc;
   std::vector<unsigned long long> keys(n);
   LRS_CUDA(cudaMemcpyAsync(keys.data(), m->keys, n * sizeof(keys[0]), cudaMemcpyDeviceToHost, st));
   LRS_CUDA(cudaStreamSynchronize(st));
@@ -1750,7 +1754,7 @@ lrs_status lrs_model_decode_enqueue(lrs_model* m, size_t n_seqs, const uint32_t*
     if (it == m->graphs.end()) {
       cudaGraph_t graph;
       LRS_CUDA(cudaStreamBeginCapture(st, cudaStreamCaptureModeThreadLocal));
-      rc = step1 ? enqueue_step1(m) : enqueue_step(m, B, -1, false, true, cap_steps);
+      rc = step1 ? enqueue_step1(m) : enqueue_step(m, B, -1, false, true, cap_steps, m->opt.max_seq_len);
       cudaError_t e = cudaStreamEndCapture(st, &graph);
       if (rc) return rc;
       if (e != cudaSuccess) return fail(LRS_ERR_CUDA, std::string("graph capture: ") + cudaGetErrorString(e));
@@ -1776,7 +1780,7 @@ lrs_status lrs_model_decode_enqueue(lrs_model* m, size_t n_seqs, const uint32_t*
     for (size_t s = 0; s < n_steps; s++) LRS_CUDA(cudaGraphLaunch(exec, st));
   } else {
     for (size_t s = 0; s < n_steps; s++)
-      if ((rc = step1 ? enqueue_step1(m) : enqueue_step(m, B, -1, false, true, cap_steps))) return rc;
+      if ((rc = step1 ? enqueue_step1(m) : enqueue_step(m, B, -1, false, true, cap_steps, m->opt.max_seq_len))) return rc;
   }
   return LRS_OK;
 } catch (...) {
@@ -1827,7 +1831,7 @@ lrs_status lrs_model_profile_step(lrs_model* m, size_t n_seqs, const uint32_t* s
   cudaEventRecord(s0, st);
   m->prof = &ev;
   m->prof_attn = &aev;
-  rc = enqueue_step(m, B, -1, false, true, 0);
+  rc = enqueue_step(m, B, -1, false, true, 0, m->opt.max_seq_len);
   m->prof = nullptr;
   m->prof_attn = nullptr;
   cudaEventRecord(s1, st);
