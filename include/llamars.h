@@ -393,9 +393,12 @@ lrs_status lrs_tree_greedy_path(const uint32_t* tokens, const int32_t* parents,
                                 const uint32_t* argmax, size_t n, uint32_t* nodes_out,
                                 size_t* n_out, uint32_t* next_out);
 
-/* Keeps a path of the tree last verified at start_pos: its nodes' K and V move to
- * positions start_pos, start_pos + 1, ... in every layer, and the slot continues
- * at start_pos + n.  `nodes` ascends. */
+/* Keeps a path of the tree that the slot's last call verified, at start_pos: its
+ * nodes' K and V move to positions start_pos, start_pos + 1, ... in every layer, and
+ * the slot continues at start_pos + n.  The path starts at a node without a parent,
+ * and each node is the parent of the next (lrs_tree_greedy_path's is one).  Any other
+ * path is refused, and so is every path after another call has written positions of
+ * the slot (lrs_model_accept_tree of one of them included).  n = 0 does nothing. */
 lrs_status lrs_model_accept_tree(lrs_model* model, uint32_t seq, uint32_t start_pos,
                                  const uint32_t* nodes, size_t n);
 

@@ -876,8 +876,8 @@ class CudaQwen2Model:
         return out
 
     def accept_tree(self, nodes: Sequence[int], start_pos: int, seq: int = 0) -> None:
-        """Keeps a path of the tree verified at start_pos (lrs_model_accept_tree):
-        the slot continues at start_pos + len(nodes)."""
+        """Keeps a path of the tree that the slot's last call verified, at start_pos
+        (lrs_model_accept_tree): the slot continues at start_pos + len(nodes)."""
         n = np.ascontiguousarray(nodes, dtype=np.uint32)
         _check(_lib.lrs_model_accept_tree(self._h, seq, start_pos, _uptr(n), n.size))
 

@@ -406,6 +406,12 @@ struct lrs_model {
   int pages_per_seq = 0, total_pages = 0;
   std::vector<int> free_pages;
   std::vector<std::vector<int>> seq_pages;
+  // the tree that each slot holds since lrs_model_verify_tree (no parents: none)
+  struct Tree {
+    uint32_t start = 0;
+    std::vector<int32_t> parents;
+  };
+  std::vector<Tree> trees;
   int* d_pages = nullptr;
   // activations, for up to max_items items per step
   int max_items = 0, max_split = 64;
@@ -584,7 +590,10 @@ int nsplit_for(const lrs_model* m, int batch) {
   return std::max(1, std::min({want, m->max_split, maxs}));
 }
 
+// Before a step writes positions of a slot, up to last_pos: their pages are there,
+// and a tree that the slot held is no longer one to accept.
 int32_t ensure_pages(lrs_model* m, int seq, uint32_t last_pos) {
+  m->trees[seq].parents.clear();
   size_t need = last_pos / kPageSize + 1;
   auto& pg = m->seq_pages[seq];
   if (pg.size() >= need) return LRS_OK;
@@ -1290,6 +1299,7 @@ int32_t create_model(lrs_backend* be, const lrs_model_desc* d, const lrs_model_o
   }
   for (int pg = m->total_pages - 1; pg >= 0; pg--) m->free_pages.push_back(pg);
   m->seq_pages.resize(opt.max_sequences);
+  m->trees.resize(opt.max_sequences);
   if ((rc = model_alloc(m.get(), (void**)&m->d_pages,
                         (size_t)m->total_pages * sizeof(int))))
     return cleanup(rc);
@@ -1496,6 +1506,7 @@ lrs_status lrs_model_reset(lrs_model* m, uint32_t seq) try {
   // before they are read); here the slot's pages go back to the pool.
   for (int pg : m->seq_pages[seq]) m->free_pages.push_back(pg);
   m->seq_pages[seq].clear();
+  m->trees[seq].parents.clear();
   return LRS_OK;
 } catch (...) {
   return lrs::status_of_current_exception();
@@ -1652,6 +1663,8 @@ lrs_status lrs_model_verify_tree(lrs_model* m, uint32_t seq, const uint32_t* tok
   LRS_CUDA(cudaStreamSynchronize(st));
   if ((rc = check_device_error(m->be))) return rc;
   for (size_t i = 0; i < n; i++) argmax_out[i] = (uint32_t)(keys[i] & 0xffffffffull);
+  m->trees[seq].start = start_pos;
+  m->trees[seq].parents.assign(parents, parents + n);
   return LRS_OK;
 } catch (...) {
   return lrs::status_of_current_exception();
@@ -1662,11 +1675,16 @@ lrs_status lrs_model_accept_tree(lrs_model* m, uint32_t seq, uint32_t start_pos,
   if (!m || (n && !nodes)) return fail(LRS_ERR_INVALID, "null argument");
   if (seq >= m->opt.max_sequences) return fail(LRS_ERR_INVALID, "sequence slot out of range");
   if (n == 0) return LRS_OK;
+  lrs_model::Tree& tree = m->trees[seq];
+  if (tree.parents.empty() || tree.start != start_pos)
+    return fail(LRS_ERR_INVALID, "slot " + std::to_string(seq) + " holds no verified tree at position " +
+                                     std::to_string(start_pos));
   for (size_t i = 0; i < n; i++)
-    if (nodes[i] >= LRS_TREE_MAX_NODES || (i && nodes[i] <= nodes[i - 1]))
-      return fail(LRS_ERR_INVALID, "a path's nodes ascend, below " + std::to_string(LRS_TREE_MAX_NODES));
-  if (((size_t)start_pos + nodes[n - 1]) / kPageSize >= m->seq_pages[seq].size())
-    return fail(LRS_ERR_INVALID, "the path leaves the positions that slot " + std::to_string(seq) + " holds");
+    if (nodes[i] >= tree.parents.size() || tree.parents[nodes[i]] != (i ? (int32_t)nodes[i - 1] : -1))
+      return fail(LRS_ERR_INVALID, "node " + std::to_string(nodes[i]) + " does not follow " +
+                                       (i ? "node " + std::to_string(nodes[i - 1]) : "the committed positions") +
+                                       " in the verified tree of " + std::to_string(tree.parents.size()) + " nodes");
+  tree.parents.clear();  // its rows move
   LRS_CUDA(cudaSetDevice(m->be->device));
   cudaStream_t st = m->be->stream;
   const int head[4] = {(int)seq, (int)start_pos, 0, (int)n};

@@ -20,3 +20,47 @@ def test_a_prompt_does_not_depend_on_the_room(lrs, backend, hd):
     for other in got[1:]:
         for a, b in zip(got[0], other):
             assert np.array_equal(a, b)
+
+
+@pytest.mark.parametrize("kv", ["F32", "Q8_0"])
+def test_only_paths_of_the_verified_tree_are_accepted(lrs, backend, kv):
+    """A node past the tree, a node that its predecessor is not the parent of, another
+    start or slot, a tree already accepted or written over: refused, nothing moved."""
+    cfg, _, m = _model(lrs, backend, kv, 64)
+    prompt = lrs.prompt_tokens(5, 9, cfg.vocab_size)
+    tokens, parents = [5, 6, 7, 8, 9], [-1, 0, 0, 1, -1]
+
+    def refused(nodes, start=9, seq=0):
+        with pytest.raises(lrs.LrsError, match="tree") as e:
+            m.accept_tree(nodes, start, seq=seq)
+        assert e.value.code == 1
+
+    m.prefill(prompt, want_logits=False)
+    refused([0])  # nothing is verified yet
+    want = m.verify_tree(tokens, parents, 9)
+    for nodes in ([0, 5], [5], [63], [0, 3], [1], [1, 3], [0, 1, 2], [0, 0], [1, 0], [0, 4], [2 ** 32 - 1]):
+        refused(nodes)
+    for start, seq in ((8, 0), (10, 0), (9, 1)):
+        refused([0], start, seq)
+    m.accept_tree([], 9)
+    m.accept_tree([0, 1, 3], 9)  # the refused calls have not touched it
+    refused([0, 1])
+    # the kept rows are those of the tokens one after another
+    logits, _ = m.forward_token(11, 12)
+    m.prefill(list(prompt) + [5, 6, 8], seq=1, want_logits=False)
+    other, _ = m.forward_token(11, 12, seq=1)
+    assert np.abs(logits - other).max() < 2e-2
+    # whatever writes the slot's positions ends its tree; calls on other slots do not
+    for call in (lambda: m.prefill([1, 2], 9), lambda: m.forward_token(3, 9), lambda: m.decode_greedy([3], [9], 2),
+                 lambda: m.forward_sample(3, 9, lrs.Sampler(), [1], 0.5), lambda: m.reset(0),
+                 lambda: m.profile_step([3], [9])):
+        m.prefill(prompt, want_logits=False)
+        m.verify_tree(tokens, parents, 9)
+        call()
+        refused([0])
+    m.prefill(prompt, want_logits=False)
+    assert np.array_equal(m.verify_tree(tokens, parents, 9), want)
+    m.forward_token(3, 15, seq=1)
+    m.verify_tree([4, 4], [-1, -1], 20, seq=1)
+    m.accept_tree([4], 9)
+    m.accept_tree([1], 20, seq=1)
