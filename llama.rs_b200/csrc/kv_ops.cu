@@ -528,6 +528,13 @@ int32_t unaligned(const char* what) {
   return fail(LRS_ERR_INVALID, std::string(what) + ": an array is not aligned to its values");
 }
 
+// `n` rows `ld` floats apart lie in the address space (a negative stride of a
+// language with signed sizes arrives as one that does not).
+bool stride_fits(size_t n, size_t ld) { return n == 0 || ld <= ((size_t)1 << 45) / n; }
+int32_t bad_stride(const char* what, size_t ld) {
+  return fail(LRS_ERR_INVALID, std::string(what) + ": rows " + std::to_string(ld) + " values apart exceed the address space");
+}
+
 int32_t check_rows(const lrs_kv_cache* c, size_t n, size_t* ld, const char* what) {
   int32_t rc = lrs_kv_check(c, nullptr);
   if (rc) return rc;
@@ -537,6 +544,7 @@ int32_t check_rows(const lrs_kv_cache* c, size_t n, size_t* ld, const char* what
     return fail(LRS_ERR_INVALID, std::string(what) + ": row stride " + std::to_string(*ld) +
                                      " is below the row's " + std::to_string(width) + " values");
   if (n > (size_t)INT_MAX) return fail(LRS_ERR_INVALID, std::string(what) + ": too many rows");
+  if (!stride_fits(n, *ld)) return bad_stride(what, *ld);
   return LRS_OK;
 }
 
@@ -729,6 +737,7 @@ lrs_status lrs_tree_attention(lrs_backend* be, const lrs_kv_cache* c, const lrs_
   if (out_ld == 0) out_ld = width;
   if (q_ld < width || out_ld < width)
     return fail(LRS_ERR_INVALID, "lrs_tree_attention: row stride below the row's " + std::to_string(width) + " values");
+  if (!stride_fits(t->n_nodes, std::max(q_ld, out_ld))) return bad_stride("lrs_tree_attention", std::max(q_ld, out_ld));
   if (!std::isfinite(scale)) return fail(LRS_ERR_INVALID, "lrs_tree_attention: scale must be finite");
   if (t->n_trees == 0 || t->n_nodes == 0) return LRS_OK;
   if (!be || !d_q || !d_out) return fail(LRS_ERR_INVALID, "null argument");
