@@ -740,6 +740,9 @@ lrs_status lrs_tree_attention(lrs_backend* be, const lrs_kv_cache* c, const lrs_
   if (!stride_fits(t->n_nodes, std::max(q_ld, out_ld))) return bad_stride("lrs_tree_attention", std::max(q_ld, out_ld));
   if (!std::isfinite(scale)) return fail(LRS_ERR_INVALID, "lrs_tree_attention: scale must be finite");
   if (t->n_trees == 0 || t->n_nodes == 0) return LRS_OK;
+  // (a row is read before any CTA writes it only where both have the same place)
+  if (d_q && d_out == d_q && q_ld != out_ld)
+    return fail(LRS_ERR_INVALID, "lrs_tree_attention: out that is q must have q's row stride");
   if (!be || !d_q || !d_out) return fail(LRS_ERR_INVALID, "null argument");
   if (!aligned(d_q) || !aligned(d_out)) return unaligned("lrs_tree_attention");
   TreeArgs a = tree_args(*c, *t, n_heads, be->d_err + kErrQueued);

@@ -22,3 +22,10 @@ def test_wide_strides_are_taken(lrs):
     for call in (lambda: be.kv_store(c, A, A, 2, A, A, ld=2 ** 44), lambda: be.tree_attention(c, _trees(lrs), A, A, 4, q_ld=2 ** 43)):
         with pytest.raises(lrs.LrsError, match="null argument"):
             call()
+
+
+@pytest.mark.parametrize("q_ld,out_ld", [(0, 1024), (1024, 0), (600, 601)])
+def test_out_that_is_q_has_its_stride(lrs, q_ld, out_ld):
+    with pytest.raises(lrs.LrsError, match="stride") as e:
+        _Host(lrs).tree_attention(_cache(lrs), _trees(lrs), A, A, 4, q_ld=q_ld, out_ld=out_ld)
+    assert e.value.code == INVALID
