@@ -19,7 +19,7 @@ def test_strides_past_the_address_space_are_refused(lrs, ld):
 def test_wide_strides_are_taken(lrs):
     """Up to the address space: the calls get as far as the null backend."""
     c, be = _cache(lrs), _Host(lrs)
-    for call in (lambda: be.kv_store(c, A, A, 2, A, A, ld=2 ** 44), lambda: be.tree_attention(c, _trees(lrs), A, A, 4, q_ld=2 ** 43)):
+    for call in (lambda: be.kv_store(c, A, A, 2, A, A, ld=2 ** 44), lambda: be.tree_attention(c, _trees(lrs), A, 2 * A, 4, q_ld=2 ** 43)):
         with pytest.raises(lrs.LrsError, match="null argument"):
             call()
 
