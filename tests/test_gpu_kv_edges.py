@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 
 import kv_plain
+import kv_terms
 from test_gpu_kv import DTYPES, Cache, Trees, dev, sync_ok
 
 pytestmark = pytest.mark.gpu
@@ -153,3 +154,39 @@ def test_skipped_entries_are_not_the_models(lrs, backend, stream):
             backend.synchronize()
         assert e.value.code == 1
         backend.synchronize()  # once
+
+
+# ---------------------------------------------------------- products of terms --
+@pytest.mark.parametrize("hd,at,group,room", [(64, 0, 1, 0), (64, 35, 1, 0), (128, 40, 1, 0), (128, 97, 1, 0),
+                                              # rows and room that take units of 32 and of 64 rows
+                                              (64, 35, 20, 600), (128, 40, 20, 600), (64, 0, 60, 300), (128, 97, 60, 300)])
+@pytest.mark.parametrize("before", [0, 100, 300])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_each_product_of_terms_counts(lrs, backend, dtype, before, hd, at, group, room):
+    """Outputs that rest on one product each, to half of what losing it does.  What else
+    moves them: the sums of products 2^20 times the result at most, with 2^-23 of the
+    largest (an eighth of the result), and for the third term of P, 14 units of 2^-22
+    where the exponents' and exponentials' roundings make 3.4."""
+    import torch
+    cases = kv_terms.cases(dtype, hd, at)
+    for (part, a, b), case in cases.items():
+        q, k, v = kv_terms.padded(case, before, (at + 10) % hd)
+        n = len(k)
+        cache = Cache(lrs, dtype, 1, hd, [n], extra=room)
+        for which, rows in enumerate((k, v)):
+            for p in range(n):
+                cache.rows[which][cache.pages[0, p // 64], 0, p % 64] = rows[p]
+            cache.value[which] = kv_plain.held(lrs, cache.dtype, cache.rows[which])
+            cache.pool[which].copy_(dev(kv_plain.pack(lrs, cache.dtype, cache.rows[which], bool(which))))
+        trees = Trees(lrs, backend, cache, [(n - 1, 1)], group, max_len=max(n, room * 64))
+        trees.scale = kv_terms.SCALE
+        trees.qbuf[:hd * group] = np.tile(q, group)
+        trees.d["q"].copy_(dev(trees.qbuf))
+        torch.cuda.synchronize()
+        trees.run(backend)
+        sync_ok(backend)
+        got = trees.out.cpu().numpy()[:hd * group].reshape(group, hd)
+        kk, vv = (cache.rows_of(0, n, i) for i in range(2))
+        want, _ = kv_plain.attention(q.reshape(1, 1, hd), kk, vv, n - 1, [1], kv_terms.SCALE)
+        lost = kv_terms.emulate(dtype, q, kk[0], vv[0], *(((a, b),) if i == part else () for i in (0, 1)))
+        assert (np.abs(got - want.reshape(hd)) <= np.abs(lost - want.reshape(hd)) / 2).all(), (part, a, b)
