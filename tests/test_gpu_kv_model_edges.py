@@ -3,6 +3,7 @@ import numpy as np
 import pytest
 
 from test_gpu_kv_model import _model
+from test_plain_model import model as plain_case
 
 pytestmark = pytest.mark.gpu
 
@@ -64,3 +65,45 @@ def test_only_paths_of_the_verified_tree_are_accepted(lrs, backend, kv):
     m.verify_tree([4, 4], [-1, -1], 20, seq=1)
     m.accept_tree([4], 9)
     m.accept_tree([1], 20, seq=1)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("kv", ["BF16", "Q8_0"])
+def test_logits_are_the_cache_types(lrs, orc, backend, kv, hd):
+    """Prompt chunks and single tokens over a cache type against a 64-bit model whose rows
+    are held in it: within a third of what the type itself does to the logits, which the
+    f32 cache's are off by."""
+    cfg, sm, plain = plain_case(lrs, orc, hd)
+    tokens = [int(t) for t in lrs.prompt_tokens(5, 150, cfg.vocab_size)]
+    exact, held = (plain.logits(tokens, lrs.KvType[t]) for t in ("F32", kv))
+    m = lrs.CudaQwen2Model(backend, sm.desc(), max_seq_len=512, max_sequences=2, kv_dtype=lrs.KvType[kv])
+    for n in (64, 130, 150):
+        got, _ = m.prefill(tokens[:n])
+        effect = np.abs(held[n - 1] - exact[n - 1]).max()
+        assert np.abs(got - held[n - 1]).max() < effect / 3 < np.abs(got - exact[n - 1]).max()
+    for i, t in enumerate(tokens):
+        got, _ = m.forward_token(t, i, seq=1)
+        if i >= 20:  # (of few rows the effect is small)
+            effect = np.abs(held[i] - exact[i]).max()
+            assert np.abs(got - held[i]).max() < effect / 3, i
+
+
+@pytest.mark.parametrize("kv", ["F32", "BF16", "Q8_0"])
+def test_verified_nodes_are_the_64_bit_models(lrs, orc, backend, kv):
+    """Each node's token is the best of the path to it, or as near as the logits may be off:
+    for f32 1e-4 (test_plain_model), else a third of what the type does, on either side."""
+    cfg, sm, plain = plain_case(lrs, orc, 64)
+    rng = np.random.default_rng(8)
+    m = lrs.CudaQwen2Model(backend, sm.desc(), max_seq_len=512, max_sequences=1, kv_dtype=lrs.KvType[kv])
+    for ctx, n in ((3, 6), (120, 20), (200, 9)):
+        prompt = [int(t) for t in lrs.prompt_tokens(5, ctx, cfg.vocab_size)]
+        parents = [-1] + [int(rng.integers(0, i)) for i in range(1, n)]
+        tokens = [int(t) for t in rng.integers(0, cfg.vocab_size, n)]
+        m.prefill(prompt, want_logits=False)
+        got = m.verify_tree(tokens, parents, ctx)
+        paths = []
+        for i, p in enumerate(parents):
+            paths.append((paths[p] if p >= 0 else []) + [tokens[i]])
+            exact, held = (plain.logits(prompt + paths[i], lrs.KvType[t])[-1] for t in ("F32", kv))
+            tol = max(1e-4, np.abs(held - exact).max() / 3)
+            assert held.max() - held[got[i]] <= 2 * tol, (ctx, i)
