@@ -38,9 +38,13 @@ class PlainModel:
         a, b = x[..., :half], x[..., half:]
         return np.concatenate([a * np.cos(angle) - b * np.sin(angle), a * np.sin(angle) + b * np.cos(angle)], -1)
 
-    def logits(self, tokens, kv):
-        """[n, vocab]: the logits after each token, every K and V row held as `kv` holds it."""
+    def logits(self, tokens, kv, split=None):
+        """[n, vocab]: the logits after each token, every K and V row held as `kv` holds it;
+        `split` restates what a kernel's dot products make of a row of x."""
         n, eps, hold = len(tokens), self.cfg.rms_norm_eps, lambda x: kv_plain.held(self.lrs, kv, x.astype(np.float32))
+
+        def dot(x, w):
+            return (x if split is None else np.array([split(r.astype(np.float32)) for r in x])) @ w.T
 
         def norm(x, w):
             return x / np.sqrt((x * x).mean(-1, keepdims=True) + eps) * w
@@ -48,16 +52,16 @@ class PlainModel:
         pos, seen = np.arange(n), np.tril(np.ones((n, n), bool))
         for w in self.layers:
             y = norm(x, w["in_norm"])
-            q = self.rotate((y @ w["q"].T + w["qb"]).reshape(n, self.nh, self.hd), pos)
-            k = hold(self.rotate((y @ w["k"].T + w["kb"]).reshape(n, self.nkv, self.hd), pos))
-            v = hold((y @ w["v"].T + w["vb"]).reshape(n, self.nkv, self.hd))
+            q = self.rotate((dot(y, w["q"]) + w["qb"]).reshape(n, self.nh, self.hd), pos)
+            k = hold(self.rotate((dot(y, w["k"]) + w["kb"]).reshape(n, self.nkv, self.hd), pos))
+            v = hold((dot(y, w["v"]) + w["vb"]).reshape(n, self.nkv, self.hd))
             att = np.empty((n, self.nh, self.hd))
             for h in range(self.nh):
                 s = q[:, h] @ k[:, h * self.nkv // self.nh].T / np.sqrt(self.hd)
                 p = np.where(seen, np.exp(np.where(seen, s - np.where(seen, s, -np.inf).max(1, keepdims=True), 0.0)), 0.0)
                 att[:, h] = p / p.sum(1, keepdims=True) @ v[:, h * self.nkv // self.nh]
-            x = x + att.reshape(n, -1) @ w["o"].T
+            x = x + dot(att.reshape(n, -1), w["o"])
             y = norm(x, w["post_norm"])
-            g = y @ w["g"].T
-            x = x + (g / (1.0 + np.exp(-g)) * (y @ w["u"].T)) @ w["d"].T
-        return norm(x, self.norm) @ self.head.T
+            g = dot(y, w["g"])
+            x = x + dot(g / (1.0 + np.exp(-g)) * dot(y, w["u"]), w["d"])
+        return dot(norm(x, self.norm), self.head)

@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 
 from plain_model import PlainModel
+from test_x_split import split_b1, split_batched
 
 
 def model(lrs, orc, hd):
@@ -38,3 +39,17 @@ def test_a_cache_type_moves_the_logits_more_than_roundings(lrs, orc, kv, hd):
                   for layer in plain.layers]
     moved = np.abs(off.logits(prompt, lrs.KvType[kv])[-1] - held).max()
     assert 0 < 3 * moved < np.abs(held - exact).max()
+
+
+def test_what_the_split_of_x_does_to_the_logits(lrs, orc):
+    """The single-token dots see x in int8 pairs, off by up to 2^-16 of the largest of eight
+    (test_x_split): each logit is off by a sum of hundreds of such roundings, rms 1.6e-5 and
+    8e-5 at most over the 150,000 here.  4e-4, 25 times the rms, is the bar of f32 caches'
+    logits in the tests of the models.  The batched dots' split is 300 times finer."""
+    cfg = lrs.LlamaConfig(512, 1024, 8, 4, 2, 2048, 1e-6, 1e6, 4096, 64, False)
+    plain = PlainModel(lrs, orc, lrs.SynthModel(cfg, 11, lrs.LoadQuantization.Q4KM), cfg)
+    prompt = lrs.prompt_tokens(11, 74, cfg.vocab_size)
+    exact, single, batched = (plain.logits(prompt, lrs.KvType.F32, split) for split in (None, split_b1, split_batched))
+    assert 2e-5 < np.abs(single - exact).max() < 1e-4
+    assert np.sqrt(((single - exact) ** 2).mean()) < 2e-5
+    assert np.abs(batched - exact).max() < 1e-6
