@@ -61,17 +61,17 @@ __device__ __forceinline__ bool q8_codes(const float (&x)[8], float inv, uint32_
 // Rows [blockIdx.x * rows, + rows) of K (blockIdx.z = 0) or V (1) of head
 // blockIdx.y.  The rows' cells are looked up once, one row a thread; then a lane
 // owns eight consecutive columns, and a warp has kBatch rows' loads under way
-// before it encodes the first (the lookups and loads, not the arithmetic, are what
-// a row waits for).  Q8_0: four lanes share a block's maximum by shuffles (as
+// before it encodes the first.  Q8_0: four lanes share a block's maximum by shuffles (as
 // integers: a NaN or a value past the limit shows there and takes the block to the
 // slow form).  V interleaves four positions per word, so the codes of the
 // CTA's rows meet in shared memory and leave as 16-byte stores wherever four
 // consecutive rows are four aligned positions of one slot, and as single bytes
 // elsewhere (a decode step's rows, the ends of a run): byte stores never touch a
 // neighbouring position.
-// Bound by DRAM for many rows: 65,536 rows of 4 heads x 128 into q8_0 take 80 us, 4.3
-// TB/s of what is read and written (bf16 64 us, f32 90 us); by the launch and the
-// lookups for a decode step's (5 us together with the load).
+// 65,536 rows of 4 heads x 128, L2 flushed before: into f32 93 us and bf16 70 us, both 5.8
+// TB/s of what is read and written and near DRAM's rate; into q8_0 86 us, 4.0 TB/s, bound
+// by the encoding's instructions (the schedulers issue in 74 of 100 cycles, DRAM is at
+// 48 %).  A decode step's rows are the launch and the lookups (5 us together with the load).
 constexpr int kBatch = 2;
 
 template <int HD, int DT>
@@ -209,8 +209,10 @@ __global__ void __launch_bounds__(32 * kStoreWarps)
 // rows' cells are looked up once; then a thread takes four columns of a (row, head)
 // at a time, kLoadBatch of them under way together, neighbouring threads writing
 // neighbouring heads of a row.  The lines that four positions share (V codes, K's
-// 16-byte chunks) come from L2 once.  65,536 rows of 4 heads x 128 from q8_0: 77 us,
-// 4.4 TB/s; from bf16 93 us, f32 88 us.
+// 16-byte chunks) come from L2 once.  65,536 rows of 4 heads x 128, L2 flushed before:
+// from f32 92 us, 5.8 TB/s, near DRAM's rate; from q8_0 82 us, 4.2 TB/s, bound by
+// instructions (66 of 100 cycles issue, DRAM 45 %); from bf16 94 us, 4.3 TB/s, waiting for
+// its loads (15 of a warp's 23 cycles an instruction), of 8 bytes a lane where f32's are 16.
 constexpr int kLoadRows = 32, kLoadThreads = 256, kLoadBatch = 4;
 
 template <int HD, int DT>

@@ -41,15 +41,18 @@
 // rescaling of O run only in the tiles that raise it (the first one, mostly).
 //
 // What bounds it.  64 trees of 8 nodes on 2,100 to 4,100 positions, q8_0, 4 KV heads
-// of 7 queries, 128 wide: 114 us, 2.0 TB/s of the cache's bytes and 0.53 PFLOP/s of the
-// three products; 4 trees of 64 nodes on 7,200 to 8,200: 113 us, 0.75 PFLOP/s.  A tile
-// takes some 3,000 clocks, of which the tensor pipe needs 1,536 and the copies, at DRAM's
+// of 7 queries, 128 wide: 114 us (104 back to back), 2.0 TB/s of the cache's bytes and 0.53
+// PFLOP/s of the three products; 4 trees of 64 nodes on 7,200 to 8,200: 114 us, 0.75 PFLOP/s.
+// A tile takes some 3,000 clocks, of which the tensor pipe needs 1,536 and the copies, at DRAM's
 // rate, 1,476; the schedulers issue in 65 of 100 clocks.  So the bound is the instructions
 // of decoding (a lane's 128 values of K or V take some 450) and of the softmax, whose
 // warps make 8 to 12 clocks an instruction beside one another.  A CTA spends some 15,000
 // clocks before its first product (the schedule, cold instruction fetches, q) and after
 // its last one: small calls are that and the launch (5 nodes on 100 positions, bf16, 12.3
-// us; a decode step of 64 sequences at 700 to 1,100, q8_0, 35 us).
+// us; a decode step of 64 sequences at 700 to 1,100, q8_0, 35 us).  bf16 and f32 caches,
+// which need less decoding or more bytes, take longer (64 x 8 in bf16 228 us, 32 x 8 in f32
+// 151): their warps mostly wait (the schedulers issue in 27 and 35 of 100 cycles, DRAM is at
+// 22 and 36 %, the tensor pipe at 14 and 24 %).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -79,8 +82,8 @@ struct TaShape {
   static constexpr int kA = DT == LRS_KV_F32 ? 3 : DT == LRS_KV_BF16 ? 1 : 2;  // terms of K, V
   static constexpr int kB = DT == LRS_KV_Q8_0 ? 2 : 3;                        // terms of q, P
   static constexpr bool kF16 = DT == LRS_KV_Q8_0;
-  // Groups of four warps: K, V (up to 32 rows two, half of the positions each: a decode
-  // step of 64 sequences 41 us, with one 45; at 64 rows the threads are spent), the
+  // Groups of four warps: K, V (up to 32 rows two, half of the positions each: they took
+  // 9 % off a decode step of 64 sequences; at 64 rows the threads are spent), the
   // softmax (16 rows each: groups of 32 took the same time at 64 rows, and would be half
   // idle below), O; then a warp each for K's copies, V's and the MMAs.
   static constexpr int kSG = NR / 16, kVG = NR == 64 ? 1 : 2;
@@ -1338,10 +1341,11 @@ long long tiles_of(const TreeArgs& a, int nr) {
 
 // Rows a unit: 16 while that gives a CTA two tiles at most, as the 16-row kernel starts
 // and ends sooner; else the smallest of 16, 32, 64 that holds a tree's rows, as each unit
-// decodes K and V for itself.  Measured with 16 / 32 / 64 rows, q8_0, 4 KV heads x 7 x 128:
-// 8 nodes on 1,100 positions 16.5 / 16.6 / 20.3 us, 5 on 3,000 19.9 / 22.2 / 24.8 us, 64
-// trees of one node on 700 to 1,100 34 / 38 / 41 us, but 64 of 8 on 2,100 to 4,100 221 /
-// 158 / 107 us; 8 of 13, f32, 2 x 6 x 128, on 1,500 to 2,050 78 / 53 / 55 us.
+// decodes K and V for itself.  Measured back to back with 16 / 32 / 64 rows, 4 KV heads x 7
+// x 128: q8_0, 8 nodes on 1,100 positions 14.5 / 14.5 / 18.3 us, 5 on 3,000 17.6 / 18.6 /
+// 20.7 us, 64 trees of one node on 700 to 1,100 35 / 37 / 41 us, but 64 of 8 on 2,100 to
+// 4,100 216 / 145 / 104 us; bf16, 64 of one 76 / 76 / 80 us, 64 of 8 695 / 395 / 224 us; f32,
+// 2 x 6 x 128, 8 of 13 on 1,500 to 2,050 64 / 43 / 43 us.
 int unit_rows(const TreeArgs& a, int sms) {
   const int rows = a.max_nodes * a.group;
   return rows <= 16 || tiles_of(a, 16) <= 2ll * sms ? 16 : rows <= 32 ? 32 : 64;
