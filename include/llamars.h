@@ -357,7 +357,8 @@ typedef struct lrs_tree_batch {
  * infinite; a non-finite value that it does attend to, or that q holds, makes its
  * outputs non-finite (all of the row's, if the value belongs to another node),
  * but that an infinity in K may count as the score of -inf that it makes, a weight
- * of zero; scores that are all -inf give NaN.
+ * of zero; scores that are all -inf give NaN.  The sums are f32 sums of V times
+ * weights up to 2^15: V past 2^80 that a node attends to may overflow them.
  * `d_workspace` (16-byte aligned, lrs_tree_attention_workspace bytes, contents
  * free; a batch with no field above another's needs no more than that one) is in
  * use until the work has finished: calls that may overlap, and graphs that may

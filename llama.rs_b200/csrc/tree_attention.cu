@@ -344,8 +344,10 @@ struct TaRing {
   }
 };
 
-// Two f32 values as `TERMS` 16-bit pairs whose sum they are (to 2^-22, 2^-24).
-template <bool F16, int TERMS>
+// Two f32 values as `TERMS` 16-bit pairs whose sum they are (to 2^-22, 2^-24).  LARGE: up
+// to f32's largest, which round to bf16's infinity: there the first term is bf16's largest
+// value and the second one the rest (an infinity leaves an infinity and a NaN).
+template <bool F16, int TERMS, bool LARGE = false>
 __device__ __forceinline__ void ta_split(float2 v, uint32_t (&t)[TERMS]) {
 #pragma unroll
   for (int i = 0; i < TERMS; i++) {
@@ -354,8 +356,12 @@ __device__ __forceinline__ void ta_split(float2 v, uint32_t (&t)[TERMS]) {
       t[i] = *reinterpret_cast<const uint32_t*>(&h);
       if (i + 1 < TERMS) v = add2(v, make_float2(-__low2float(h), -__high2float(h)));
     } else {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
-      t[i] = *reinterpret_cast<const uint32_t*>(&h);
+      if (LARGE && i == 0) {
+        asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(t[i]) : "f"(v.y), "f"(v.x));
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+        t[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
       if (i + 1 < TERMS)
         v = add2(v, make_float2(-__uint_as_float(t[i] << 16), -__uint_as_float(t[i] & 0xffff0000u)));
     }
@@ -515,10 +521,10 @@ __device__ __forceinline__ void decode_k(const uint8_t* raw, uint32_t at, int r,
         for (int i = 0; i < 4; i++) {
           const float4 f = *reinterpret_cast<const float4*>(row + b * 64 + i * 16);
           uint32_t y[S::kA];
-          ta_split<false, S::kA>(make_float2(f.x, f.y), y);
+          ta_split<false, S::kA, true>(make_float2(f.x, f.y), y);
 #pragma unroll
           for (int k = 0; k < S::kA; k++) x[k][i * 2] = y[k];
-          ta_split<false, S::kA>(make_float2(f.z, f.w), y);
+          ta_split<false, S::kA, true>(make_float2(f.z, f.w), y);
 #pragma unroll
           for (int k = 0; k < S::kA; k++) x[k][i * 2 + 1] = y[k];
         }
@@ -575,7 +581,7 @@ __device__ __forceinline__ void decode_v(const uint8_t* raw, uint32_t col, int w
         } else {
           const float* f = reinterpret_cast<const float*>(raw) + r * HD + h;
           uint32_t y[S::kA];
-          ta_split<false, S::kA>(make_float2(f[0], f[HD]), y);
+          ta_split<false, S::kA, true>(make_float2(f[0], f[HD]), y);
 #pragma unroll
           for (int q = 0; q < S::kA; q++) x[q][i] = y[q];
         }
@@ -674,7 +680,7 @@ __device__ __forceinline__ void load_q(const TreeArgs& a, const TaUnit& it, uint
         float2 v = mul2(make_float2(x[j][2 * e], x[j][2 * e + 1]), make_float2(f0, f0));
         if constexpr (S::kF16) v = mul2(v, make_float2(f1, f1));
         uint32_t z[S::kB];
-        ta_split<S::kF16, S::kB>(v, z);
+        ta_split<S::kF16, S::kB, true>(v, z);
 #pragma unroll
         for (int k = 0; k < S::kB; k++) y[k][e] = z[k];
       }

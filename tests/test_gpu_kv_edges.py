@@ -190,3 +190,40 @@ def test_each_product_of_terms_counts(lrs, backend, dtype, before, hd, at, group
         want, _ = kv_plain.attention(q.reshape(1, 1, hd), kk, vv, n - 1, [1], kv_terms.SCALE)
         lost = kv_terms.emulate(dtype, q, kk[0], vv[0], *(((a, b),) if i == part else () for i in (0, 1)))
         assert (np.abs(got - want.reshape(hd)) <= np.abs(lost - want.reshape(hd)) / 2).all(), (part, a, b)
+
+
+# ------------------------------------------------------- the ends of the types --
+@pytest.mark.parametrize("value", [3.4028234663852886e38, -3.4028234663852886e38, 3.3961775e38])
+@pytest.mark.parametrize("ctx", [61, 2000])
+@pytest.mark.parametrize("dtype", ["F32", "BF16"])
+def test_the_largest_values_in_masked_places(lrs, backend, dtype, ctx, value):
+    """The type's largest K and V at a node reach only the rows that attend to it; K's
+    with a query that is zero there is a score of zero."""
+    n, bad = 8, 5
+    cache = Cache(lrs, dtype, 2, 128, [ctx + n])
+    trees = Trees(lrs, backend, cache, [(ctx, n)], 3, seed=4)
+    for i in range(6, 8):
+        trees.masks[0][i] = 1 << i | 1 << 2
+    trees.d["mask"][:n].copy_(dev(np.array(trees.masks[0], np.uint64)))
+    trees.qbuf[77::128] = 0.0
+    trees.d["q"].copy_(dev(trees.qbuf))
+    p = ctx + bad
+    bf16_max = float(np.sign(value) * 3.3895313892515355e38)
+    for which, col in ((0, 77), (1, 40)):
+        at = cache.pages[0, p // 64], slice(None), p % 64, col
+        cache.rows[which][at] = value if dtype == "F32" else bf16_max
+        cache.value[which] = kv_plain.held(lrs, cache.dtype, cache.rows[which])
+        outside = ~np.broadcast_to(cache.inside[:, None], cache.rows[which].shape[:3])
+        t = kv_plain.pack(lrs, cache.dtype, cache.rows[which], bool(which))
+        cache.pool[which].copy_(dev(np.where(cache.marks(outside, bool(which)), 0xff, t).astype(np.uint8)))
+    trees.run(backend)
+    sync_ok(backend)
+    got = trees.out.cpu().numpy()[:n * trees.out_ld].reshape(n, 6, 128)
+    k, v = (cache.rows_of(0, ctx + n, i) for i in range(2))
+    seen = [i for i in range(n) if trees.masks[0][i] >> bad & 1]
+    assert seen and len(seen) < n
+    for rows, cols in ((sorted(set(range(n)) - set(seen)), range(128)), (seen, [c for c in range(128) if c != 40])):
+        vv = v[..., list(cols)]
+        want, err = kv_plain.attention(trees.q(0), k, vv, ctx, trees.masks[0], trees.scale)
+        for i in rows:
+            assert (np.abs(got[i][:, list(cols)] - want[i]) <= err[i]).all(), i
