@@ -227,3 +227,81 @@ def test_the_largest_values_in_masked_places(lrs, backend, dtype, ctx, value):
         want, err = kv_plain.attention(trees.q(0), k, vv, ctx, trees.masks[0], trees.scale)
         for i in rows:
             assert (np.abs(got[i][:, list(cols)] - want[i]) <= err[i]).all(), i
+
+
+# --------------------------------------------------- calls that the header allows --
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("ctx", [0, 90, 1000])
+def test_masks_of_any_nodes(lrs, backend, dtype, ctx):
+    """A mask may name any nodes of the tree, later ones too, and leave out the node itself."""
+    rng = np.random.default_rng(ctx)
+    s = [(ctx, 64), (ctx // 2, 17)]
+    cache = Cache(lrs, dtype, 1, 64, [c + n for c, n in reversed(s)])
+    trees = Trees(lrs, backend, cache, s, 5)
+    trees.masks = [[int(m) & (1 << n) - 1 for m in rng.integers(0, 2 ** 64, n, dtype=np.uint64)] for _, n in s]
+    trees.masks[0][3] = 1 << 63
+    trees.d["mask"][:81].copy_(dev(np.array([m for t in trees.masks for m in t], np.uint64)))
+    trees.run(backend)
+    sync_ok(backend)
+    trees.check()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_trees_that_share_a_slot(lrs, backend, dtype):
+    """Several trees on one slot, from different committed lengths, overlapping."""
+    s = [(700, 3), (100, 5), (700, 3), (698, 5)]
+    cache = Cache(lrs, dtype, 2, 128, [703])
+    cache.pages = np.repeat(cache.pages, 4, axis=0)  # (the class gives each tree a slot)
+    trees = Trees(lrs, backend, cache, s, 3)
+    trees.d["seq"].fill_(0)
+    trees.run(backend)
+    sync_ok(backend)
+    trees.check()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-30, -3.0])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_scales(lrs, backend, dtype, scale):
+    s = [(300, 4), (0, 3)]
+    cache = Cache(lrs, dtype, 1, 64, [c + n for c, n in reversed(s)])
+    trees = Trees(lrs, backend, cache, s, 4)
+    trees.scale = scale
+    trees.run(backend)
+    sync_ok(backend)
+    trees.check()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_widest_rows(lrs, backend, dtype):
+    """64 nodes of 64 query heads a KV head: 64 units of 64 rows each."""
+    s = [(130, 64), (1, 33)]
+    cache = Cache(lrs, dtype, 1, 64, [c + n for c, n in reversed(s)])
+    trees = Trees(lrs, backend, cache, s, 64)
+    trees.run(backend)
+    sync_ok(backend)
+    trees.check()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_two_calls_under_way(lrs, backend, dtype):
+    """Calls of two host threads on streams of their own, a workspace each."""
+    import threading
+
+    import torch
+    s = [(900, 9), (30, 4), (400, 20)]
+    cache = Cache(lrs, dtype, 2, 64, [c + n for c, n in reversed(s)])
+    both = [Trees(lrs, backend, cache, s, 7, seed=i) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in both]
+    torch.cuda.synchronize()
+
+    def work(i):
+        for _ in range(20):
+            both[i].run(backend, stream=streams[i].cuda_stream)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    sync_ok(backend)
+    for t in both:
+        t.check()

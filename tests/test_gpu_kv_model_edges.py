@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from test_gpu_kv_model import _model
+from test_gpu_kv_model import _model, _near_best
 from test_plain_model import model as plain_case
 
 pytestmark = pytest.mark.gpu
@@ -107,3 +107,56 @@ def test_verified_nodes_are_the_64_bit_models(lrs, orc, backend, kv):
             exact, held = (plain.logits(prompt + paths[i], lrs.KvType[t])[-1] for t in ("F32", kv))
             tol = max(1e-4, np.abs(held - exact).max() / 3)
             assert held.max() - held[got[i]] <= 2 * tol, (ctx, i)
+
+
+def test_a_persistent_step_continues_an_accepted_tree(lrs, backend):
+    """Decoding in one kernel a step, before and after trees verified by several."""
+    cfg, _, m = _model(lrs, backend, "F32", 64, persistent_decode=True)
+    _, _, plain = _model(lrs, backend, "F32", 64)
+    prompt = lrs.prompt_tokens(5, 60, cfg.vocab_size)
+    got = []
+    for x in (m, plain):
+        x.prefill(prompt, want_logits=False)
+        a = x.decode_greedy([7], [60], 4)[:, 0]
+        tree = [int(a[-1]), 5, 9, 5]
+        x.verify_tree(tree, [-1, 0, 0, 2], 64)
+        x.accept_tree([0, 2, 3], 64)
+        logits, _ = x.forward_token(11, 67)
+        got.append((a, logits, x.decode_greedy([12], [68], 4)[:, 0]))
+    assert np.array_equal(got[0][0], got[1][0]) and np.array_equal(got[0][2], got[1][2])
+    assert np.abs(got[0][1] - got[1][1]).max() < 4e-4
+
+
+@pytest.mark.parametrize("kv", ["F32", "Q8_0"])
+def test_the_last_positions_of_a_slot(lrs, orc, backend, kv):
+    """A full tree that ends at the context's end; a chunk of one token behind one of 64."""
+    cfg, sm, plain = plain_case(lrs, orc, 64)
+    m = lrs.CudaQwen2Model(backend, sm.desc(), max_seq_len=129, max_sequences=1, kv_dtype=lrs.KvType[kv])
+    tokens = [int(t) for t in lrs.prompt_tokens(5, 129, cfg.vocab_size)]
+
+    def tol(n):
+        exact, held = (plain.logits(tokens[:n], lrs.KvType[t]) for t in ("F32", kv))
+        return held, max(4e-4, np.abs(held[-1] - exact[-1]).max() / 3)
+    held, bar = tol(129)
+    for n in (65, 129):
+        assert np.abs(m.prefill(tokens[:n])[0] - held[n - 1]).max() < bar
+    m.prefill(tokens[:65], want_logits=False)
+    got = m.verify_tree(tokens[65:], list(range(-1, 63)), 65)
+    for i in range(64):
+        assert held[65 + i].max() - held[65 + i][got[i]] <= 2 * bar
+    m.accept_tree(list(range(64)), 65)
+    with pytest.raises(lrs.LrsError, match="exceeds"):
+        m.verify_tree([1, 2], [-1, 0], 128)
+
+
+def test_a_batch_of_more_sequences_than_a_chunk(lrs, backend):
+    """q8_0 decode steps of 70 sequences of ragged lengths, each as it decodes alone."""
+    cfg, _, m = _model(lrs, backend, "Q8_0", 64, seqs=70, max_seq=256)
+    lens = [3 + 2 * i for i in range(70)]
+    first = []
+    for i, n in enumerate(lens):
+        first.append(int(m.prefill(lrs.prompt_tokens(40 + i, n, cfg.vocab_size), seq=i)[1]))
+    got = m.decode_greedy(first, lens, 6)
+    for i in (0, 1, 33, 63, 64, 69):
+        logits, _ = m.forward_token(first[i], lens[i], seq=i)
+        assert _near_best(logits, int(got[0, i]), 1e-3)
