@@ -100,6 +100,7 @@ int32_t check_device_error(lrs_backend* be, int word = kErrOwn) {
   int h = 0;
   LRS_CUDA(cudaMemcpy(&h, be->d_err + word, sizeof(int), cudaMemcpyDeviceToHost));
   if (h) {
+    std::lock_guard<std::mutex> lock(be->taking);  // the place it is taken to is one
     LRS_CUDA(launch_take_error(be->d_err + word, be->d_err + kErrTaken, be->stream));
     LRS_CUDA(cudaMemcpyAsync(&h, be->d_err + kErrTaken, sizeof(int), cudaMemcpyDeviceToHost, be->stream));
     LRS_CUDA(cudaStreamSynchronize(be->stream));

@@ -4,6 +4,7 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <mutex>
 
 // The backend's error words: what its own work left (matvecs, the sampler, the
 // models' steps), what the operators that callers queue left, and the place that a
@@ -15,6 +16,7 @@ struct lrs_backend {
   int sms = 148;
   cudaStream_t stream = nullptr;
   int* d_err = nullptr;  // [kErrWords]
+  std::mutex taking;     // of the host thread that takes a word
   float* d_x = nullptr;
   float* d_y = nullptr;
   size_t x_cap = 0, y_cap = 0;

@@ -305,3 +305,30 @@ def test_two_calls_under_way(lrs, backend, dtype):
     sync_ok(backend)
     for t in both:
         t.check()
+
+
+def test_one_of_two_threads_reports_a_skipped_entry(lrs, backend):
+    """Two threads that synchronize at once: an entry skipped before is reported by one."""
+    import threading
+
+    import torch
+    cache = Cache(lrs, "F32", 1, 64, [64])
+    d_seq, d_pos, dx = dev([9], np.int32), dev([3], np.int32), dev(np.ones(64, np.float32))
+    torch.cuda.synchronize()
+    for _ in range(300):
+        backend.kv_store(cache.c, d_seq.data_ptr(), d_pos.data_ptr(), 1, dx.data_ptr(), dx.data_ptr(), stream=0)
+        torch.cuda.synchronize()
+        codes, gate = [], threading.Barrier(2)
+
+        def report():
+            gate.wait()
+            try:
+                backend.synchronize()
+            except lrs.LrsError as e:
+                codes.append(e.code)
+        threads = [threading.Thread(target=report) for _ in range(2)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert codes == [1]
