@@ -73,7 +73,8 @@ void lrs_backend_destroy(lrs_backend* backend);
 const char* lrs_backend_name(const lrs_backend* backend);
 /* KernelBackend::threads (src/backend.rs:71): the device's SM count. */
 size_t lrs_backend_threads(const lrs_backend* backend);
-/* Blocks until all work queued by this backend has finished. */
+/* Blocks until all work queued on the backend's stream has finished, and returns an
+ * error that the backend's work, or an operator on a caller's stream, has left. */
 lrs_status lrs_backend_synchronize(lrs_backend* backend);
 
 /* --------------------------------------------------------------- tensor -- */

@@ -95,17 +95,21 @@ const NcclApi& nccl() {
       return fail(LRS_ERR_CUDA, std::string("NCCL: ") + nccl().GetErrorString(r_));        \
   } while (0)
 
-// What one of the backend's error words holds, which is clear then.
-int32_t check_device_error(lrs_backend* be, int word = kErrOwn) {
-  int h = 0;
-  LRS_CUDA(cudaMemcpy(&h, be->d_err + word, sizeof(int), cudaMemcpyDeviceToHost));
-  if (h) {
+// What the backend's own error word holds, or (queued) else the operators', which is
+// clear then.
+int32_t check_device_error(lrs_backend* be, bool queued = false) {
+  static_assert(kErrOwn == 0 && kErrQueued == 1, "read by one copy");
+  int h[2] = {0, 0};
+  LRS_CUDA(cudaMemcpy(h, be->d_err, (queued ? 2 : 1) * sizeof(int), cudaMemcpyDeviceToHost));
+  for (int word = 0; word < 2; word++) {
+    if (!h[word]) continue;
+    int got = 0;
     std::lock_guard<std::mutex> lock(be->taking);  // the place it is taken to is one
     LRS_CUDA(launch_take_error(be->d_err + word, be->d_err + kErrTaken, be->stream));
-    LRS_CUDA(cudaMemcpyAsync(&h, be->d_err + kErrTaken, sizeof(int), cudaMemcpyDeviceToHost, be->stream));
+    LRS_CUDA(cudaMemcpyAsync(&got, be->d_err + kErrTaken, sizeof(int), cudaMemcpyDeviceToHost, be->stream));
     LRS_CUDA(cudaStreamSynchronize(be->stream));
-    if (h == 0) return LRS_OK;  // another thread's call has reported it
-    if (h == kErrCacheIndex)
+    if (got == 0) continue;  // another thread's call has reported it
+    if (got == kErrCacheIndex)
       return fail(LRS_ERR_INVALID,
                   "a KV cache operator skipped a slot, position, page, node or length out of range");
     return fail(LRS_ERR_DEVICE_TIMEOUT, "a bounded device-side wait gave up (TMA copy not completed)");
@@ -252,8 +256,7 @@ lrs_status lrs_backend_synchronize(lrs_backend* be) try {
   if (!be) return fail(LRS_ERR_INVALID, "null backend");
   LRS_CUDA(cudaSetDevice(be->device));
   LRS_CUDA(cudaStreamSynchronize(be->stream));
-  int32_t rc = check_device_error(be);
-  return rc ? rc : check_device_error(be, kErrQueued);
+  return check_device_error(be, true);
 } catch (...) {
   return lrs::status_of_current_exception();
 }
