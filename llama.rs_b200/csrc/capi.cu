@@ -1738,9 +1738,10 @@ lrs_status lrs_model_decode_enqueue(lrs_model* m, size_t n_seqs, const uint32_t*
     tok[i] = (int)first_tokens[i];
     pos[i] = (int)start_pos[i];
     sq[i] = (int)seqs[i];
-    int32_t rc = ensure_pages(m, sq[i], start_pos[i] + (uint32_t)n_steps - 1);
-    if (rc) return rc;
   }
+  int32_t rc;
+  for (int i = 0; i < B; i++)
+    if ((rc = ensure_pages(m, sq[i], start_pos[i] + (uint32_t)n_steps - 1))) return rc;
   // tokens_out: [n_steps][B]; row s holds the token step s produced.
   size_t need = n_steps * (size_t)B;
   if (need > m->tokens_out_cap) {
@@ -1755,8 +1756,7 @@ lrs_status lrs_model_decode_enqueue(lrs_model* m, size_t n_seqs, const uint32_t*
       return fail(LRS_ERR_OOM, "token buffer allocation failed");
     m->tokens_out_cap = cap;
   }
-  int32_t rc = set_items(m, B, tok.data(), pos.data(), sq.data());
-  if (rc) return rc;
+  if ((rc = set_items(m, B, tok.data(), pos.data(), sq.data()))) return rc;
   cudaStream_t st = m->be->stream;
   LRS_CUDA(cudaMemsetAsync(m->d_step, 0, 4, st));
   const int cap_steps = (int)(m->tokens_out_cap / B);
@@ -1840,11 +1840,11 @@ lrs_status lrs_model_profile_step(lrs_model* m, size_t n_seqs, const uint32_t* s
     tok[i] = (int)tokens[i];
     ps[i] = (int)pos[i];
     sq[i] = (int)seqs[i];
-    int32_t rc = ensure_pages(m, sq[i], pos[i]);
-    if (rc) return rc;
   }
-  int32_t rc = set_items(m, B, tok.data(), ps.data(), sq.data());
-  if (rc) return rc;
+  int32_t rc;
+  for (int i = 0; i < B; i++)
+    if ((rc = ensure_pages(m, sq[i], pos[i]))) return rc;
+  if ((rc = set_items(m, B, tok.data(), ps.data(), sq.data()))) return rc;
   cudaStream_t st = m->be->stream;
   std::vector<cudaEvent_t> ev, aev;
   cudaEvent_t s0, s1;

@@ -160,3 +160,16 @@ def test_a_batch_of_more_sequences_than_a_chunk(lrs, backend):
     for i in (0, 1, 33, 63, 64, 69):
         logits, _ = m.forward_token(first[i], lens[i], seq=i)
         assert _near_best(logits, int(got[0, i]), 1e-3)
+
+
+def test_refused_calls_leave_the_verified_tree(lrs, backend):
+    """A batch that is refused for another item has written nothing."""
+    cfg, _, m = _model(lrs, backend, "F32", 64)
+    m.prefill(lrs.prompt_tokens(5, 9, cfg.vocab_size), want_logits=False)
+    m.verify_tree([5, 6], [-1, 0], 9)
+    for call in (lambda: m.decode_greedy([3, 3], [9, 9], 2, [0, 99]), lambda: m.decode_greedy([3, 3], [9, 600], 2, [0, 1]),
+                 lambda: m.decode_greedy([3, 3], [9, 9], 2, [0, 0]), lambda: m.profile_step([3, 3], [9, 9], [0, 99]),
+                 lambda: m.prefill([cfg.vocab_size], 9), lambda: m.verify_tree([5], [0], 9)):
+        with pytest.raises(lrs.LrsError):
+            call()
+    m.accept_tree([0, 1], 9)
