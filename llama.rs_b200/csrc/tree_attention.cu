@@ -695,7 +695,7 @@ __device__ __forceinline__ void load_q(const TreeArgs& a, const TaUnit& it, uint
 // The copies of K's or V's raw tiles into their ring, by one warp each: they take
 // turns of some 100 instructions a slot, at a pace of 10 clocks and more beside the other
 // warps (one warp for both was what f32 caches waited for: 8 trees of 13 nodes on 1,550 to 2,050
-// positions took 54 us, now 43).
+// positions took 54 us, now 42).
 template <int HD, int DT, int NR, bool V>
 struct TaCopy {
   using S = TaShape<HD, DT, NR>;
